@@ -377,6 +377,128 @@ jfh_status jfh_engine_profile_batch(jfh_engine * engine, jfh_session * const * s
                                     uint32_t iterations, jfh_kernel_stat * out, uint32_t capacity,
                                     uint32_t * out_count);
 
+/* ---------------------------------------------------------------- operators on a paged cache */
+
+/* Operators of a decoder layer on the caller's device memory, for serving code
+ * that keeps its K/V caches in pages (no counterpart in the reference, whose
+ * sessions own one contiguous cache each): rotary positions, new rows written
+ * into the pages, attention over them. They stand next to
+ * jfh_engine_matmul_noalloc, which gives such code the weight products.
+ *
+ * Every call checks its arguments, enqueues kernels on the caller's stream
+ * (hipStream_t; NULL: the null stream) of `device` and returns without
+ * waiting; it allocates nothing, so it can be recorded into a stream capture,
+ * and keeps no state: calls on several streams do not disturb each other as
+ * long as the memory they write is their own. The arrays must be usable on
+ * that device and stay until the work is done. Arrays in device memory (page
+ * tables, lengths, row starts) are not checked on the host: whatever they
+ * hold, no kernel reaches outside the caches and rows that the call names. */
+
+typedef enum jfh_value_type { JFH_VALUE_F32 = 1, JFH_VALUE_F16 = 2, JFH_VALUE_BF16 = 3 } jfh_value_type;
+
+/* Rows of heads: value d of head h of row r at data[r * row_stride +
+ * h * head_stride + d], strides in values. */
+typedef struct jfh_rows {
+    void * data;
+    int64_t row_stride;
+    int64_t head_stride;
+    uint32_t n_rows; /* 0: the call does nothing */
+    uint32_t n_head;
+    uint32_t head_dim;
+    uint32_t type; /* jfh_value_type */
+} jfh_rows;
+
+typedef enum jfh_rope_layout {
+    JFH_ROPE_HALF = 0,       /* value i turns with value i + n_rot / 2 */
+    JFH_ROPE_INTERLEAVED = 1 /* value 2 i turns with value 2 i + 1 */
+} jfh_rope_layout;
+
+/* How the angles grow past the trained context, by `factor` s >= 1. Pair i of
+ * position p turns by p f_i, f_i = base^(-2 i / n_rot). */
+typedef enum jfh_rope_scaling {
+    JFH_ROPE_NONE = 0,   /* f_i */
+    JFH_ROPE_LINEAR = 1, /* f_i / s */
+    JFH_ROPE_NTK = 2,    /* f_i of the base base * s^(n_rot / (n_rot - 2)) */
+    JFH_ROPE_YARN = 3    /* f_i (1 - r_i) + f_i r_i / s, r_i rising from 0 to 1 between the pairs that turn beta_fast
+                          * (rounded down) and beta_slow (rounded up) times over original_context positions; the
+                          * rotated values are multiplied by attention_factor, 0.1 ln s + 1 where that is 0 */
+} jfh_rope_scaling;
+
+typedef struct jfh_rope_params {
+    uint32_t n_rot;  /* leading values of a head that turn: even, 2..256; the others stay */
+    uint32_t layout; /* jfh_rope_layout */
+    uint32_t scaling; /* jfh_rope_scaling */
+    uint32_t original_context; /* JFH_ROPE_YARN */
+    double base;
+    double factor;
+    double beta_fast;        /* JFH_ROPE_YARN */
+    double beta_slow;        /* JFH_ROPE_YARN */
+    double attention_factor; /* JFH_ROPE_YARN */
+} jfh_rope_params;
+
+typedef struct jfh_rope jfh_rope; /* a rotation's frequencies; host memory, any device, any number of calls at once */
+
+jfh_status jfh_rope_create(const jfh_rope_params * params, jfh_rope ** out);
+void jfh_rope_destroy(jfh_rope * rope);
+
+/* y = x rotated by its rows' positions (device, int32 [n_rows], any sign; a
+ * negative one turns back). x and y have the same rows, heads and head_dim,
+ * any types and strides; y may be x itself, and overlaps it in no other way.
+ * Computed in f32 from angles in f64, rounded once. */
+jfh_status jfh_rope_rotate(const jfh_rope * rope, const jfh_rows * x, const int32_t * positions, const jfh_rows * y,
+                           int32_t device, void * stream);
+
+/* One layer's K/V cache in pages of page_size positions (a power of two up to
+ * 65536), f16 or bf16. Value d of position i of page p of K/V head h at
+ * page_stride * p + head_stride * h + slot_stride * i + d of k and of v;
+ * strides are multiples of 8 values, k and v 16-byte aligned, head_dim a
+ * multiple of 8 up to 256. weights and positions, [n_pages][n_head_kv]
+ * [page_size] each, may be NULL: the attention weight that a cached position
+ * has had, and its position in the text. */
+typedef struct jfh_paged_cache {
+    void * k;
+    void * v;
+    float * weights;
+    int32_t * positions;
+    int64_t page_stride;
+    int64_t head_stride;
+    int64_t slot_stride;
+    uint32_t n_pages;
+    uint32_t page_size;
+    uint32_t n_head_kv;
+    uint32_t head_dim;
+    uint32_t type; /* JFH_VALUE_F16 or JFH_VALUE_BF16 */
+    int32_t device; /* HIP device ordinal of the memory and the stream */
+} jfh_paged_cache;
+
+/* The sequences of a step. Sequence s has lengths[s] slots in use, the step's
+ * new rows included; slot t lies in page table[s * table_stride + t /
+ * page_size], at t % page_size. Rows row_starts[s] .. row_starts[s + 1] - 1 of
+ * the step are its new ones, at its last slots in that order; there may be
+ * none. An entry of the table that is no page (negative, or n_pages and more)
+ * is an absent page: nothing is written there, and nobody sees its positions.
+ * The arrays are in device memory; max_rows and max_length bound what they
+ * hold (rows and slots beyond them are left out) and fix the launches, so a
+ * captured call may be replayed with other contents. */
+typedef struct jfh_paged_batch {
+    const int32_t * table;      /* [n_seq][table_stride] */
+    int32_t * lengths;          /* [n_seq] */
+    const int32_t * row_starts; /* [n_seq + 1], ascending from 0 */
+    uint32_t n_seq;
+    uint32_t table_stride;
+    uint32_t max_rows;
+    uint32_t max_length; /* at most table_stride * page_size */
+} jfh_paged_batch;
+
+/* Writes a step's K and V rows (any type and strides, the cache's K/V heads
+ * and head_dim) at its sequences' last slots: K rotated by rope (NULL: as it
+ * is), V as it is, weight 0 and the row's position (device, int32 [n_rows]).
+ * positions may be NULL without rope and without cache positions. A sequence
+ * shorter than its rows keeps the last ones. No two sequences may share a page
+ * that the step writes. */
+jfh_status jfh_paged_append(const jfh_paged_cache * cache, const jfh_paged_batch * batch, const jfh_rows * k,
+                            const jfh_rows * v, const jfh_rope * rope, const int32_t * positions, void * stream);
+
 /* ---------------------------------------------------------------- tokenizer */
 
 /* Byte-level BPE tokenizer of a Qwen2 GGUF vocabulary: the reference's

@@ -8,8 +8,8 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import (POINTER, c_char, c_char_p, c_double, c_float, c_int32, c_size_t, c_uint8, c_uint16, c_uint32,
-                    c_uint64, c_void_p)
+from ctypes import (POINTER, c_char, c_char_p, c_double, c_float, c_int32, c_int64, c_size_t, c_uint8, c_uint16,
+                    c_uint32, c_uint64, c_void_p)
 
 PACKAGE_DIR = os.path.dirname(os.path.abspath(__file__))
 LIBRARY_PATH = os.path.join(PACKAGE_DIR, "libjfh.so")
@@ -95,6 +95,29 @@ class KernelStat(ctypes.Structure):
     _fields_ = [("label", c_char * 64), ("launches", c_double), ("total_ms", c_double), ("bytes", c_double)]
 
 
+class Rows(ctypes.Structure):
+    _fields_ = [("data", c_void_p), ("row_stride", c_int64), ("head_stride", c_int64), ("n_rows", c_uint32),
+                ("n_head", c_uint32), ("head_dim", c_uint32), ("type", c_uint32)]
+
+
+class RopeParams(ctypes.Structure):
+    _fields_ = [("n_rot", c_uint32), ("layout", c_uint32), ("scaling", c_uint32), ("original_context", c_uint32),
+                ("base", c_double), ("factor", c_double), ("beta_fast", c_double), ("beta_slow", c_double),
+                ("attention_factor", c_double)]
+
+
+class PagedCache(ctypes.Structure):
+    _fields_ = [("k", c_void_p), ("v", c_void_p), ("weights", c_void_p), ("positions", c_void_p),
+                ("page_stride", c_int64), ("head_stride", c_int64), ("slot_stride", c_int64), ("n_pages", c_uint32),
+                ("page_size", c_uint32), ("n_head_kv", c_uint32), ("head_dim", c_uint32), ("type", c_uint32),
+                ("device", c_int32)]
+
+
+class PagedBatch(ctypes.Structure):
+    _fields_ = [("table", c_void_p), ("lengths", c_void_p), ("row_starts", c_void_p), ("n_seq", c_uint32),
+                ("table_stride", c_uint32), ("max_rows", c_uint32), ("max_length", c_uint32)]
+
+
 # name -> (restype, argtypes)
 SIGNATURES = {
     "jfh_session_profile_step": (Status, [c_void_p, POINTER(c_int32), c_uint32, c_uint32, c_uint32, POINTER(KernelStat),
@@ -159,6 +182,11 @@ SIGNATURES = {
                                         POINTER(c_double)]),
     "jfh_prompt_lookup_propose": (Status, [POINTER(c_uint32), c_size_t, c_uint32, c_uint32, c_uint32,
                                            POINTER(c_uint32), POINTER(c_uint32)]),
+    "jfh_rope_create": (Status, [POINTER(RopeParams), POINTER(c_void_p)]),
+    "jfh_rope_destroy": (None, [c_void_p]),
+    "jfh_rope_rotate": (Status, [c_void_p, POINTER(Rows), c_void_p, POINTER(Rows), c_int32, c_void_p]),
+    "jfh_paged_append": (Status, [POINTER(PagedCache), POINTER(PagedBatch), POINTER(Rows), POINTER(Rows), c_void_p,
+                                  c_void_p, c_void_p]),
     "jfh_tokenizer_open": (Status, [c_char_p, POINTER(c_void_p)]),
     "jfh_tokenizer_destroy": (None, [c_void_p]),
     "jfh_tokenizer_tokenize": (Status, [c_void_p, c_char_p, c_size_t, POINTER(c_int32), c_uint32, POINTER(c_uint32)]),

@@ -3,6 +3,7 @@
 
 #include "jfh_engine.hpp"
 #include "jfh_runtime.hpp"
+#include "jfh_status.hpp"
 #include "jfh_tokenizer.hpp"
 
 #include <hip/hip_runtime_api.h>
@@ -39,40 +40,10 @@ struct jfh_session {
 
 namespace {
 
-jfh_status ok() {
-    jfh_status s{};
-    s.code = JFH_STATUS_OK;
-    return s;
-}
-
-jfh_status error(int32_t code, const char* message) {
-    jfh_status s{};
-    s.code = code;
-    std::snprintf(s.message, sizeof(s.message), "%s", message);
-    return s;
-}
-
-template <typename F>
-jfh_status guarded(F&& fn) {
-    try {
-        fn();
-        return ok();
-    } catch (const jfh::Error& e) {
-        return error(static_cast<int32_t>(e.code()), e.what());
-    } catch (const std::invalid_argument& e) {
-        return error(JFH_STATUS_INVALID_ARGUMENT, e.what());
-    } catch (const std::bad_alloc&) {
-        return error(JFH_STATUS_OUT_OF_MEMORY, "host allocation failed");
-    } catch (const std::exception& e) {
-        return error(JFH_STATUS_DEVICE_ERROR, e.what());
-    }
-}
-
-void require(bool condition, const char* message) {
-    if (!condition) throw jfh::Error(jfh::Status::InvalidArgument, message);
-}
-
-void require(bool condition, const std::string& message) { require(condition, message.c_str()); }
+using jfh::capi::error;
+using jfh::capi::guarded;
+using jfh::capi::ok;
+using jfh::capi::require;
 
 void fill_view(const jfh_model* m, size_t index, jfh_tensor_view* out) {
     const jfh::TensorView& t = m->model->tensors()[index];

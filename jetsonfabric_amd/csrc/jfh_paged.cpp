@@ -1,0 +1,186 @@
+// C entry points of the paged-cache operators (include/jfh.h): argument checks, frequencies, launches.
+#include "jfh_paged.hpp"
+
+#include "jfh_status.hpp"
+
+#include <algorithm>
+#include <cmath>
+#include <memory>
+
+struct jfh_rope {
+    jfh::paged::Rotation rotation;
+};
+
+namespace {
+
+namespace paged = jfh::paged;
+
+using jfh::capi::guarded;
+using jfh::capi::require;
+
+constexpr uint64_t kMaxIndex = 0x7FFFFFFF;
+
+void check(hipError_t e, const char* what) {
+    if (e == hipSuccess) return;
+    (void) hipGetLastError();  // it is reported here: the next call's launch is not to find it
+    throw jfh::Error(jfh::Status::DeviceError, std::string(what) + ": " + hipGetErrorString(e));
+}
+
+// The calling thread's device is `device` while this lives.
+class OnDevice {
+public:
+    explicit OnDevice(int device) : device_(device) {
+        check(hipGetDevice(&before_), "find the current device");
+        if (before_ != device_) check(hipSetDevice(device_), "select the cache's device");
+    }
+    ~OnDevice() {
+        if (before_ != device_) (void) hipSetDevice(before_);
+    }
+    OnDevice(const OnDevice&) = delete;
+    OnDevice& operator=(const OnDevice&) = delete;
+
+private:
+    int device_, before_ = 0;
+};
+
+bool aligned(const void* p, uintptr_t bytes) { return reinterpret_cast<uintptr_t>(p) % bytes == 0; }
+
+paged::Rows rows_of(const jfh_rows* x, const char* name) {
+    const std::string n = name;
+    require(x != nullptr, n + " rows are required");
+    require(x->type >= JFH_VALUE_F32 && x->type <= JFH_VALUE_BF16, n + " rows have an unknown value type");
+    require(x->n_rows <= kMaxIndex, n + " has more rows than a step can hold");
+    require(x->n_head > 0 && x->n_head <= 65536 && x->head_dim > 0 && x->head_dim <= 65536,
+            n + " rows have no heads, no values or too many");
+    require(x->row_stride >= 0 && x->head_stride >= 0, n + " rows have a negative stride");
+    require(x->n_rows == 0 || (x->data != nullptr && aligned(x->data, x->type == JFH_VALUE_F32 ? 4 : 2)),
+            n + " rows are missing or not aligned to their values");
+    return paged::Rows{x->data, x->row_stride, x->head_stride, x->n_rows, x->n_head, x->head_dim, x->type};
+}
+
+paged::Cache cache_of(const jfh_paged_cache* c) {
+    require(c != nullptr, "a cache is required");
+    require(c->k && c->v && aligned(c->k, 16) && aligned(c->v, 16), "the cache's k and v must be 16-byte aligned");
+    require(c->type == JFH_VALUE_F16 || c->type == JFH_VALUE_BF16, "a cache holds f16 or bf16 values");
+    require(c->n_pages > 0 && c->n_pages <= kMaxIndex, "a cache needs pages");
+    require(c->page_size > 0 && c->page_size <= paged::kMaxPageSize && (c->page_size & (c->page_size - 1)) == 0,
+            "the page size must be a power of two up to 65536");
+    require(c->n_head_kv > 0 && c->n_head_kv <= 65536, "a cache needs heads");
+    require(c->head_dim >= 8 && c->head_dim <= paged::kMaxHeadDim && c->head_dim % 8 == 0,
+            "the cache's head dim must be a multiple of 8 up to 256");
+    require(c->page_stride % 8 == 0 && c->head_stride % 8 == 0 && c->slot_stride % 8 == 0 && c->page_stride >= 0 &&
+                c->head_stride >= 0 && c->slot_stride >= 0,
+            "the cache's strides must be multiples of 8 values");
+    const int64_t dim = c->head_dim;
+    require((c->page_size == 1 || c->slot_stride >= dim) && (c->n_head_kv == 1 || c->head_stride >= dim) &&
+                (c->n_pages == 1 || c->page_stride >= dim),
+            "the cache's strides let its rows overlap");
+    require(aligned(c->weights, 4) && aligned(c->positions, 4), "the cache's weights and positions must be aligned");
+    uint32_t shift = 0;
+    while ((1U << shift) < c->page_size) ++shift;
+    return paged::Cache{c->k, c->v, c->weights, c->positions, c->page_stride, c->head_stride, c->slot_stride,
+                        c->n_pages, shift, c->n_head_kv, c->head_dim, c->type};
+}
+
+paged::Batch batch_of(const jfh_paged_batch* b, const jfh_paged_cache& c, bool rows) {
+    require(b != nullptr, "a batch is required");
+    require(b->n_seq <= 0xFFFFFF, "a batch holds at most 16777215 sequences");
+    require(b->n_seq == 0 || (b->table && b->lengths && (b->row_starts || !rows)),
+            "a batch needs its table, lengths and row starts");
+    const uint64_t slots = static_cast<uint64_t>(b->table_stride) * c.page_size;
+    require(b->max_length <= slots, "the batch's max_length exceeds its table");
+    require(b->max_length <= kMaxIndex - 1024 && b->max_rows <= kMaxIndex, "the batch's bounds exceed 2^31");
+    return paged::Batch{b->table, b->lengths, b->row_starts, b->n_seq, b->table_stride, b->max_rows, b->max_length};
+}
+
+paged::Rotation rotation_of(const jfh_rope_params& p) {
+    require(p.n_rot >= 2 && p.n_rot <= 2 * paged::kMaxRotPairs && p.n_rot % 2 == 0,
+            "a rotation turns an even number of values, 2 to 256");
+    require(p.layout <= JFH_ROPE_INTERLEAVED, "unknown rotation layout");
+    require(p.scaling <= JFH_ROPE_YARN, "unknown rotation scaling");
+    require(std::isfinite(p.base) && p.base > 1.0, "the rotation's base must be above 1");
+    const bool scaled = p.scaling != JFH_ROPE_NONE;
+    require(!scaled || (std::isfinite(p.factor) && p.factor >= 1.0), "the rotation's factor must be at least 1");
+    require(p.scaling != JFH_ROPE_NTK || p.n_rot > 2, "this scaling needs more than one pair");
+    const double n = p.n_rot, pi = std::acos(-1.0);
+    double base = p.base, lo = 0.0, hi = 1.0;
+    paged::Rotation r{};
+    r.size = 1.0F;
+    r.n_rot = p.n_rot;
+    r.interleaved = p.layout == JFH_ROPE_INTERLEAVED ? 1U : 0U;
+    if (p.scaling == JFH_ROPE_NTK) base *= std::pow(p.factor, n / (n - 2.0));
+    if (p.scaling == JFH_ROPE_YARN) {
+        require(p.original_context > 0 && std::isfinite(p.beta_fast) && std::isfinite(p.beta_slow) && p.beta_slow > 0.0 &&
+                    p.beta_fast >= p.beta_slow,
+                "this scaling needs the original context and beta_fast >= beta_slow > 0");
+        require(std::isfinite(p.attention_factor) && p.attention_factor >= 0.0,
+                "the attention factor must be 0 (by the factor) or above");
+        // the pair that turns `turns` times over the original context
+        const auto pair = [&](double turns) {
+            return n * std::log(p.original_context / (turns * 2.0 * pi)) / (2.0 * std::log(p.base));
+        };
+        lo = std::max(std::floor(pair(p.beta_fast)), 0.0);
+        hi = std::min(std::ceil(pair(p.beta_slow)), n - 1.0);
+        r.size = static_cast<float>(p.attention_factor > 0.0 ? p.attention_factor : 0.1 * std::log(p.factor) + 1.0);
+    }
+    for (uint32_t i = 0; i < p.n_rot / 2; ++i) {
+        double f = std::pow(base, -2.0 * i / n);
+        if (p.scaling == JFH_ROPE_LINEAR) f /= p.factor;
+        if (p.scaling == JFH_ROPE_YARN) {
+            const double far = std::clamp((i - lo) / std::max(hi - lo, 1e-3), 0.0, 1.0);
+            f = f * (1.0 - far) + f / p.factor * far;
+        }
+        r.turns[i] = f / (2.0 * pi);
+    }
+    return r;
+}
+
+}  // namespace
+
+jfh_status jfh_rope_create(const jfh_rope_params* params, jfh_rope** out) {
+    return guarded([&] {
+        require(params && out, "rotation parameters and an output are required");
+        *out = nullptr;
+        *out = new jfh_rope{rotation_of(*params)};
+    });
+}
+
+void jfh_rope_destroy(jfh_rope* rope) { delete rope; }
+
+jfh_status jfh_rope_rotate(const jfh_rope* rope, const jfh_rows* x, const int32_t* positions, const jfh_rows* y,
+                           int32_t device, void* stream) {
+    return guarded([&] {
+        require(rope != nullptr, "a rotation is required");
+        const paged::Rows in = rows_of(x, "x"), out = rows_of(y, "y");
+        require(in.rows == out.rows && in.heads == out.heads && in.head_dim == out.head_dim,
+                "x and y must have the same rows, heads and head dim");
+        require(rope->rotation.n_rot <= in.head_dim, "the rotation turns more values than a head has");
+        require(in.data != out.data || (in.type == out.type && in.row_stride == out.row_stride &&
+                                        in.head_stride == out.head_stride),
+                "rows rotated in place must keep their type and strides");
+        if (in.rows == 0) return;
+        require(positions != nullptr && aligned(positions, 4), "positions are required");
+        const OnDevice guard(device);
+        check(paged::launch_rotate(rope->rotation, in, positions, out, static_cast<hipStream_t>(stream)), "rotate rows");
+    });
+}
+
+jfh_status jfh_paged_append(const jfh_paged_cache* cache, const jfh_paged_batch* batch, const jfh_rows* k,
+                            const jfh_rows* v, const jfh_rope* rope, const int32_t* positions, void* stream) {
+    return guarded([&] {
+        const paged::Cache c = cache_of(cache);
+        const paged::Batch b = batch_of(batch, *cache, true);
+        const paged::Rows kr = rows_of(k, "k"), vr = rows_of(v, "v");
+        require(kr.rows == vr.rows, "k and v must have the same rows");
+        require(kr.heads == c.n_head_kv && vr.heads == c.n_head_kv && kr.head_dim == c.head_dim && vr.head_dim == c.head_dim,
+                "k and v must have the cache's heads and head dim");
+        require(!rope || rope->rotation.n_rot <= c.head_dim, "the rotation turns more values than a head has");
+        require((!rope && !c.positions) || positions, "positions are required with a rotation or cache positions");
+        require(aligned(positions, 4), "positions must be aligned");
+        if (kr.rows == 0 || b.n_seq == 0) return;
+        const OnDevice guard(cache->device);
+        check(paged::launch_append(rope ? &rope->rotation : nullptr, c, b, kr, vr, positions,
+                                   static_cast<hipStream_t>(stream)),
+              "append rows");
+    });
+}

@@ -1,0 +1,156 @@
+"""Operators of a decoder layer on torch tensors in device memory, around a K/V cache in pages.
+
+``Rope`` rotates queries and keys; ``PagedCache`` is one layer's cache, whose
+pages, page tables and lengths belong to the caller; ``PagedBatch`` is what a
+step's sequences look like. Every call enqueues its kernels on torch's current
+stream of the cache's device and returns without waiting. It can be captured
+into a graph, and replayed with other contents of the same tensors.
+"""
+from __future__ import annotations
+
+import ctypes
+import sys
+
+from . import _capi
+from ._capi import check, library
+
+__all__ = ["Rope", "PagedCache", "PagedBatch"]
+
+_TYPES = {"torch.float32": 1, "torch.float16": 2, "torch.bfloat16": 3}
+_LAYOUTS = {"half": 0, "interleaved": 1}
+_SCALINGS = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3}
+
+
+def _type(x, name: str) -> int:
+    t = _TYPES.get(str(x.dtype))
+    if t is None:
+        raise ValueError(f"{name} holds {x.dtype}: float32, float16 and bfloat16 are supported")
+    return t
+
+
+def _rows(x, name: str, device: int) -> _capi.Rows:
+    """A tensor [rows, heads, head dim] of any strides whose heads are contiguous."""
+    if x.dim() != 3:
+        raise ValueError(f"{name} must be [rows, heads, head dim]")
+    if not x.is_cuda or x.get_device() != device:
+        raise ValueError(f"{name} must be on GPU {device}")
+    rows, heads, dim = x.shape
+    row_stride, head_stride, one = x.stride()
+    if one != 1 and dim > 1:
+        raise ValueError(f"the values of a head of {name} must be contiguous")
+    return _capi.Rows(x.data_ptr(), row_stride, head_stride, rows, heads, dim, _type(x, name))
+
+
+def _array(x, name: str, dtype: str, device: int, shape: tuple | None = None) -> int:
+    """Address of a contiguous device array."""
+    if str(x.dtype) != dtype or not x.is_cuda or x.get_device() != device or not x.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous {dtype} tensor on GPU {device}")
+    if shape is not None and x.shape != shape:
+        raise ValueError(f"{name} must have shape {list(shape)}, not {list(x.shape)}")
+    return x.data_ptr()
+
+
+def _stream(device: int) -> int:
+    return sys.modules["torch"].cuda.current_stream(device).cuda_stream
+
+
+class Rope:
+    """Rotary positions (jfh_rope_params): the leading n_rot values of a head turn in pairs,
+    (i, i + n_rot / 2) in the "half" layout, (2 i, 2 i + 1) in the "interleaved" one, by position *
+    base^(-2 i / n_rot); ``scaling`` "linear", "ntk" or "yarn" stretches the angles for contexts
+    ``factor`` times the trained one."""
+
+    def __init__(self, n_rot: int, base: float = 1.0e6, layout: str = "half", scaling: str = "none", factor: float = 1.0,
+                 original_context: int = 32768, beta_fast: float = 32.0, beta_slow: float = 1.0,
+                 attention_factor: float = 0.0):
+        self._h = ctypes.c_void_p()
+        if layout not in _LAYOUTS:
+            raise ValueError(f"layout must be one of {sorted(_LAYOUTS)}")
+        if scaling not in _SCALINGS:
+            raise ValueError(f"scaling must be one of {sorted(_SCALINGS)}")
+        params = _capi.RopeParams(n_rot, _LAYOUTS[layout], _SCALINGS[scaling], original_context, base, factor, beta_fast,
+                                  beta_slow, attention_factor)
+        check(library().jfh_rope_create(ctypes.byref(params), ctypes.byref(self._h)))
+
+    def close(self) -> None:
+        if self._h:
+            library().jfh_rope_destroy(self._h)
+            self._h = ctypes.c_void_p()
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+    @property
+    def handle(self) -> ctypes.c_void_p:
+        return self._h
+
+    def rotate(self, x, positions, out=None):
+        """x [rows, heads, head dim] rotated by positions (int32 [rows]) into out, which may be x or
+        have another type; a new tensor like x by default. Returns out."""
+        if out is None:
+            out = sys.modules["torch"].empty_like(x)
+        device = x.get_device()
+        a, b = _rows(x, "x", device), _rows(out, "out", device)
+        at = _array(positions, "positions", "torch.int32", device, (x.shape[0],))
+        check(library().jfh_rope_rotate(self._h, ctypes.byref(a), at, ctypes.byref(b), device, _stream(device)))
+        return out
+
+
+class PagedBatch:
+    """The sequences of a step (jfh_paged_batch), int32 tensors on the cache's GPU: table [sequences,
+    pages], lengths [sequences] (slots in use, the new rows included) and row_starts [sequences + 1].
+    max_rows and max_length bound the rows of a sequence and its length."""
+
+    def __init__(self, table, lengths, row_starts, max_rows: int, max_length: int):
+        device = table.get_device()
+        if table.dim() != 2:
+            raise ValueError("table must be [sequences, pages]")
+        n = table.shape[0]
+        self.table, self.lengths, self.row_starts = table, lengths, row_starts
+        self.device = device
+        self.c = _capi.PagedBatch(_array(table, "table", "torch.int32", device),
+                                  _array(lengths, "lengths", "torch.int32", device, (n,)),
+                                  _array(row_starts, "row_starts", "torch.int32", device, (n + 1,)), n, table.shape[1],
+                                  max_rows, max_length)
+        self.ref = ctypes.byref(self.c)
+
+
+class PagedCache:
+    """One layer's K/V cache in pages (jfh_paged_cache): k and v [pages, K/V heads, page size, head
+    dim], float16 or bfloat16, of equal strides (a permuted view of another order will do); weights
+    (float32) and positions (int32) [pages, K/V heads, page size], which only a cache that is cut needs."""
+
+    def __init__(self, k, v, weights=None, positions=None):
+        device = k.get_device()
+        if k.dim() != 4 or k.shape != v.shape or k.dtype != v.dtype or k.stride() != v.stride():
+            raise ValueError("k and v must be [pages, K/V heads, page size, head dim] of one type and equal strides")
+        if not k.is_cuda or v.get_device() != device:
+            raise ValueError("k and v must be on one GPU")
+        if k.stride(3) != 1:
+            raise ValueError("the values of a head must be contiguous")
+        pages, heads, page_size, dim = k.shape
+        meta = (pages, heads, page_size)
+        self.k, self.v, self.weights, self.positions = k, v, weights, positions
+        self.device = device
+        self.c = _capi.PagedCache(
+            k.data_ptr(), v.data_ptr(),
+            None if weights is None else _array(weights, "weights", "torch.float32", device, meta),
+            None if positions is None else _array(positions, "positions", "torch.int32", device, meta),
+            k.stride(0), k.stride(1), k.stride(2), pages, page_size, heads, dim, _type(k, "k"), device)
+        self.ref = ctypes.byref(self.c)
+
+    def _of(self, batch: PagedBatch):
+        if batch.device != self.device:
+            raise ValueError(f"the batch is on GPU {batch.device}, the cache on GPU {self.device}")
+        return batch.ref
+
+    def append(self, batch: PagedBatch, k, v, positions=None, rope: Rope | None = None) -> None:
+        """Writes a step's rows k and v [rows, K/V heads, head dim] at its sequences' last slots, k
+        rotated by rope; positions int32 [rows]."""
+        a, b = _rows(k, "k", self.device), _rows(v, "v", self.device)
+        at = None if positions is None else _array(positions, "positions", "torch.int32", self.device, (k.shape[0],))
+        check(library().jfh_paged_append(self.ref, self._of(batch), ctypes.byref(a), ctypes.byref(b),
+                                         None if rope is None else rope.handle, at, _stream(self.device)))

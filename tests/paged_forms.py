@@ -1,0 +1,112 @@
+"""The paged-cache operators in 64 bits on the CPU, row by row from their definitions, and random caches to try them on."""
+from __future__ import annotations
+
+import math
+
+import torch
+
+TYPES = {"f32": torch.float32, "f16": torch.float16, "bf16": torch.bfloat16}
+
+
+def half_step(dtype) -> float:
+    """Largest relative error of one rounding to the type."""
+    return torch.finfo(dtype).eps / 2
+
+
+def frequencies(n_rot, base=1.0e6, scaling="none", factor=1.0, original_context=32768, beta_fast=32.0, beta_slow=1.0,
+                attention_factor=0.0):
+    """(angle per position of each pair, size of the rotated values)"""
+    f, size = [], 1.0
+    if scaling == "ntk":
+        base = base * factor ** (n_rot / (n_rot - 2))
+    if scaling == "yarn":
+        size = attention_factor or 0.1 * math.log(factor) + 1
+        lo, hi = (n_rot * math.log(original_context / (b * 2 * math.pi)) / (2 * math.log(base)) for b in (beta_fast, beta_slow))
+        lo, hi = max(math.floor(lo), 0), min(math.ceil(hi), n_rot - 1)
+    for i in range(n_rot // 2):
+        w = base ** (-2 * i / n_rot)
+        if scaling == "linear":
+            w /= factor
+        if scaling == "yarn":
+            r = min(max((i - lo) / max(hi - lo, 1e-3), 0.0), 1.0)
+            w = w * (1 - r) + w / factor * r
+        f.append(w)
+    return torch.tensor(f, dtype=torch.float64), size
+
+
+def rotate(x, positions, n_rot, layout="half", **kw):
+    """x [rows, heads, dim] (any type) rotated, f64, and the bound |a| + |b| of each rotated value's terms."""
+    f, size = frequencies(n_rot, **kw)
+    y = x.double().clone()
+    terms = torch.zeros_like(y)
+    angle = positions.double()[:, None] * f
+    c, s = (angle.cos() * size)[:, None], (angle.sin() * size)[:, None]
+    i = torch.arange(n_rot // 2)
+    lo, hi = (i, i + n_rot // 2) if layout == "half" else (2 * i, 2 * i + 1)
+    a, b = x.double()[..., lo], x.double()[..., hi]
+    y[..., lo], y[..., hi] = a * c - b * s, a * s + b * c
+    terms[..., lo] = terms[..., hi] = (a.abs() + b.abs()) * size
+    return y, terms
+
+
+# Rotated values: cos and sin carry the rounding of the angle to a float (2^-25 half turns, 9.4e-8 rad) and sincospi's own
+# error (below 2 steps, 1.2e-7), the size, products and sum three more roundings of 2^-24: below 4.0e-7 of |a| + |b|.
+ROTATION = 4.0e-7
+
+
+def rotation_bound(y, terms, dtype):
+    # the smallest normal's step covers results below f16's normal range
+    return half_step(dtype) * (y.abs() + ROTATION * terms) + ROTATION * terms + torch.finfo(dtype).tiny * torch.finfo(dtype).eps
+
+
+class Sequences:
+    """A random cache and step. rows[s] new rows of sequence s, lengths[s] slots with them; pages in random order, the
+    pool padded with pages of nobody; absent: (sequence, page number) pairs whose table entry is no page."""
+
+    def __init__(self, rows, lengths, kv_heads, dim, page, dtype, seed=0, order="pages", absent=(), pad_rows=0, extra_pages=3,
+                 wide_table=0):
+        g = torch.Generator().manual_seed(seed)
+        self.rows, self.lens, self.page, self.kv_heads, self.dim, self.dtype = list(rows), list(lengths), page, kv_heads, dim, dtype
+        per = max(1, -(-max(lengths) // page)) + wide_table
+        self.n_pages = len(self.rows) * per + extra_pages
+        self.table = torch.randperm(self.n_pages, generator=g)[:len(self.rows) * per].to(torch.int32).reshape(len(self.rows), per)
+        for n, (s, p) in enumerate(absent):
+            self.table[s, p] = [-1, self.n_pages, 2**31 - 1, -2**31][n % 4]
+        starts = [0]
+        for r in self.rows:
+            starts.append(starts[-1] + r)
+        self.starts, self.total = starts, starts[-1] + pad_rows
+        self.row_starts = torch.tensor(starts, dtype=torch.int32)
+        self.lengths = torch.tensor(self.lens, dtype=torch.int32)
+        self.order = order
+        size = (self.n_pages, kv_heads, page, dim)
+        self.k = torch.randn(size, generator=g).to(dtype)
+        self.v = torch.randn(size, generator=g).to(dtype)
+        self.weights = torch.rand(size[:3], generator=g)
+        self.positions = torch.randint(0, 1 << 20, size[:3], generator=g, dtype=torch.int32)
+        self.max_rows, self.max_length = max(self.rows), max(self.lens)
+
+    def slot(self, s, t):
+        """(page, place) of slot t of sequence s, None on an absent page."""
+        p = int(self.table[s, t // self.page])
+        return (p, t % self.page) if 0 <= p < self.n_pages else None
+
+    def to_gpu(self):
+        """The pool on the GPU (as [pages, heads, page, dim] views of storage in the asked order), table, lengths, starts."""
+        def pool(x):
+            if self.order == "tokens":  # [pages, page, heads, dim]
+                return x.transpose(1, 2).contiguous().cuda().transpose(1, 2)
+            if self.order == "padded":  # heads and slots further apart than they need to be
+                big = torch.zeros(x.shape[0], x.shape[1] + 1, x.shape[2] + 2, x.shape[3] + 8, dtype=x.dtype)
+                big[:, :x.shape[1], :x.shape[2], :x.shape[3]] = x
+                return big.cuda()[:, :x.shape[1], :x.shape[2], :x.shape[3]]
+            return x.cuda()
+        return (pool(self.k), pool(self.v), self.weights.cuda(), self.positions.cuda(), self.table.cuda(),
+                self.lengths.cuda(), self.row_starts.cuda())
+
+    def rows_of(self, s):
+        """(row, slot) of the sequence's new rows that have a slot."""
+        for i in range(self.rows[s]):
+            t = self.lens[s] - self.rows[s] + i
+            if t >= 0:
+                yield self.starts[s] + i, t

@@ -1,0 +1,157 @@
+"""The paged-cache operators without a GPU: what they refuse, rotations that cannot be made, and their index arithmetic.
+
+The refused calls carry addresses that no call may touch."""
+from __future__ import annotations
+
+import ctypes
+import os
+import subprocess
+
+import pytest
+
+import jetsonfabric_amd as jf
+from jetsonfabric_amd import _capi
+from jetsonfabric_amd._capi import check
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+AT = 1 << 20  # an aligned address; nothing is there
+
+
+def rows(**kw):
+    return _capi.Rows(**{"data": AT, "row_stride": 256, "head_stride": 64, "n_rows": 3, "n_head": 4, "head_dim": 64,
+                         "type": 2, **kw})
+
+
+def cache(**kw):
+    return _capi.PagedCache(**{"k": AT, "v": AT, "weights": AT, "positions": AT, "page_stride": 4096, "head_stride": 1024,
+                               "slot_stride": 64, "n_pages": 9, "page_size": 16, "n_head_kv": 4, "head_dim": 64, "type": 2,
+                               "device": 0, **kw})
+
+
+def batch(**kw):
+    return _capi.PagedBatch(**{"table": AT, "lengths": AT, "row_starts": AT, "n_seq": 2, "table_stride": 4, "max_rows": 3,
+                               "max_length": 64, **kw})
+
+
+def refused(call, match):
+    with pytest.raises(jf.InvalidArgument, match=match):
+        check(call())
+
+
+BAD_CACHES = [({"k": None}, "aligned"), ({"v": AT + 8}, "aligned"), ({"type": 1}, "f16 or bf16"), ({"type": 9}, "f16 or bf16"),
+              ({"n_pages": 0}, "pages"), ({"n_pages": 1 << 31}, "pages"), ({"page_size": 24}, "power of two"),
+              ({"page_size": 0}, "power of two"), ({"page_size": 1 << 17}, "power of two"), ({"n_head_kv": 0}, "heads"),
+              ({"head_dim": 60}, "head dim"), ({"head_dim": 264}, "head dim"), ({"head_dim": 0}, "head dim"),
+              ({"slot_stride": 65}, "strides"), ({"head_stride": -1024}, "strides"), ({"page_stride": 4100}, "strides"),
+              ({"slot_stride": 56}, "overlap"), ({"head_stride": 8}, "overlap"), ({"page_stride": 0}, "overlap"),
+              ({"weights": AT + 2}, "aligned"), ({"positions": AT + 1}, "aligned")]
+BAD_BATCHES = [({"table": None}, "table, lengths"), ({"lengths": None}, "table, lengths"),
+               ({"row_starts": None}, "row starts"), ({"max_length": 65}, "max_length"), ({"table_stride": 3}, "max_length"),
+               ({"table_stride": 1 << 31, "max_length": (1 << 31) - 1}, "2\\^31"), ({"max_rows": 1 << 31}, "2\\^31"),
+               ({"n_seq": 1 << 24}, "sequences")]
+
+
+def _append(c=None, b=None, k=None, v=None, rope=None, positions=AT):
+    return jf.library().jfh_paged_append(ctypes.byref(c or cache()), ctypes.byref(b or batch()), ctypes.byref(k or rows()),
+                                         ctypes.byref(v or rows()), rope, positions, None)
+
+
+@pytest.mark.parametrize("change,match", BAD_CACHES)
+def test_caches_are_checked(change, match):
+    refused(lambda: _append(c=cache(**change)), match)
+
+
+@pytest.mark.parametrize("change,match", BAD_BATCHES)
+def test_batches_are_checked(change, match):
+    refused(lambda: _append(b=batch(**change)), match)
+
+
+@pytest.mark.parametrize("change,match", [
+    ({"data": None}, "k rows are missing"), ({"data": AT + 1}, "aligned"), ({"type": 1, "data": AT + 2}, "aligned"),
+    ({"type": 0}, "value type"), ({"type": 4}, "value type"), ({"n_head": 3}, "heads and head dim"),
+    ({"head_dim": 32}, "heads and head dim"), ({"n_head": 0}, "no heads"), ({"row_stride": -1}, "negative stride"),
+    ({"n_rows": 4}, "same rows"), ({"n_rows": 1 << 31}, "more rows")])
+def test_appended_rows_are_checked(change, match):
+    refused(lambda: _append(k=rows(**change)), match)
+
+
+def test_appends_ask_for_positions():
+    refused(lambda: _append(positions=None), "positions are required")
+    refused(lambda: _append(c=cache(positions=None), positions=None, rope=jf.Rope(64).handle), "positions are required")
+    refused(lambda: _append(positions=AT + 2), "aligned")
+    refused(lambda: _append(rope=jf.Rope(66).handle), "more values than a head")
+
+
+def test_missing_arguments_are_refused():
+    lib = jf.library()
+    assert lib.jfh_paged_append(None, ctypes.byref(batch()), ctypes.byref(rows()), ctypes.byref(rows()), None, AT, None).code == 1
+    assert lib.jfh_paged_append(ctypes.byref(cache()), None, ctypes.byref(rows()), ctypes.byref(rows()), None, AT, None).code == 1
+    assert lib.jfh_paged_append(ctypes.byref(cache()), ctypes.byref(batch()), None, ctypes.byref(rows()), None, AT, None).code == 1
+    assert lib.jfh_rope_rotate(None, ctypes.byref(rows()), AT, ctypes.byref(rows()), 0, None).code == 1
+    assert lib.jfh_rope_create(None, ctypes.byref(ctypes.c_void_p())).code == 1
+    lib.jfh_rope_destroy(None)
+
+
+def test_steps_without_rows_or_sequences_do_nothing():
+    check(_append(k=rows(n_rows=0, data=None), v=rows(n_rows=0, data=None)))
+    check(_append(b=batch(n_seq=0, table=None, lengths=None, row_starts=None)))
+    none = rows(n_rows=0, data=None)
+    check(jf.library().jfh_rope_rotate(jf.Rope(64).handle, ctypes.byref(none), None, ctypes.byref(none), 0, None))
+
+
+@pytest.mark.parametrize("kw,match", [
+    ({"n_rot": 0}, "even number"), ({"n_rot": 7}, "even number"), ({"n_rot": 258}, "even number"),
+    ({"base": 1.0}, "base"), ({"base": float("nan")}, "base"), ({"scaling": "linear", "factor": 0.5}, "factor"),
+    ({"scaling": "yarn", "factor": float("inf")}, "factor"), ({"scaling": "ntk", "n_rot": 2, "factor": 2.0}, "more than one pair"),
+    ({"scaling": "yarn", "factor": 2.0, "original_context": 0}, "original context"),
+    ({"scaling": "yarn", "factor": 2.0, "beta_fast": 0.5}, "beta_fast"),
+    ({"scaling": "yarn", "factor": 2.0, "beta_slow": 0.0}, "beta_fast"),
+    ({"scaling": "yarn", "factor": 2.0, "attention_factor": -1.0}, "attention factor")])
+def test_rotations_are_checked(kw, match):
+    with pytest.raises(jf.InvalidArgument, match=match):
+        jf.Rope(**{"n_rot": 64, **kw})
+
+
+def test_rotation_names_are_checked():
+    with pytest.raises(ValueError, match="layout"):
+        jf.Rope(64, layout="pairs")
+    with pytest.raises(ValueError, match="scaling"):
+        jf.Rope(64, scaling="dynamic")
+
+
+def _rotate(x, y, rope=None, positions=AT):
+    rope = rope or jf.Rope(64)
+    return jf.library().jfh_rope_rotate(rope.handle, ctypes.byref(x), positions, ctypes.byref(y), 0, None)
+
+
+def test_rotated_rows_are_checked():
+    refused(lambda: _rotate(rows(), rows(n_head=5)), "same rows, heads")
+    refused(lambda: _rotate(rows(), rows(head_dim=128)), "same rows, heads")
+    refused(lambda: _rotate(rows(head_dim=32), rows(head_dim=32)), "more values than a head")
+    refused(lambda: _rotate(rows(), rows(row_stride=512)), "in place")
+    refused(lambda: _rotate(rows(), rows(type=3)), "in place")
+    refused(lambda: _rotate(rows(), rows(data=AT + 4096), positions=None), "positions")
+    refused(lambda: _rotate(rows(), rows(data=AT + 4096, type=7)), "value type")
+
+
+def test_index_arithmetic_cpp_tests():
+    exe = os.path.join(ROOT, "tests", "cpp", "paged_test")
+    subprocess.run(["make", "-C", os.path.join(ROOT, "tests", "cpp"), "paged_test"], check=True, capture_output=True)
+    r = subprocess.run([exe], capture_output=True, text=True, timeout=60)
+    assert r.returncode == 0, r.stdout + r.stderr
+    assert "paged tests passed" in r.stdout
+
+
+def test_tensors_are_checked():
+    import torch
+
+    with pytest.raises(ValueError, match="on GPU|on one GPU"):
+        jf.Rope(64).rotate(torch.zeros(2, 1, 64), torch.zeros(2, dtype=torch.int32))
+    pages = torch.zeros(4, 2, 16, 64, dtype=torch.float16)
+    with pytest.raises(ValueError, match="GPU"):
+        jf.PagedCache(pages, pages)
+    with pytest.raises(ValueError, match="equal strides"):
+        jf.PagedCache(pages, pages.float())
+    with pytest.raises(ValueError, match="GPU"):
+        jf.PagedBatch(torch.zeros(1, 4, dtype=torch.int32), torch.zeros(1, dtype=torch.int32),
+                      torch.zeros(2, dtype=torch.int32), 1, 64)
