@@ -499,6 +499,25 @@ typedef struct jfh_paged_batch {
 jfh_status jfh_paged_append(const jfh_paged_cache * cache, const jfh_paged_batch * batch, const jfh_rows * k,
                             const jfh_rows * v, const jfh_rope * rope, const int32_t * positions, void * stream);
 
+/* Attention of a step's rows over the cache, the rows' own positions included:
+ * out = softmax(scale * q K^T) V per row and head, head h reading K/V head
+ * h / (n_head / n_head_kv). With causal, row r of a sequence's n sees its slots
+ * 0 .. lengths - n + r, otherwise all of them. q and out have the cache's type
+ * and head_dim, 16-byte aligned, strides in multiples of 8 values; lse (device,
+ * float [n_rows][n_head], may be NULL) receives ln sum exp(scale q K^T). A row
+ * that sees nothing gives 0 and -inf; what a row does not see does not reach
+ * it, infinities and NaN included; rows of no sequence are left as they were.
+ * Sums are f32, the weights are rounded to the cache's type for their product
+ * with V. workspace: workspace_bytes of device memory, 16-byte aligned, at
+ * least what jfh_paged_attention_workspace says for the same batch and q (0
+ * where the step needs none); a call in flight, or a captured one, needs its
+ * own. */
+jfh_status jfh_paged_attention_workspace(const jfh_paged_cache * cache, const jfh_paged_batch * batch,
+                                         const jfh_rows * q, size_t * bytes);
+jfh_status jfh_paged_attention(const jfh_paged_cache * cache, const jfh_paged_batch * batch, const jfh_rows * q,
+                               float scale, uint32_t causal, const jfh_rows * out, float * lse, void * workspace,
+                               size_t workspace_bytes, void * stream);
+
 /* ---------------------------------------------------------------- tokenizer */
 
 /* Byte-level BPE tokenizer of a Qwen2 GGUF vocabulary: the reference's

@@ -82,7 +82,8 @@ paged::Cache cache_of(const jfh_paged_cache* c) {
                         c->n_pages, shift, c->n_head_kv, c->head_dim, c->type};
 }
 
-paged::Batch batch_of(const jfh_paged_batch* b, const jfh_paged_cache& c, bool rows) {
+// A batch of a step of n_rows rows (no rows: of a call that looks at the sequences' slots alone).
+paged::Batch batch_of(const jfh_paged_batch* b, const jfh_paged_cache& c, bool rows, uint32_t n_rows = 0) {
     require(b != nullptr, "a batch is required");
     require(b->n_seq <= 0xFFFFFF, "a batch holds at most 16777215 sequences");
     require(b->n_seq == 0 || (b->table && b->lengths && (b->row_starts || !rows)),
@@ -90,7 +91,8 @@ paged::Batch batch_of(const jfh_paged_batch* b, const jfh_paged_cache& c, bool r
     const uint64_t slots = static_cast<uint64_t>(b->table_stride) * c.page_size;
     require(b->max_length <= slots, "the batch's max_length exceeds its table");
     require(b->max_length <= kMaxIndex - 1024 && b->max_rows <= kMaxIndex, "the batch's bounds exceed 2^31");
-    return paged::Batch{b->table, b->lengths, b->row_starts, b->n_seq, b->table_stride, b->max_rows, b->max_length};
+    return paged::Batch{b->table, b->lengths, b->row_starts, b->n_seq, b->table_stride,
+                        std::min(b->max_rows, n_rows), b->max_length};
 }
 
 paged::Rotation rotation_of(const jfh_rope_params& p) {
@@ -135,6 +137,38 @@ paged::Rotation rotation_of(const jfh_rope_params& p) {
     return r;
 }
 
+// Rows that attention reads or writes: the cache's type and head dim, in steps of 16 bytes.
+paged::Rows attended(const jfh_rows* x, const paged::Cache& c, const char* name) {
+    const paged::Rows r = rows_of(x, name);
+    const std::string n = name;
+    require(r.type == c.type && r.head_dim == c.head_dim, n + " must have the cache's type and head dim");
+    require(r.heads % c.n_head_kv == 0, n + "'s heads must be a multiple of the cache's");
+    require(aligned(r.data, 16) && r.row_stride % 8 == 0 && r.head_stride % 8 == 0,
+            n + " must be 16-byte aligned, with strides in multiples of 8 values");
+    require(static_cast<uint64_t>(r.rows) * r.heads <= kMaxIndex, n + " has more rows than a step can hold");
+    return r;
+}
+
+float score_scale(float scale) {
+    require(std::isfinite(scale) && scale > 0.0F, "the score scale must be above 0");
+    return static_cast<float>(static_cast<double>(scale) / std::log(2.0));
+}
+
+struct AttendPlan {
+    uint32_t splits;
+    size_t partial, marks;  // bytes
+};
+
+AttendPlan attend_plan(const paged::Cache& c, const paged::Batch& b, const paged::Rows& q) {
+    AttendPlan p{b.n_seq ? paged::attend_splits(c, b, q.heads / c.n_head_kv) : 1, 0, 0};
+    if (p.splits > 1) {
+        const size_t n = static_cast<size_t>(p.splits) * q.rows * q.heads;
+        p.partial = n * c.head_dim * sizeof(float);
+        p.marks = n * 2 * sizeof(float);
+    }
+    return p;
+}
+
 }  // namespace
 
 jfh_status jfh_rope_create(const jfh_rope_params* params, jfh_rope** out) {
@@ -169,8 +203,8 @@ jfh_status jfh_paged_append(const jfh_paged_cache* cache, const jfh_paged_batch*
                             const jfh_rows* v, const jfh_rope* rope, const int32_t* positions, void* stream) {
     return guarded([&] {
         const paged::Cache c = cache_of(cache);
-        const paged::Batch b = batch_of(batch, *cache, true);
         const paged::Rows kr = rows_of(k, "k"), vr = rows_of(v, "v");
+        const paged::Batch b = batch_of(batch, *cache, true, kr.rows);
         require(kr.rows == vr.rows, "k and v must have the same rows");
         require(kr.heads == c.n_head_kv && vr.heads == c.n_head_kv && kr.head_dim == c.head_dim && vr.head_dim == c.head_dim,
                 "k and v must have the cache's heads and head dim");
@@ -182,5 +216,43 @@ jfh_status jfh_paged_append(const jfh_paged_cache* cache, const jfh_paged_batch*
         check(paged::launch_append(rope ? &rope->rotation : nullptr, c, b, kr, vr, positions,
                                    static_cast<hipStream_t>(stream)),
               "append rows");
+    });
+}
+
+jfh_status jfh_paged_attention_workspace(const jfh_paged_cache* cache, const jfh_paged_batch* batch, const jfh_rows* q,
+                                         size_t* bytes) {
+    return guarded([&] {
+        require(bytes != nullptr, "an output for the workspace's size is required");
+        const paged::Cache c = cache_of(cache);
+        const paged::Rows x = attended(q, c, "q");
+        const AttendPlan p = attend_plan(c, batch_of(batch, *cache, true, x.rows), x);
+        *bytes = p.partial + p.marks;
+    });
+}
+
+jfh_status jfh_paged_attention(const jfh_paged_cache* cache, const jfh_paged_batch* batch, const jfh_rows* q, float scale,
+                               uint32_t causal, const jfh_rows* out, float* lse, void* workspace, size_t workspace_bytes,
+                               void* stream) {
+    return guarded([&] {
+        paged::Attend a{};
+        a.cache = cache_of(cache);
+        a.q = attended(q, a.cache, "q");
+        a.batch = batch_of(batch, *cache, true, a.q.rows);
+        a.out = attended(out, a.cache, "out");
+        require(a.q.rows == a.out.rows && a.q.heads == a.out.heads, "q and out must have the same rows and heads");
+        require(aligned(lse, 4), "lse must be aligned");
+        a.lse = lse;
+        a.scale_log2 = score_scale(scale);
+        a.causal = causal ? 1U : 0U;
+        if (a.q.rows == 0 || a.batch.n_seq == 0 || a.batch.max_rows == 0) return;
+        const AttendPlan p = attend_plan(a.cache, a.batch, a.q);
+        require(workspace_bytes >= p.partial + p.marks && (p.splits == 1 || workspace) && aligned(workspace, 16),
+                "attention of this step needs " + std::to_string(p.partial + p.marks) +
+                    " bytes of workspace, 16-byte aligned");
+        a.splits = p.splits;
+        a.partial = static_cast<float*>(workspace);
+        a.marks = a.partial + p.partial / sizeof(float);
+        const OnDevice guard(cache->device);
+        check(paged::launch_attend(a, static_cast<hipStream_t>(stream)), "attention over pages");
     });
 }

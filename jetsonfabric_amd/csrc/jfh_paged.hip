@@ -13,6 +13,8 @@ using half8 = _Float16 __attribute__((ext_vector_type(8)));
 using bhalf8 = __bf16 __attribute__((ext_vector_type(8)));
 using float4v = float __attribute__((ext_vector_type(4)));
 
+constexpr float kLn2 = 0.693147180559945309F;
+
 enum : uint32_t { kF32 = 1, kF16 = 2, kBF16 = 3 };
 
 template <typename... KArgs, typename... Args>
@@ -222,6 +224,409 @@ RowGrid row_grid(uint32_t rows, uint64_t tasks) {
     return {dim3(rows, static_cast<uint32_t>(parts < 64 ? parts : 64)), 1};
 }
 
+// ---------------------------------------------------------------- attention
+
+template <typename T> struct Values;
+template <> struct Values<_Float16> {
+    using v8 = half8;
+    static constexpr uint32_t kExponent = 0x7C00;
+    static __device__ __forceinline__ float4v mfma16(v8 a, v8 b, float4v c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+    }
+};
+template <> struct Values<__bf16> {
+    using v8 = bhalf8;
+    static constexpr uint32_t kExponent = 0x7F80;
+    static __device__ __forceinline__ float4v mfma16(v8 a, v8 b, float4v c) {
+        return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+    }
+};
+
+// Over the four lanes l, l ^ 16, l ^ 32, l ^ 48.
+__device__ __forceinline__ float groups_max(float v) {
+    const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
+__device__ __forceinline__ float groups_sum(float v) {
+    const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
+}
+
+// Whether one of two 16-bit values is infinite or NaN.
+template <typename T>
+__device__ __forceinline__ bool nonfinite(uint32_t two) {
+    constexpr uint32_t e = Values<T>::kExponent;
+    return (two & e) == e || (two & (e << 16)) == (e << 16);
+}
+
+// sum + v p where v may hold infinities and NaN in rows that some columns of p do not see: a weight of 0 must leave them
+// out. Their share comes from products of their marks with `seen` (1 where a column sees the row), which count them.
+template <typename T>
+__device__ __forceinline__ float4v weighted_nonfinite(typename Values<T>::v8 v, typename Values<T>::v8 p,
+                                                      typename Values<T>::v8 seen, float4v sum) {
+    typename Values<T>::v8 rest, pos, neg, nan;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float x = static_cast<float>(v[i]);
+        const bool finite = fabsf(x) < INFINITY;
+        rest[i] = finite ? v[i] : static_cast<T>(0.0F);
+        pos[i] = static_cast<T>(x == INFINITY ? 1.0F : 0.0F);
+        neg[i] = static_cast<T>(x == -INFINITY ? 1.0F : 0.0F);
+        nan[i] = static_cast<T>(x != x ? 1.0F : 0.0F);
+    }
+    const float4v zero{0.0F, 0.0F, 0.0F, 0.0F};
+    const float4v a = Values<T>::mfma16(pos, seen, zero), b = Values<T>::mfma16(neg, seen, zero),
+                  c = Values<T>::mfma16(nan, seen, zero);
+    sum = Values<T>::mfma16(rest, p, sum);
+#pragma unroll
+    for (int r = 0; r < 4; ++r) {
+        if (a[r] > 0.0F) sum[r] += INFINITY;
+        if (b[r] > 0.0F) sum[r] -= INFINITY;
+        if (c[r] > 0.0F) sum[r] = NAN;
+    }
+    return sum;
+}
+
+// Column c of eight rows of 16-bit values, two to a word.
+template <int VW>
+__device__ __forceinline__ uint4 column(const uint32_t (&v)[8][VW], int c) {
+    const uint32_t pick = c % 2 ? 0x07060302U : 0x05040100U;
+    return uint4{__builtin_amdgcn_perm(v[1][c / 2], v[0][c / 2], pick), __builtin_amdgcn_perm(v[3][c / 2], v[2][c / 2], pick),
+                 __builtin_amdgcn_perm(v[5][c / 2], v[4][c / 2], pick), __builtin_amdgcn_perm(v[7][c / 2], v[6][c / 2], pick)};
+}
+
+// Weight of sums with maximum m among others with maximum `now`. A part that has seen nothing (l = 0) weighs nothing; one
+// whose scores are NaN (m = -inf, l NaN) goes on as such.
+__device__ __forceinline__ float split_share(float m, float l, float now) {
+    return l == 0.0F ? 0.0F : m == -INFINITY ? 1.0F : exp2f(m - now);
+}
+
+constexpr int kAttendThreads = 256;
+constexpr int kAttendWaves = 4;
+constexpr int kFewKeys = 32;    // keys of a wave's tile
+constexpr float kRescale = 8.0F;  // a row's running maximum is raised when a tile exceeds it by this (base 2)
+
+// Query m of a K/V head's rows * group queries is head m % group of the sequence's row m / group.
+struct Query {
+    int row, head;
+};
+__device__ __forceinline__ Query query_of(int m, int group, uint32_t kv_head) {
+    const int row = m / group;
+    return Query{row, static_cast<int>(kv_head) * group + (m - row * group)};
+}
+
+// Few query rows: o = softmax(scale q K^T) V for up to 16 MT queries of a K/V head, 4 waves that divide its keys.
+//
+// The bytes of K and V bound it. A wave takes tiles of 32 keys from global memory to registers, in the layout of the
+// rows: S^T = K Q^T on 16x16x32 products has a K row's 16 bytes per lane as its A operand. O^T += V^T P^T wants 8 keys of
+// one column per lane; lane (i, g) loads rows 16 u + 4 g + r (u = 0, 1, r = 0..3), columns VEC i .. VEC i + VEC - 1, and
+// 16-bit permutes of those rows give the operands of VEC products, the c-th of columns VEC i + c. The keys of lane group g
+// are those whose scores the group holds after S^T, so P needs no exchange between lanes. No LDS on the way.
+// Running maximum and sum are f32, base 2; P is rounded to the cache's type for the product (half a step per weight, as
+// the output), its sum is not. A row's maximum is raised only when a tile exceeds it by 2^8: P stays far below 65504.
+template <typename T, int HDP, int MT>
+__global__ __launch_bounds__(kAttendThreads, HDP * MT <= 128 ? 2 : 1) void k_attend_few(Attend a, int group) {
+    using V = Values<T>;
+    using v8 = typename V::v8;
+    constexpr int VEC = HDP / 16;   // columns per lane of V
+    constexpr int KC = HDP / 32;    // products per 16 keys of S^T
+    constexpr int VW = VEC / 2;     // words per lane and V row
+    constexpr int kChunk = VW < 4 ? VW : 4;  // words of one load
+    constexpr int OS = HDP + 4;     // floats per query of the waves' sums in LDS
+    __shared__ float part_o[kAttendWaves][16][OS];
+    __shared__ float part_m[kAttendWaves][16], part_l[kAttendWaves][16];
+    __shared__ uint4 q_lds[MT][KC][64];
+
+    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+    const int i = lane % 16, g = lane / 16;
+    const uint32_t pairs = a.cache.n_head_kv * a.batch.n_seq;  // K/V heads of sequences
+    const uint32_t split = blockIdx.x % a.splits, pair = blockIdx.x / a.splits % pairs;
+    const uint32_t h = pair % a.cache.n_head_kv, s = pair / a.cache.n_head_kv;
+    const int m0 = static_cast<int>(blockIdx.x / a.splits / pairs) * 16 * MT;
+    const Span span = sequence_span(a.batch, a.q.rows, s);
+    const int queries = span.rows * group;
+    if (m0 >= queries) return;
+    const int dim = static_cast<int>(a.cache.head_dim);
+    const int first = span.len - span.rows;  // slot of row 0
+
+    // queries to LDS in operand order, zeros behind the last one and beyond head_dim
+    for (int t = threadIdx.x; t < MT * KC * 64; t += kAttendThreads) {
+        const int l = t % 64, c = t / 64 % KC, mt = t / 64 / KC;
+        const int m = m0 + 16 * mt + l % 16, d = 32 * c + 8 * (l / 16);
+        uint4 x{0, 0, 0, 0};
+        if (m < queries && d < dim) {
+            const Query q = query_of(m, group, h);
+            x = *reinterpret_cast<const uint4*>(static_cast<const T*>(a.q.data) + (span.row0 + q.row) * a.q.row_stride +
+                                                q.head * a.q.head_stride + d);
+        }
+        q_lds[mt][c][l] = x;
+    }
+    __syncthreads();
+
+    int limit[MT];  // slots that the lane's query sees: 0 .. limit - 1
+    int least = span.len;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+        const int m = m0 + 16 * mt + i;
+        limit[mt] = m < queries && a.causal ? max(0, first + m / group + 1) : span.len;
+    }
+    if (a.causal) least = max(0, first + m0 / group + 1);
+    const int last = min(queries, m0 + 16 * MT) - 1;
+    const int end = a.causal ? max(0, first + last / group + 1) : span.len;  // slots that any query here sees
+
+    // the split's tiles: equal parts of the sequence's
+    const int tiles = (span.len + kFewKeys - 1) / kFewKeys;
+    const int per = (tiles + static_cast<int>(a.splits) - 1) / static_cast<int>(a.splits);
+    const int t0 = static_cast<int>(split) * per, t1 = min(min(tiles, t0 + per), (end + kFewKeys - 1) / kFewKeys);
+
+    float4v o[MT][VEC];
+    float top[MT], sum[MT];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+        top[mt] = -INFINITY;
+        sum[mt] = 0.0F;
+#pragma unroll
+        for (int c = 0; c < VEC; ++c) o[mt][c] = float4v{0.0F, 0.0F, 0.0F, 0.0F};
+    }
+
+    const T* k_head = static_cast<const T*>(a.cache.k) + h * a.cache.head_stride;
+    const T* v_head = static_cast<const T*>(a.cache.v) + h * a.cache.head_stride;
+
+    for (int t = t0 + wave; t < t1; t += kAttendWaves) {
+        const int base = t * kFewKeys;
+        // offsets of the lane's K rows; -1: not in use, or on an absent page
+        int64_t at[2];
+        uint32_t present[2];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int slot = base + 16 * u + i;
+            at[u] = -1;
+            if (slot < end) {
+                const int page = page_of(a.cache, a.batch, s, slot);
+                if (page >= 0) at[u] = slot_offset(a.cache, page, slot);
+            }
+            present[u] = static_cast<uint32_t>(__ballot(at[u] >= 0)) & 0xFFFFU;
+        }
+        const bool all_present = (present[0] & present[1]) == 0xFFFFU;
+        const bool hidden = base + kFewKeys > least;  // some query here does not see some of the tile
+        uint4 k[2][KC];
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const T* row = k_head + max(at[u], static_cast<int64_t>(0));
+#pragma unroll
+            for (int c = 0; c < KC; ++c) {
+                const int d = 32 * c + 8 * g;
+                k[u][c] = *reinterpret_cast<const uint4*>(row + (d < dim ? d : 0));
+                if (d >= dim) k[u][c] = uint4{0, 0, 0, 0};
+            }
+        }
+        uint32_t v[8][VW];
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const int64_t row = __shfl(at[j / 4], 4 * g + j % 4);
+#pragma unroll
+            for (int w = 0; w < VW; w += kChunk) {
+                const int d = VEC * i + 2 * w;
+                const T* from = v_head + max(row, static_cast<int64_t>(0)) + (d < dim ? d : 0);
+                __builtin_memcpy(&v[j][w], __builtin_assume_aligned(from, 4 * kChunk), 4 * kChunk);
+                // what is not there must be a number: its weight is 0
+                if (row < 0 || d >= dim) {
+#pragma unroll
+                    for (int e = 0; e < kChunk; ++e) v[j][w + e] = 0;
+                }
+            }
+        }
+        bool odd = false;
+        if (hidden) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+#pragma unroll
+                for (int w = 0; w < VW; ++w) odd |= nonfinite<T>(v[j][w]);
+            }
+        }
+        const bool careful = __ballot(odd) != 0;
+
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+            float4v sc[2] = {float4v{0.0F, 0.0F, 0.0F, 0.0F}, float4v{0.0F, 0.0F, 0.0F, 0.0F}};
+#pragma unroll
+            for (int c = 0; c < KC; ++c) {
+                const v8 q = __builtin_bit_cast(v8, q_lds[mt][c][lane]);
+#pragma unroll
+                for (int u = 0; u < 2; ++u) sc[u] = V::mfma16(__builtin_bit_cast(v8, k[u][c]), q, sc[u]);
+            }
+            // scores of keys base + 16 u + 4 g + r, query i
+            uint32_t seen = 0xFF;
+            if (!all_present || hidden) {
+                seen = 0;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int u = j / 4, e = 4 * g + j % 4;
+                    const bool sees = (present[u] >> e & 1U) && base + 16 * u + e < limit[mt];
+                    seen |= static_cast<uint32_t>(sees) << j;
+                    if (!sees) sc[u][j % 4] = -INFINITY;
+                }
+            }
+            float most = sc[0][0];
+#pragma unroll
+            for (int j = 1; j < 8; ++j) most = fmaxf(most, sc[j / 4][j % 4]);
+            most = groups_max(most) * a.scale_log2;
+            if (__ballot(most > top[mt] + kRescale)) {
+                const float now = fmaxf(top[mt], most);
+                const float shrink = now == -INFINITY ? 1.0F : exp2f(top[mt] - now);
+                top[mt] = now;
+                sum[mt] *= shrink;
+#pragma unroll
+                for (int c = 0; c < VEC; ++c) o[mt][c] *= shrink;
+            }
+            const float ref = top[mt] == -INFINITY ? 0.0F : top[mt];
+            v8 p;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float w = __builtin_amdgcn_exp2f(fmaf(sc[j / 4][j % 4], a.scale_log2, -ref));
+                sum[mt] += w;
+                p[j] = static_cast<T>(w);
+            }
+            if (!careful) {
+#pragma unroll
+                for (int c = 0; c < VEC; ++c) {
+                    o[mt][c] = V::mfma16(__builtin_bit_cast(v8, column<VW>(v, c)), p, o[mt][c]);
+                }
+            } else {
+                v8 seen_mark;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) seen_mark[j] = static_cast<T>(seen >> j & 1U ? 1.0F : 0.0F);
+#pragma unroll
+                for (int c = 0; c < VEC; ++c) {
+                    o[mt][c] = weighted_nonfinite<T>(__builtin_bit_cast(v8, column<VW>(v, c)), p, seen_mark, o[mt][c]);
+                }
+            }
+        }
+    }
+
+    // the waves' sums, 16 queries at a time
+    const int rows_heads = static_cast<int>(a.q.rows * a.q.heads);
+    for (int mt = 0; mt < MT; ++mt) {
+        if (m0 + 16 * mt >= queries) break;
+        __syncthreads();
+#pragma unroll
+        for (int n = 0; n < MT; ++n) {
+            if (n != mt) continue;
+            const float l = groups_sum(sum[n]);
+            if (g == 0) part_m[wave][i] = top[n], part_l[wave][i] = l;
+            // lane (i, g) holds columns VEC (4 g + r) + c of query i
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+#pragma unroll
+                for (int c = 0; c < VEC; c += 4) {
+                    *reinterpret_cast<float4v*>(&part_o[wave][i][VEC * (4 * g + r) + c]) =
+                        float4v{o[n][c][r], o[n][c + 1][r], o[n][c + 2][r], o[n][c + 3][r]};
+                }
+            }
+        }
+        __syncthreads();
+        // 16 threads per query
+        const int n = threadIdx.x / 16, m = m0 + 16 * mt + n;
+        if (m < queries) {
+            float now = part_m[0][n];
+#pragma unroll
+            for (int w = 1; w < kAttendWaves; ++w) now = fmaxf(now, part_m[w][n]);
+            float share[kAttendWaves], l = 0.0F;
+#pragma unroll
+            for (int w = 0; w < kAttendWaves; ++w) {
+                share[w] = split_share(part_m[w][n], part_l[w][n], now);
+                l += part_l[w][n] * share[w];
+            }
+            const Query q = query_of(m, group, h);
+            const int64_t row = span.row0 + q.row;
+            const int64_t at = row * a.q.heads + q.head;
+            const bool whole = a.splits == 1;
+            const float scale = !whole ? 1.0F : l == 0.0F ? 0.0F : 1.0F / l;
+            for (int d = threadIdx.x % 16 * 8; d < dim; d += 128) {
+                float x[8];
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    x[e] = 0.0F;
+#pragma unroll
+                    for (int w = 0; w < kAttendWaves; ++w) {
+                        if (share[w] != 0.0F) x[e] += part_o[w][n][d + e] * share[w];
+                    }
+                    x[e] *= scale;
+                }
+                if (whole) {
+                    store(a.out.data, row * a.out.row_stride + q.head * a.out.head_stride + d, a.out.type, x);
+                } else {
+                    store(a.partial, (static_cast<int64_t>(split) * rows_heads + at) * dim + d, kF32, x);
+                }
+            }
+            if (threadIdx.x % 16 == 0) {
+                if (whole) {
+                    if (a.lse) a.lse[at] = now * kLn2 + logf(l);
+                } else {
+                    *reinterpret_cast<float2*>(a.marks + 2 * (static_cast<int64_t>(split) * rows_heads + at)) = float2{now, l};
+                }
+            }
+        }
+    }
+}
+
+// Joins the splits of one row and head: 32 (head dims up to 128: 16) threads hold a partial's columns 8 each, the others
+// take other splits. Rows of no sequence are left as they are.
+constexpr int kJoinThreads = 256;
+
+__global__ __launch_bounds__(kJoinThreads) void k_attend_join(Attend a) {
+    __shared__ float part[16][kMaxHeadDim];
+    __shared__ float part_l[16];
+    const int64_t at = blockIdx.x, all = static_cast<int64_t>(a.q.rows) * a.q.heads;
+    const int row = static_cast<int>(at / a.q.heads), head = static_cast<int>(at % a.q.heads);
+    Span span;
+    if (sequence_of(a.batch, a.q.rows, row, &span) < 0) return;
+    const int dim = static_cast<int>(a.cache.head_dim), splits = static_cast<int>(a.splits);
+    const float2* marks = reinterpret_cast<const float2*>(a.marks) + at;
+    float now = -INFINITY;
+    for (int s = threadIdx.x % 64; s < splits; s += 64) now = fmaxf(now, marks[s * all].x);
+#pragma unroll
+    for (int o = 32; o; o /= 2) now = fmaxf(now, __shfl_xor(now, o));
+
+    const int wide = dim <= 128 ? 16 : 32, takers = kJoinThreads / wide;
+    const int d = threadIdx.x % wide * 8, taker = threadIdx.x / wide;
+    float x[8] = {}, l = 0.0F;
+    for (int s = taker; s < splits; s += takers) {
+        const float2 mark = marks[s * all];
+        if (mark.y == 0.0F) continue;
+        const float share = split_share(mark.x, mark.y, now);
+        l += mark.y * share;
+        if (d < dim) {
+            float y[8];
+            load(a.partial, (s * all + at) * dim + d, kF32, y);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) x[e] += y[e] * share;
+        }
+    }
+    if (d < dim) store(part[taker], d, kF32, x);
+    if (d == 0) part_l[taker] = l;
+    __syncthreads();
+    if (static_cast<int>(threadIdx.x) >= wide) return;
+    l = 0.0F;
+    for (int t = 0; t < takers; ++t) l += part_l[t];
+    if (d == 0 && a.lse) a.lse[at] = now * kLn2 + logf(l);
+    if (d >= dim) return;
+    for (int e = 0; e < 8; ++e) x[e] = 0.0F;
+    for (int t = 0; t < takers; ++t) {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) x[e] += part[t][d + e];
+    }
+    const float scale = l == 0.0F ? 0.0F : 1.0F / l;
+#pragma unroll
+    for (int e = 0; e < 8; ++e) x[e] *= scale;
+    store(a.out.data, row * a.out.row_stride + head * a.out.head_stride + d, a.out.type, x);
+}
+
 }  // namespace
 
 hipError_t launch_rotate(const Rotation& r, const Rows& x, const int32_t* positions, const Rows& y, hipStream_t stream) {
@@ -238,6 +643,51 @@ hipError_t launch_append(const Rotation* rotation, const Cache& c, const Batch& 
     const uint64_t units = (r.n_rot / 2 + (k.head_dim - r.n_rot) + v.head_dim) / (wide ? 8 : 1) + 1;
     const RowGrid g = row_grid(k.rows, c.n_head_kv * units);
     return launch(wide ? k_append<8> : k_append<1>, g.grid, dim3(kRotateThreads), stream, r, c, b, k, v, positions, g.rows);
+}
+
+namespace {
+
+// Tiles of 16 queries per work-group: as many as a sequence may have, up to what the registers hold (4; 2 of wide heads).
+uint32_t few_tiles(uint32_t head_dim, uint64_t queries) { return queries <= 16 ? 1 : queries <= 32 || head_dim > 128 ? 2 : 4; }
+
+template <typename T, int HDP>
+hipError_t attend_few(const Attend& a, hipStream_t stream) {
+    const int group = static_cast<int>(a.q.heads / a.cache.n_head_kv);
+    const uint64_t queries = static_cast<uint64_t>(a.batch.max_rows) * group;
+    const uint32_t mt = few_tiles(a.cache.head_dim, queries);
+    const uint64_t groups = (queries + 16 * mt - 1) / (16 * mt) * a.cache.n_head_kv * a.batch.n_seq * a.splits;
+    if (groups > 0x7FFFFFFF) return hipErrorInvalidConfiguration;
+    const dim3 grid(static_cast<uint32_t>(groups));
+    const dim3 block(kAttendThreads);
+    if (mt == 1) return launch(k_attend_few<T, HDP, 1>, grid, block, stream, a, group);
+    if (mt == 2) return launch(k_attend_few<T, HDP, 2>, grid, block, stream, a, group);
+    if constexpr (HDP <= 128) return launch(k_attend_few<T, HDP, 4>, grid, block, stream, a, group);
+    return hipErrorInvalidValue;
+}
+
+template <typename T>
+hipError_t attend(const Attend& a, hipStream_t stream) {
+    if (a.cache.head_dim <= 64) return attend_few<T, 64>(a, stream);
+    if (a.cache.head_dim <= 128) return attend_few<T, 128>(a, stream);
+    return attend_few<T, 256>(a, stream);
+}
+
+}  // namespace
+
+uint32_t attend_splits(const Cache& c, const Batch& b, uint32_t group) {
+    const uint64_t queries = static_cast<uint64_t>(b.max_rows) * group;
+    const uint32_t mt = few_tiles(c.head_dim, queries);
+    const uint64_t groups = c.n_head_kv * static_cast<uint64_t>(b.n_seq) * ((queries + 16 * mt - 1) / (16 * mt));
+    // two work-groups per compute unit; a split of fewer than two tiles per wave costs more than it gains
+    const uint64_t wanted = groups ? (2 * kComputeUnits + groups - 1) / groups : 1;
+    const uint64_t most = b.max_length / (2 * kAttendWaves * kFewKeys);
+    return static_cast<uint32_t>(wanted < most ? wanted : most > 0 ? most : 1);
+}
+
+hipError_t launch_attend(const Attend& a, hipStream_t stream) {
+    const hipError_t e = a.cache.type == kF16 ? attend<_Float16>(a, stream) : attend<__bf16>(a, stream);
+    if (e != hipSuccess || a.splits == 1) return e;
+    return launch(k_attend_join, dim3(a.q.rows * a.q.heads), dim3(kJoinThreads), stream, a);
 }
 
 }  // namespace jfh::paged

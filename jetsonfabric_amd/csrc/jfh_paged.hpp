@@ -104,8 +104,24 @@ struct Rotation {
     uint32_t n_rot, interleaved;
 };
 
+struct Attend {
+    Cache cache;
+    Batch batch;
+    Rows q, out;
+    float* lse;       // [rows][heads] or null
+    float* partial;   // [splits][rows * heads][head_dim], unnormalized
+    float* marks;     // [splits][rows * heads][2]: running maximum (base 2) and sum
+    float scale_log2; // scale * log2(e)
+    uint32_t causal, splits;
+};
+
+// Parts that a step's keys are divided into, each a work-group of its own per K/V head and tile of query rows; more than
+// one where the tiles do not fill the chip.
+uint32_t attend_splits(const Cache& c, const Batch& b, uint32_t group);
+
 hipError_t launch_rotate(const Rotation& r, const Rows& x, const int32_t* positions, const Rows& y, hipStream_t stream);
 hipError_t launch_append(const Rotation* r, const Cache& c, const Batch& b, const Rows& k, const Rows& v,
                          const int32_t* positions, hipStream_t stream);
+hipError_t launch_attend(const Attend& a, hipStream_t stream);
 
 }  // namespace jfh::paged

@@ -154,3 +154,24 @@ class PagedCache:
         at = None if positions is None else _array(positions, "positions", "torch.int32", self.device, (k.shape[0],))
         check(library().jfh_paged_append(self.ref, self._of(batch), ctypes.byref(a), ctypes.byref(b),
                                          None if rope is None else rope.handle, at, _stream(self.device)))
+
+    def attend(self, batch: PagedBatch, q, scale: float | None = None, causal: bool = True, out=None, lse=None):
+        """softmax(scale q K^T) V of a step's rows q [rows, heads, head dim] over their sequences' slots
+        (scale 1 / sqrt(head dim) by default) and ln sum exp of the scores, float32 [rows, heads].
+        Returns (out, lse), written where they are given; rows of no sequence are left as they were,
+        zeros in new tensors."""
+        torch = sys.modules["torch"]
+        if out is None:
+            out = torch.zeros_like(q)
+        if lse is None:
+            lse = torch.zeros(q.shape[:2], dtype=torch.float32, device=q.device)
+        a, b = _rows(q, "q", self.device), _rows(out, "out", self.device)
+        at = _array(lse, "lse", "torch.float32", self.device, q.shape[:2])
+        need = ctypes.c_size_t()
+        check(library().jfh_paged_attention_workspace(self.ref, self._of(batch), ctypes.byref(a), ctypes.byref(need)))
+        space = torch.empty(need.value, dtype=torch.uint8, device=q.device) if need.value else None
+        check(library().jfh_paged_attention(self.ref, batch.ref, ctypes.byref(a),
+                                            a.head_dim ** -0.5 if scale is None else scale, int(causal), ctypes.byref(b),
+                                            at, None if space is None else space.data_ptr(), need.value,
+                                            _stream(self.device)))
+        return out, lse

@@ -110,3 +110,67 @@ class Sequences:
             t = self.lens[s] - self.rows[s] + i
             if t >= 0:
                 yield self.starts[s] + i, t
+
+    def poison(self):
+        """NaN and infinities in every slot that no sequence uses, and in the pages of nobody."""
+        used = torch.zeros(self.n_pages, self.page, dtype=torch.bool)
+        for s in range(len(self.rows)):
+            for t in range(self.lens[s]):
+                at = self.slot(s, t)
+                if at is not None:
+                    used[at] = True
+        bad = ~used[:, None, :, None].expand_as(self.k)
+        values = torch.tensor([math.nan, math.inf, -math.inf], dtype=self.dtype).repeat(self.k.numel() // 3 + 1)
+        self.k[bad] = values[:self.k.numel()].reshape(self.k.shape)[bad]
+        self.v[bad] = values[1:self.k.numel() + 1].reshape(self.k.shape)[bad]
+        return self
+
+    def gather(self, s):
+        """K and V [K/V heads, slots, dim] (f64) of a sequence, and which slots are there."""
+        n = self.lens[s]
+        k, v = (torch.zeros(self.kv_heads, n, self.dim, dtype=torch.float64) for _ in range(2))
+        there = torch.zeros(n, dtype=torch.bool)
+        for p in range(-(-n // self.page)):
+            at = self.slot(s, p * self.page)
+            t0, t1 = p * self.page, min(n, (p + 1) * self.page)
+            if at is not None:
+                k[:, t0:t1], v[:, t0:t1] = self.k[at[0], :, :t1 - t0].double(), self.v[at[0], :, :t1 - t0].double()
+                there[t0:t1] = True
+        return k, v, there
+
+    def sees(self, s, causal, there):
+        """[rows, slots] what each new row of a sequence sees."""
+        n, r = self.lens[s], self.rows[s]
+        t = torch.arange(n)
+        end = torch.arange(n - r + 1, n + 1)[:, None] if causal else torch.full((r, 1), n)
+        return (t < end) & there
+
+    def attend(self, q, scale, causal=True):
+        """out, lse (f64) and their bounds for q [rows, heads, dim]."""
+        group = q.shape[1] // self.kv_heads
+        out, lse = torch.zeros(q.shape, dtype=torch.float64), torch.zeros(q.shape[:2], dtype=torch.float64)
+        bound, lse_bound = torch.zeros_like(out), torch.zeros_like(lse)
+        step, tiny = half_step(self.dtype), 2.0**-25 if self.dtype == torch.float16 else 0.0
+        for s in range(len(self.rows)):
+            k, v, there = self.gather(s)
+            sees = self.sees(s, causal, there)
+            r = slice(self.starts[s], self.starts[s + 1])
+            for h in range(q.shape[1]):
+                x, kh, vh = q[r, h].double(), k[h // group], v[h // group]
+                score = (x @ kh.T * scale).masked_fill(~sees, -math.inf)
+                # a score: dim products and sums in f32, its product with the scale and the difference to the maximum
+                off = ((self.dim + 2) * 2.0**-24 * scale * (x.abs() @ kh.abs().T) + 2.0**-22 * score.abs()).masked_fill(~sees, 0)
+                off = off.amax(-1, keepdim=True) if off.shape[1] else torch.zeros(len(x), 1)
+                some = sees.any(-1)
+                lse[r, h] = torch.logsumexp(score, -1)
+                p = torch.where(some[:, None], torch.softmax(score, -1), 0.0)
+                p = torch.where(sees, p, 0.0)
+                n = sees.shape[1]
+                out[r, h] = p @ vh
+                size = p @ vh.abs()
+                # weights: a half step of their rounding, their score, exp2 (2^-22); sums of n terms and 64 parts in f32
+                bound[r, h] = size * (step + 2 * off + 2.0**-21 + (n + 64) * 2.0**-23)
+                bound[r, h] += tiny * (sees.double() @ vh.abs())  # weights below f16's normal range, of a sum of 1 at least
+                bound[r, h] += step * (out[r, h].abs() + bound[r, h]) + 2.0**-25
+                lse_bound[r, h] = off[:, 0] + 2.0**-21 + (n + 64) * 2.0**-23 + 2.0**-22 * lse[r, h].abs().nan_to_num(posinf=0)
+        return out, lse, bound, lse_bound

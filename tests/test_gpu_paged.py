@@ -183,3 +183,125 @@ def test_bounds_leave_out_what_lies_beyond_them():
         page, i = seq.slot(s, t)
         want[page, :, i] = v[row]
     assert torch.equal(vp.cpu(), want)
+
+
+# ---------------------------------------------------------------- attention
+
+def attended(seq, heads, causal=True, scale=None, q=None, lse=True):
+    """Attention of random queries over seq's cache, checked; returns (q, out, lse) on the CPU."""
+    scale = seq.dim ** -0.5 if scale is None else scale
+    q = normal(seq.total, heads, seq.dim, seed=77, std=1.5).to(seq.dtype) if q is None else q
+    kp, vp, _, _, table, lengths, starts = seq.to_gpu()
+    cache = jf.PagedCache(kp, vp)
+    batch = jf.PagedBatch(table, lengths, starts, seq.max_rows, seq.max_length)
+    out = torch.full(q.shape, 7.0, dtype=seq.dtype, device="cuda")
+    got, got_lse = cache.attend(batch, q.cuda(), scale, causal, out=out,
+                                lse=torch.full(q.shape[:2], 5.0, device="cuda"))
+    assert got is out
+    want, want_lse, bound, lse_bound = seq.attend(q, scale, causal)
+    n = seq.starts[-1]
+    within(out[:n].cpu(), want[:n], bound[:n])
+    some = want_lse[:n] > -float("inf")
+    assert torch.equal(got_lse[:n].cpu()[~some], want_lse[:n].float()[~some])
+    within(got_lse[:n].cpu()[some], want_lse[:n][some], lse_bound[:n][some])
+    assert (out[n:] == 7).all() and (got_lse[n:] == 5).all()  # rows of no sequence
+    return q, out.cpu(), got_lse.cpu()
+
+
+ATTENDS = [
+    # rows, lengths, heads, K/V heads, dim, page, what else
+    ([1], [1], 1, 1, 64, 1, {}),
+    ([1], [256], 12, 2, 128, 16, {}),
+    ([1, 1, 1], [31, 32, 33], 28, 4, 128, 16, {"order": "tokens"}),
+    ([1] * 5, [1, 700, 17, 64, 129], 8, 2, 64, 32, {"absent": [(1, 3), (3, 0), (3, 1)]}),
+    ([1, 0, 1], [5000, 3, 4097], 40, 8, 128, 64, {"pad_rows": 2}),
+    ([9, 9], [1033, 9], 40, 8, 128, 16, {}),
+    ([5, 3, 0, 7], [300, 3, 5, 2], 7, 1, 96, 8, {"pad_rows": 3, "order": "padded"}),
+    ([4, 2], [2000, 2], 4, 1, 256, 256, {}),
+    ([2, 6], [70, 100], 12, 2, 200, 4, {"absent": [(0, 5), (1, 24)]}),
+    ([33, 1, 130], [33, 900, 400], 6, 3, 80, 2, {"absent": [(2, 0), (2, 7)], "wide_table": 3}),
+    ([100], [100], 28, 4, 128, 16, {}),
+    ([77, 200], [1500, 333], 10, 2, 64, 64, {"order": "tokens", "pad_rows": 1}),
+    ([3], [40], 16, 16, 8, 8, {}),
+    ([1], [9000], 4, 1, 72, 1, {}),
+    ([20], [65], 3, 1, 256, 16, {}),
+]
+
+
+@pytest.mark.parametrize("rows,lens,heads,kv,dim,page,more", ATTENDS)
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+def test_attention(rows, lens, heads, kv, dim, page, more, kind):
+    for causal in (True, False):
+        attended(Sequences(rows, lens, kv, dim, page, TYPES[kind], seed=len(rows), **more).poison(), heads, causal)
+
+
+@pytest.mark.parametrize("rows", [1, 40])
+def test_attention_of_rows_that_see_nothing(rows):
+    """Sequences without slots, with fewer slots than rows, with absent pages alone; other rows beside them."""
+    seq = Sequences([rows, rows, rows, rows], [0, rows // 2, 48, 50], 2, 64, 16, torch.float16, seed=3,
+                    absent=[(2, 0), (2, 1), (2, 2), (2, 3)]).poison()
+    q, out, lse = attended(seq, 6)
+    assert (out[:rows] == 0).all() and (lse[:rows] == -float("inf")).all()
+    assert (out[2 * rows:3 * rows] == 0).all()
+
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("rows", [6, 150])
+def test_attention_does_not_take_hidden_infinities(kind, rows):
+    """Later rows' K and V are infinite or NaN: rows that do not see them are as if those were numbers."""
+    seq = Sequences([rows], [rows + 37], 1, 64, 16, TYPES[kind], seed=8)
+    at = {t: seq.slot(0, t) for t in range(37, rows + 37)}
+    q = normal(rows, 4, 64, seed=9).to(seq.dtype)
+    clean = seq.attend(q, 0.125)
+    for t, v in ((39, float("inf")), (40, float("nan")), (rows + 36, -float("inf"))):
+        seq.v[at[t][0], 0, at[t][1], 3] = v
+    seq.k[at[41][0], 0, at[41][1], 5] = float("nan")
+    kp, vp, _, _, table, lengths, starts = seq.to_gpu()
+    out, lse = jf.PagedCache(kp, vp).attend(jf.PagedBatch(table, lengths, starts, rows, rows + 37), q.cuda(), 0.125)
+    out = out.cpu()
+    seen = torch.arange(64) != 3
+    within(out[:4][..., seen], clean[0][:4][..., seen], clean[2][:4][..., seen])
+    within(out[:2], clean[0][:2], clean[2][:2])
+    assert (out[2, :, 3] == float("inf")).all()       # row 2 sees slot 39
+    assert torch.isnan(out[3, :, 3]).all()            # and row 3 a NaN
+    assert torch.isnan(out[4:]).all()                 # a NaN score makes the row NaN
+    assert torch.isnan(lse[4:]).all() and torch.isfinite(lse[:4]).all()
+
+
+def test_attention_of_infinite_queries_and_scores():
+    seq = Sequences([3, 1], [40, 50], 1, 64, 16, torch.float16, seed=1)
+    q = normal(4, 2, 64, seed=2).half()
+    want = seq.attend(q, 0.125)
+    q[1, 0, 0], q[2, 1, 7] = float("nan"), float("inf")
+    kp, vp, _, _, table, lengths, starts = seq.to_gpu()
+    out, _ = jf.PagedCache(kp, vp).attend(jf.PagedBatch(table, lengths, starts, 3, 50), q.cuda(), 0.125)
+    out = out.cpu()
+    assert torch.isnan(out[1, 0]).all() and torch.isnan(out[2, 1]).all()
+    for r, h in ((0, 0), (0, 1), (1, 1), (2, 0), (3, 0), (3, 1)):
+        within(out[r, h], want[0][r, h], want[2][r, h])
+
+
+@pytest.mark.parametrize("rows", [1, 8, 90])
+def test_attention_of_large_scores(rows):
+    """Scores over hundreds: one slot takes nearly everything; a scale that is not 1 / sqrt(dim)."""
+    seq = Sequences([rows], [777], 2, 128, 16, torch.bfloat16, seed=5)
+    q = normal(rows, 8, 128, seed=6, std=6.0).bfloat16()
+    attended(seq, 8, q=q, scale=0.5)
+    attended(seq, 8, q=q, scale=1e-6)
+
+
+def test_attention_of_strided_rows_on_another_stream():
+    seq = Sequences([3, 2], [80, 300], 2, 64, 16, torch.float16, seed=6)
+    fused = normal(5, 14 * 64, seed=3).half()
+    view = fused.unflatten(1, (14, 64))[:, 2:10]
+    want = seq.attend(view, 0.125)
+    kp, vp, _, _, table, lengths, starts = seq.to_gpu()
+    cache, batch = jf.PagedCache(kp, vp), jf.PagedBatch(table, lengths, starts, 3, 300)
+    gpu = fused.cuda()
+    out = torch.zeros(5, 8, 3 * 64, dtype=torch.float16, device="cuda")[..., 64:128]
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        cache.attend(batch, gpu.unflatten(1, (14, 64))[:, 2:10], 0.125, out=out)
+    stream.synchronize()
+    within(out.cpu(), want[0], want[2])

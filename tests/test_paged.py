@@ -82,6 +82,47 @@ def test_appends_ask_for_positions():
     refused(lambda: _append(rope=jf.Rope(66).handle), "more values than a head")
 
 
+def _attend(c=None, b=None, q=None, out=None, scale=0.125, lse=AT, space=AT, size=1 << 40):
+    return jf.library().jfh_paged_attention(ctypes.byref(c or cache()), ctypes.byref(b or batch()), ctypes.byref(q or rows()),
+                                            scale, 1, ctypes.byref(out or rows()), lse, space, size, None)
+
+
+@pytest.mark.parametrize("change,match", BAD_CACHES)
+def test_attended_caches_are_checked(change, match):
+    refused(lambda: _attend(c=cache(**change)), match)
+
+
+@pytest.mark.parametrize("change,match", BAD_BATCHES)
+def test_attended_batches_are_checked(change, match):
+    refused(lambda: _attend(b=batch(**change)), match)
+
+
+@pytest.mark.parametrize("change,match", [
+    ({"type": 3}, "cache's type"), ({"type": 1}, "cache's type"), ({"head_dim": 32}, "head dim"), ({"n_head": 6}, "multiple of"),
+    ({"data": AT + 8}, "16-byte"), ({"row_stride": 260}, "16-byte"), ({"head_stride": 4}, "16-byte"), ({"n_rows": 2}, "same rows"),
+    ({"n_head": 8}, "same rows and heads"), ({"n_rows": (1 << 31) - 1}, "more rows"), ({"data": None}, "missing")])
+def test_attention_rows_are_checked(change, match):
+    refused(lambda: _attend(q=rows(**change)), match)
+    if "same rows" not in match:
+        refused(lambda: _attend(out=rows(**change)), match)
+
+
+def test_attention_arguments_are_checked():
+    for scale in (0.0, -1.0, float("nan"), float("inf")):
+        refused(lambda: _attend(scale=scale), "score scale")
+    refused(lambda: _attend(lse=AT + 2), "lse")
+    long = {"b": batch(n_seq=1, table_stride=4096, max_length=65536), "c": cache(page_size=16)}
+    need = ctypes.c_size_t()
+    check(jf.library().jfh_paged_attention_workspace(ctypes.byref(long["c"]), ctypes.byref(long["b"]), ctypes.byref(rows()),
+                                                     ctypes.byref(need)))
+    assert need.value > 0
+    refused(lambda: _attend(**long, size=need.value - 1), f"needs {need.value} bytes")
+    refused(lambda: _attend(**long, space=None), "workspace")
+    refused(lambda: _attend(**long, space=AT + 4), "16-byte")
+    check(_attend(q=rows(n_rows=0), out=rows(n_rows=0)))
+    check(_attend(b=batch(n_seq=0)))
+
+
 def test_missing_arguments_are_refused():
     lib = jf.library()
     assert lib.jfh_paged_append(None, ctypes.byref(batch()), ctypes.byref(rows()), ctypes.byref(rows()), None, AT, None).code == 1
