@@ -382,7 +382,8 @@ jfh_status jfh_engine_profile_batch(jfh_engine * engine, jfh_session * const * s
 /* Operators of a decoder layer on the caller's device memory, for serving code
  * that keeps its K/V caches in pages (no counterpart in the reference, whose
  * sessions own one contiguous cache each): rotary positions, new rows written
- * into the pages, attention over them. They stand next to
+ * into the pages, attention over them, and caches cut back to a budget by the
+ * attention that their positions have had. They stand next to
  * jfh_engine_matmul_noalloc, which gives such code the weight products.
  *
  * Every call checks its arguments, enqueues kernels on the caller's stream
@@ -517,6 +518,32 @@ jfh_status jfh_paged_attention_workspace(const jfh_paged_cache * cache, const jf
 jfh_status jfh_paged_attention(const jfh_paged_cache * cache, const jfh_paged_batch * batch, const jfh_rows * q,
                                float scale, uint32_t causal, const jfh_rows * out, float * lse, void * workspace,
                                size_t workspace_bytes, void * stream);
+
+/* Adds to the cache's weights what attention of the step's rows q gives each
+ * position: weights[slot] += sum of exp(scale q k - lse) over the rows that see
+ * it and the heads of its K/V head, with lse, scale and causal as
+ * jfh_paged_attention had them (q may hold a part of its rows: the batch's row
+ * starts say which, at the sequences' last slots). f32, in one order whatever
+ * the launch; a row whose lse is -inf adds nothing. No two sequences may share
+ * a page. */
+jfh_status jfh_paged_weigh(const jfh_paged_cache * cache, const jfh_paged_batch * batch, const jfh_rows * q,
+                           const float * lse, float scale, uint32_t causal, void * stream);
+
+/* Cuts every sequence of more than `budget` slots down to `budget`, for each
+ * K/V head by itself: of its slots the first `budget` stay in the order
+ * protected (position below n_first, or among the n_recent up to the newest),
+ * then heavier, then lower slot; NaN is lighter than any weight. Those that stay
+ * at slots from `budget` on move into the slots of those that go, in ascending
+ * order, with their weights and positions; nothing else moves, and lengths
+ * become `budget`. Slots on absent pages are never moved to or from. The cache
+ * needs weights and positions; no two sequences may share a page; the batch's
+ * row_starts and max_rows are not used (row_starts may be NULL). Keys keep the
+ * rotation of their positions, so that new rows go on at the positions of the
+ * text. workspace as for jfh_paged_attention. */
+jfh_status jfh_paged_evict_workspace(const jfh_paged_cache * cache, const jfh_paged_batch * batch, uint32_t budget,
+                                     size_t * bytes);
+jfh_status jfh_paged_evict(const jfh_paged_cache * cache, const jfh_paged_batch * batch, uint32_t budget, uint32_t n_first,
+                           uint32_t n_recent, void * workspace, size_t workspace_bytes, void * stream);
 
 /* ---------------------------------------------------------------- tokenizer */
 

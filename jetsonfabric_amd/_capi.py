@@ -191,6 +191,11 @@ SIGNATURES = {
                                                POINTER(c_size_t)]),
     "jfh_paged_attention": (Status, [POINTER(PagedCache), POINTER(PagedBatch), POINTER(Rows), c_float, c_uint32,
                                      POINTER(Rows), c_void_p, c_void_p, c_size_t, c_void_p]),
+    "jfh_paged_weigh": (Status, [POINTER(PagedCache), POINTER(PagedBatch), POINTER(Rows), c_void_p, c_float, c_uint32,
+                                 c_void_p]),
+    "jfh_paged_evict_workspace": (Status, [POINTER(PagedCache), POINTER(PagedBatch), c_uint32, POINTER(c_size_t)]),
+    "jfh_paged_evict": (Status, [POINTER(PagedCache), POINTER(PagedBatch), c_uint32, c_uint32, c_uint32, c_void_p,
+                                 c_size_t, c_void_p]),
     "jfh_tokenizer_open": (Status, [c_char_p, POINTER(c_void_p)]),
     "jfh_tokenizer_destroy": (None, [c_void_p]),
     "jfh_tokenizer_tokenize": (Status, [c_void_p, c_char_p, c_size_t, POINTER(c_int32), c_uint32, POINTER(c_uint32)]),

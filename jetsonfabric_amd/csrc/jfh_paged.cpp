@@ -169,6 +169,20 @@ AttendPlan attend_plan(const paged::Cache& c, const paged::Batch& b, const paged
     return p;
 }
 
+// Most positions of a K/V head that move when sequences are cut, and the bytes of the lists that say which.
+uint32_t evict_width(const paged::Batch& b, uint32_t budget) {
+    return b.max_length > budget ? std::min(budget, b.max_length - budget) : 0;
+}
+
+size_t evict_bytes(const paged::Cache& c, const paged::Batch& b, uint32_t width) {
+    return width ? static_cast<size_t>(b.n_seq) * c.n_head_kv * (1 + 2 * static_cast<size_t>(width)) * sizeof(int32_t) : 0;
+}
+
+void evicted(const paged::Cache& c, uint32_t budget) {
+    require(c.weights && c.positions, "a cache that is cut needs weights and positions");
+    require(budget > 0 && budget <= kMaxIndex, "a budget of at least one position is required");
+}
+
 }  // namespace
 
 jfh_status jfh_rope_create(const jfh_rope_params* params, jfh_rope** out) {
@@ -254,5 +268,56 @@ jfh_status jfh_paged_attention(const jfh_paged_cache* cache, const jfh_paged_bat
         a.marks = a.partial + p.partial / sizeof(float);
         const OnDevice guard(cache->device);
         check(paged::launch_attend(a, static_cast<hipStream_t>(stream)), "attention over pages");
+    });
+}
+
+jfh_status jfh_paged_weigh(const jfh_paged_cache* cache, const jfh_paged_batch* batch, const jfh_rows* q, const float* lse,
+                           float scale, uint32_t causal, void* stream) {
+    return guarded([&] {
+        paged::Weigh a{};
+        a.cache = cache_of(cache);
+        require(a.cache.weights != nullptr, "the cache needs weights");
+        a.q = attended(q, a.cache, "q");
+        a.batch = batch_of(batch, *cache, true, a.q.rows);
+        a.scale_log2 = score_scale(scale);
+        a.causal = causal ? 1U : 0U;
+        if (a.q.rows == 0 || a.batch.n_seq == 0 || a.batch.max_rows == 0 || a.batch.max_length == 0) return;
+        require(lse != nullptr && aligned(lse, 4), "lse is required");
+        a.lse = lse;
+        const OnDevice guard(cache->device);
+        check(paged::launch_weigh(a, static_cast<hipStream_t>(stream)), "weigh positions");
+    });
+}
+
+jfh_status jfh_paged_evict_workspace(const jfh_paged_cache* cache, const jfh_paged_batch* batch, uint32_t budget,
+                                     size_t* bytes) {
+    return guarded([&] {
+        require(bytes != nullptr, "an output for the workspace's size is required");
+        const paged::Cache c = cache_of(cache);
+        const paged::Batch b = batch_of(batch, *cache, false);
+        evicted(c, budget);
+        *bytes = evict_bytes(c, b, evict_width(b, budget));
+    });
+}
+
+jfh_status jfh_paged_evict(const jfh_paged_cache* cache, const jfh_paged_batch* batch, uint32_t budget, uint32_t n_first,
+                           uint32_t n_recent, void* workspace, size_t workspace_bytes, void* stream) {
+    return guarded([&] {
+        paged::Evict a{};
+        a.cache = cache_of(cache);
+        a.batch = batch_of(batch, *cache, false);
+        evicted(a.cache, budget);
+        require(n_first <= kMaxIndex && n_recent <= kMaxIndex, "more positions are protected than there can be");
+        a.budget = static_cast<int32_t>(budget);
+        a.first = static_cast<int32_t>(n_first);
+        a.recent = static_cast<int32_t>(n_recent);
+        a.width = static_cast<int32_t>(evict_width(a.batch, budget));
+        if (a.width == 0 || a.batch.n_seq == 0) return;  // no sequence is longer
+        const size_t need = evict_bytes(a.cache, a.batch, static_cast<uint32_t>(a.width));
+        require(workspace && workspace_bytes >= need && aligned(workspace, 16),
+                "cutting these sequences needs " + std::to_string(need) + " bytes of workspace, 16-byte aligned");
+        a.lists = static_cast<int32_t*>(workspace);
+        const OnDevice guard(cache->device);
+        check(paged::launch_evict(a, static_cast<hipStream_t>(stream)), "cut sequences");
     });
 }

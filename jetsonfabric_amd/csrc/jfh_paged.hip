@@ -13,7 +13,7 @@ using half8 = _Float16 __attribute__((ext_vector_type(8)));
 using bhalf8 = __bf16 __attribute__((ext_vector_type(8)));
 using float4v = float __attribute__((ext_vector_type(4)));
 
-constexpr float kLn2 = 0.693147180559945309F;
+constexpr float kLn2 = 0.693147180559945309F, kLog2e = 1.44269504088896341F;
 
 enum : uint32_t { kF32 = 1, kF16 = 2, kBF16 = 3 };
 
@@ -204,24 +204,6 @@ __global__ __launch_bounds__(kRotateThreads) void k_append(Rotation r, Cache c, 
             if (c.positions) c.positions[i] = positions[row0 + row];
         }
     }
-}
-
-bool by_eights(const Rows& x) {
-    return reinterpret_cast<uintptr_t>(x.data) % 16 == 0 && x.row_stride % 8 == 0 && x.head_stride % 8 == 0 &&
-           x.head_dim % 8 == 0;
-}
-
-// Long steps: four rows per work-group, so that 64 pairs' angles are one per thread. Short ones: one row, its units
-// over up to `tasks` / 256 work-groups, since the call's time is the time of one work-group.
-struct RowGrid {
-    dim3 grid;
-    int rows;
-};
-
-RowGrid row_grid(uint32_t rows, uint64_t tasks) {
-    if (rows >= kComputeUnits * kRotateRows) return {dim3((rows + kRotateRows - 1) / kRotateRows), kRotateRows};
-    const uint64_t parts = (tasks + kRotateThreads - 1) / kRotateThreads;
-    return {dim3(rows, static_cast<uint32_t>(parts < 64 ? parts : 64)), 1};
 }
 
 // ---------------------------------------------------------------- attention
@@ -627,6 +609,302 @@ __global__ __launch_bounds__(kJoinThreads) void k_attend_join(Attend a) {
     store(a.out.data, row * a.out.row_stride + head * a.out.head_stride + d, a.out.type, x);
 }
 
+// ---------------------------------------------------------------- attention weights
+
+// weights[slot] += sum over the step's queries of a K/V head of exp(scale q k - lse): the columns of the probabilities,
+// summed. A wave owns 32 slots, whose K rows stay in registers as A operands, and goes over the queries 16 at a time; each
+// sum has one owner and one order, so results do not depend on the launch. The sums of 512 queries at a time are added to a
+// total, which keeps the f32 error of long prompts at that of a few hundred terms.
+constexpr int kWeighThreads = 256;
+constexpr int kWeighKeys = 32;   // slots of a wave
+constexpr int kWeighFlush = 32;  // query tiles between additions to the total
+
+template <typename T, int HDP>
+__global__ __launch_bounds__(kWeighThreads) void k_weigh(Weigh a, int group, int blocks) {
+    using V = Values<T>;
+    using v8 = typename V::v8;
+    constexpr int KC = HDP / 32;
+    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+    const int i = lane % 16, g = lane / 16;
+    const uint32_t pair = blockIdx.x / blocks;
+    const uint32_t h = pair % a.cache.n_head_kv, s = pair / a.cache.n_head_kv;
+    const Span span = sequence_span(a.batch, a.q.rows, s);
+    const int base = (static_cast<int>(blockIdx.x % blocks) * (kWeighThreads / 64) + wave) * kWeighKeys;
+    const int queries = span.rows * group;
+    if (base >= span.len || queries == 0) return;
+    const int dim = static_cast<int>(a.cache.head_dim), first = span.len - span.rows;
+
+    int64_t at[2], index[2];
+    uint32_t present[2];
+    uint4 k[2][KC];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+        const int slot = base + 16 * u + i;
+        const int page = slot < span.len ? page_of(a.cache, a.batch, s, slot) : -1;
+        at[u] = page >= 0 ? slot_offset(a.cache, page, slot) : 0;
+        index[u] = page >= 0 ? slot_index(a.cache, page, h, slot) : 0;
+        present[u] = static_cast<uint32_t>(__ballot(page >= 0)) & 0xFFFFU;
+        const T* row = static_cast<const T*>(a.cache.k) + h * a.cache.head_stride + at[u];
+#pragma unroll
+        for (int c = 0; c < KC; ++c) {
+            const int d = 32 * c + 8 * g;
+            k[u][c] = *reinterpret_cast<const uint4*>(row + (d < dim ? d : 0));
+            if (d >= dim) k[u][c] = uint4{0, 0, 0, 0};
+        }
+    }
+
+    float4v total[2], part[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) total[u] = part[u] = float4v{0.0F, 0.0F, 0.0F, 0.0F};
+    // the first row that sees slot `base`
+    const int from = a.causal ? max(0, base - first) * group / 16 * 16 : 0;
+    int tiles = 0;
+    for (int m0 = from; m0 < queries; m0 += 16) {
+        const int m = m0 + i;
+        const Query q = query_of(min(m, queries - 1), group, h);
+        const int64_t row = span.row0 + q.row;
+        const T* x = static_cast<const T*>(a.q.data) + row * a.q.row_stride + q.head * a.q.head_stride;
+        const float lse = a.lse[row * a.q.heads + q.head];
+        // a row that saw nothing adds nothing
+        const int limit = m >= queries || lse == -INFINITY ? 0 : a.causal ? first + q.row + 1 : span.len;
+        const float ref = lse * kLog2e;
+        float4v sc[2] = {float4v{0.0F, 0.0F, 0.0F, 0.0F}, float4v{0.0F, 0.0F, 0.0F, 0.0F}};
+#pragma unroll
+        for (int c = 0; c < KC; ++c) {
+            const int d = 32 * c + 8 * g;
+            uint4 y = *reinterpret_cast<const uint4*>(x + (d < dim ? d : 0));
+            if (d >= dim) y = uint4{0, 0, 0, 0};
+#pragma unroll
+            for (int u = 0; u < 2; ++u) sc[u] = V::mfma16(__builtin_bit_cast(v8, k[u][c]), __builtin_bit_cast(v8, y), sc[u]);
+        }
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const float p = __builtin_amdgcn_exp2f(fmaf(sc[u][r], a.scale_log2, -ref));
+                part[u][r] += base + 16 * u + 4 * g + r < limit ? p : 0.0F;
+            }
+        }
+        if (++tiles % kWeighFlush == 0) {
+#pragma unroll
+            for (int u = 0; u < 2; ++u) {
+                total[u] += part[u];
+                part[u] = float4v{0.0F, 0.0F, 0.0F, 0.0F};
+            }
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+        total[u] += part[u];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            float x = total[u][r];
+#pragma unroll
+            for (int o = 1; o < 16; o *= 2) x += __shfl_xor(x, o);
+            const int64_t to = __shfl(index[u], 4 * g + r);
+            if (i == 0 && (present[u] >> (4 * g + r) & 1U)) a.cache.weights[to] += x;
+        }
+    }
+}
+
+// ---------------------------------------------------------------- cutting a cache
+
+// What stays of a K/V head's slots: the `budget` first in the order (protected, heavier, lower slot). One work-group per
+// sequence and K/V head turns the order into 32-bit keys, finds the budget-th largest by its bytes (four counts of 256
+// bins), and lists the slots below the budget that go and those above that stay, both ascending: the latter move into the
+// former, the others stay where they are. Integer counts and scans only, so the lists do not depend on the launch.
+constexpr int kSelectThreads = 1024;
+constexpr int kSelectKeys = 32768;  // keys kept in LDS; later slots' are computed again
+
+// Order of weights as unsigned integers, 1 for NaN (nothing is lighter), 0 free.
+__device__ __forceinline__ uint32_t weight_key(float w) {
+    if (w != w) return 1U;
+    const uint32_t b = __float_as_uint(w + 0.0F);  // -0 is 0
+    return b >> 31 ? ~b : b | 0x80000000U;
+}
+
+// Exclusive sum over the work-group of two counts; `all` gets their totals.
+__device__ __forceinline__ int2 exclusive_sum(int2 v, int2 (*waves), int2* all) {
+    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+    int2 x = v;
+#pragma unroll
+    for (int o = 1; o < 64; o *= 2) {
+        const int a = __shfl_up(x.x, o), b = __shfl_up(x.y, o);
+        if (lane >= o) x.x += a, x.y += b;
+    }
+    __syncthreads();
+    if (lane == 63) waves[wave] = x;
+    __syncthreads();
+    int2 before{0, 0}, sum{0, 0};
+    for (int w = 0; w < kSelectThreads / 64; ++w) {
+        if (w == wave) before = sum;
+        sum.x += waves[w].x;
+        sum.y += waves[w].y;
+    }
+    *all = sum;
+    return int2{before.x + x.x - v.x, before.y + x.y - v.y};
+}
+
+__global__ __launch_bounds__(kSelectThreads) void k_evict_select(Evict a) {
+    __shared__ uint32_t keys[kSelectKeys];
+    __shared__ uint32_t bins[256];
+    __shared__ int2 waves[kSelectThreads / 64];
+    __shared__ uint32_t found[2];
+    const uint32_t h = blockIdx.x % a.cache.n_head_kv, s = blockIdx.x / a.cache.n_head_kv;
+    int32_t* list = a.lists + static_cast<int64_t>(blockIdx.x) * (1 + 2 * static_cast<int64_t>(a.width));
+    const int len = span_length(a.batch, s), budget = a.budget;
+    if (len <= budget) {
+        if (threadIdx.x == 0) list[0] = -1;
+        return;
+    }
+
+    // the newest position
+    int newest = INT32_MIN;
+    for (int t = threadIdx.x; t < len; t += kSelectThreads) {
+        const int page = page_of(a.cache, a.batch, s, t);
+        if (page >= 0) newest = max(newest, a.cache.positions[slot_index(a.cache, page, h, t)]);
+    }
+#pragma unroll
+    for (int o = 32; o; o /= 2) newest = max(newest, __shfl_xor(newest, o));
+    if (threadIdx.x % 64 == 0) waves[threadIdx.x / 64].x = newest;
+    __syncthreads();
+    for (int w = 0; w < kSelectThreads / 64; ++w) newest = max(newest, waves[w].x);
+
+    // protected slots; an absent page's slots below the budget count among them, as nothing can take their place
+    const int64_t recent = static_cast<int64_t>(newest) - a.recent;
+    int held = 0;
+    const auto safe = [&](int page, int t) {
+        if (page < 0) return t < budget;
+        const int p = a.cache.positions[slot_index(a.cache, page, h, t)];
+        return p < a.first || p > recent;
+    };
+    for (int t = threadIdx.x; t < len; t += kSelectThreads) held += safe(page_of(a.cache, a.batch, s, t), t);
+    int2 all;
+    exclusive_sum(int2{held, 0}, waves, &all);
+    const bool crowded = all.x >= budget;  // some of the protected go too, and nothing else stays
+
+    const auto key_of = [&](int t) {
+        const int page = page_of(a.cache, a.batch, s, t);
+        const bool keep = safe(page, t);
+        if (page < 0 || (keep && !crowded)) return keep ? 0xFFFFFFFFU : 0U;
+        return crowded && !keep ? 0U : weight_key(a.cache.weights[slot_index(a.cache, page, h, t)]);
+    };
+    for (int t = threadIdx.x; t < min(len, kSelectKeys); t += kSelectThreads) keys[t] = key_of(t);
+    const auto key_at = [&](int t) { return t < kSelectKeys ? keys[t] : key_of(t); };
+
+    uint32_t prefix = 0, mask = 0;
+    int need = budget;
+    for (int shift = 24; shift >= 0; shift -= 8) {
+        __syncthreads();
+        if (threadIdx.x < 256) bins[threadIdx.x] = 0;
+        __syncthreads();
+        for (int t = threadIdx.x; t < len; t += kSelectThreads) {
+            const uint32_t k = key_at(t);
+            if ((k & mask) == prefix) atomicAdd(&bins[k >> shift & 255U], 1U);
+        }
+        __syncthreads();
+        if (threadIdx.x < 64) {  // lane l has bins 255 - 4 l downwards
+            int own[4], sum = 0;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) sum += own[e] = static_cast<int>(bins[255 - 4 * threadIdx.x - e]);
+            int upto = sum;
+#pragma unroll
+            for (int o = 1; o < 64; o *= 2) {
+                const int v = __shfl_up(upto, o);
+                if (static_cast<int>(threadIdx.x) >= o) upto += v;
+            }
+            int above = upto - sum;
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                if (above < need && above + own[e] >= need) found[0] = 255 - 4 * threadIdx.x - e, found[1] = above;
+                above += own[e];
+            }
+        }
+        __syncthreads();
+        prefix |= found[0] << shift;
+        mask |= 255U << shift;
+        need -= static_cast<int>(found[1]);
+    }
+
+    // `need` of the slots with key `prefix` stay, the lowest; a thread owns a run of slots (odd, for the LDS banks)
+    const int run = ((len + kSelectThreads - 1) / kSelectThreads) | 1;
+    const int t0 = min(static_cast<int>(threadIdx.x) * run, len), t1 = min(t0 + run, len);
+    int equal = 0;
+    for (int t = t0; t < t1; ++t) equal += key_at(t) == prefix;
+    const int before = exclusive_sum(int2{equal, 0}, waves, &all).x;
+    int2 moves{0, 0};
+    int rank = before;
+    for (int t = t0; t < t1; ++t) {
+        const uint32_t k = key_at(t);
+        const bool stays = k > prefix || (k == prefix && rank++ < need);
+        moves.x += t < budget && !stays;
+        moves.y += t >= budget && stays;
+    }
+    int2 to = exclusive_sum(moves, waves, &all);
+    if (threadIdx.x == 0) list[0] = all.x;
+    rank = before;
+    for (int t = t0; t < t1; ++t) {
+        const uint32_t k = key_at(t);
+        const bool stays = k > prefix || (k == prefix && rank++ < need);
+        if (t < budget && !stays) list[1 + to.x++] = t;
+        if (t >= budget && stays) list[1 + a.width + to.y++] = t;
+    }
+}
+
+// 16 threads per moving position: its K and V rows, its weight and its position.
+constexpr int kMoveThreads = 256;
+constexpr int kMoveSlots = 32;  // of a work-group
+
+__global__ __launch_bounds__(kMoveThreads) void k_evict_move(Evict a, int chunks) {
+    const uint32_t pair = blockIdx.x / chunks;
+    const uint32_t h = pair % a.cache.n_head_kv, s = pair / a.cache.n_head_kv;
+    const int chunk = static_cast<int>(blockIdx.x % chunks);
+    const int32_t* list = a.lists + static_cast<int64_t>(pair) * (1 + 2 * static_cast<int64_t>(a.width));
+    const int count = list[0];
+    if (count < 0) return;
+    if (h == 0 && chunk == 0 && threadIdx.x == 0) a.batch.lengths[s] = a.budget;
+    const int part = threadIdx.x % 16;
+    for (int n = chunk * kMoveSlots + threadIdx.x / 16; n < min(count, (chunk + 1) * kMoveSlots); n += kMoveThreads / 16) {
+        const int to = list[1 + n], from = list[1 + a.width + n];
+        const int to_page = page_of(a.cache, a.batch, s, to), from_page = page_of(a.cache, a.batch, s, from);
+        if (to_page < 0 || from_page < 0) continue;
+        const int64_t x = slot_offset(a.cache, from_page, from) + h * a.cache.head_stride;
+        const int64_t y = slot_offset(a.cache, to_page, to) + h * a.cache.head_stride;
+        uint16_t* k = static_cast<uint16_t*>(a.cache.k);
+        uint16_t* v = static_cast<uint16_t*>(a.cache.v);
+        for (int d = 8 * part; d < static_cast<int>(a.cache.head_dim); d += 128) {
+            const uint4 kx = *reinterpret_cast<const uint4*>(k + x + d), vx = *reinterpret_cast<const uint4*>(v + x + d);
+            *reinterpret_cast<uint4*>(k + y + d) = kx;
+            *reinterpret_cast<uint4*>(v + y + d) = vx;
+        }
+        if (part == 0) {
+            const int64_t i = slot_index(a.cache, from_page, h, from), j = slot_index(a.cache, to_page, h, to);
+            a.cache.weights[j] = a.cache.weights[i];
+            a.cache.positions[j] = a.cache.positions[i];
+        }
+    }
+}
+
+// ---------------------------------------------------------------- launches
+
+bool by_eights(const Rows& x) {
+    return reinterpret_cast<uintptr_t>(x.data) % 16 == 0 && x.row_stride % 8 == 0 && x.head_stride % 8 == 0 &&
+           x.head_dim % 8 == 0;
+}
+
+// Long steps: four rows per work-group, so that 64 pairs' angles are one per thread. Short ones: one row, its units
+// over up to `tasks` / 256 work-groups, since the call's time is the time of one work-group.
+struct RowGrid {
+    dim3 grid;
+    int rows;
+};
+
+RowGrid row_grid(uint32_t rows, uint64_t tasks) {
+    if (rows >= kComputeUnits * kRotateRows) return {dim3((rows + kRotateRows - 1) / kRotateRows), kRotateRows};
+    const uint64_t parts = (tasks + kRotateThreads - 1) / kRotateThreads;
+    return {dim3(rows, static_cast<uint32_t>(parts < 64 ? parts : 64)), 1};
+}
+
 }  // namespace
 
 hipError_t launch_rotate(const Rotation& r, const Rows& x, const int32_t* positions, const Rows& y, hipStream_t stream) {
@@ -688,6 +966,40 @@ hipError_t launch_attend(const Attend& a, hipStream_t stream) {
     const hipError_t e = a.cache.type == kF16 ? attend<_Float16>(a, stream) : attend<__bf16>(a, stream);
     if (e != hipSuccess || a.splits == 1) return e;
     return launch(k_attend_join, dim3(a.q.rows * a.q.heads), dim3(kJoinThreads), stream, a);
+}
+
+namespace {
+
+template <typename T, int HDP>
+hipError_t weigh_few(const Weigh& a, hipStream_t stream) {
+    constexpr int kSlots = kWeighThreads / 64 * kWeighKeys;
+    const int group = static_cast<int>(a.q.heads / a.cache.n_head_kv);
+    const int blocks = static_cast<int>((a.batch.max_length + kSlots - 1) / kSlots);
+    const uint64_t groups = static_cast<uint64_t>(blocks) * a.cache.n_head_kv * a.batch.n_seq;
+    if (groups > 0x7FFFFFFF) return hipErrorInvalidConfiguration;
+    return launch(k_weigh<T, HDP>, dim3(static_cast<uint32_t>(groups)), dim3(kWeighThreads), stream, a, group, blocks);
+}
+
+template <typename T>
+hipError_t weigh(const Weigh& a, hipStream_t stream) {
+    if (a.cache.head_dim <= 64) return weigh_few<T, 64>(a, stream);
+    if (a.cache.head_dim <= 128) return weigh_few<T, 128>(a, stream);
+    return weigh_few<T, 256>(a, stream);
+}
+
+}  // namespace
+
+hipError_t launch_weigh(const Weigh& a, hipStream_t stream) {
+    return a.cache.type == kF16 ? weigh<_Float16>(a, stream) : weigh<__bf16>(a, stream);
+}
+
+hipError_t launch_evict(const Evict& a, hipStream_t stream) {
+    const uint64_t pairs = static_cast<uint64_t>(a.cache.n_head_kv) * a.batch.n_seq;
+    const int chunks = (a.width + kMoveSlots - 1) / kMoveSlots;
+    if (pairs * static_cast<uint64_t>(chunks) > 0x7FFFFFFF) return hipErrorInvalidConfiguration;
+    const hipError_t e = launch(k_evict_select, dim3(static_cast<uint32_t>(pairs)), dim3(kSelectThreads), stream, a);
+    if (e != hipSuccess) return e;
+    return launch(k_evict_move, dim3(static_cast<uint32_t>(pairs) * chunks), dim3(kMoveThreads), stream, a, chunks);
 }
 
 }  // namespace jfh::paged

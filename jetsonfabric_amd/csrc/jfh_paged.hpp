@@ -115,6 +115,23 @@ struct Attend {
     uint32_t causal, splits;
 };
 
+struct Weigh {
+    Cache cache;
+    Batch batch;
+    Rows q;
+    const float* lse;
+    float scale_log2;
+    uint32_t causal;
+};
+
+struct Evict {
+    Cache cache;
+    Batch batch;
+    int32_t budget, first, recent;
+    int32_t width;   // most positions that move
+    int32_t* lists;  // per (sequence, K/V head): their number (-1: nothing is cut), to [width], from [width]
+};
+
 // Parts that a step's keys are divided into, each a work-group of its own per K/V head and tile of query rows; more than
 // one where the tiles do not fill the chip.
 uint32_t attend_splits(const Cache& c, const Batch& b, uint32_t group);
@@ -123,5 +140,7 @@ hipError_t launch_rotate(const Rotation& r, const Rows& x, const int32_t* positi
 hipError_t launch_append(const Rotation* r, const Cache& c, const Batch& b, const Rows& k, const Rows& v,
                          const int32_t* positions, hipStream_t stream);
 hipError_t launch_attend(const Attend& a, hipStream_t stream);
+hipError_t launch_weigh(const Weigh& a, hipStream_t stream);
+hipError_t launch_evict(const Evict& a, hipStream_t stream);
 
 }  // namespace jfh::paged

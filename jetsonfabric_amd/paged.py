@@ -147,6 +147,10 @@ class PagedCache:
             raise ValueError(f"the batch is on GPU {batch.device}, the cache on GPU {self.device}")
         return batch.ref
 
+    def _workspace(self, size: int):
+        # of torch's allocator: ordered by the current stream, and a captured graph's own
+        return sys.modules["torch"].empty(size, dtype=sys.modules["torch"].uint8, device=self.k.device) if size else None
+
     def append(self, batch: PagedBatch, k, v, positions=None, rope: Rope | None = None) -> None:
         """Writes a step's rows k and v [rows, K/V heads, head dim] at its sequences' last slots, k
         rotated by rope; positions int32 [rows]."""
@@ -169,9 +173,26 @@ class PagedCache:
         at = _array(lse, "lse", "torch.float32", self.device, q.shape[:2])
         need = ctypes.c_size_t()
         check(library().jfh_paged_attention_workspace(self.ref, self._of(batch), ctypes.byref(a), ctypes.byref(need)))
-        space = torch.empty(need.value, dtype=torch.uint8, device=q.device) if need.value else None
+        space = self._workspace(need.value)
         check(library().jfh_paged_attention(self.ref, batch.ref, ctypes.byref(a),
                                             a.head_dim ** -0.5 if scale is None else scale, int(causal), ctypes.byref(b),
                                             at, None if space is None else space.data_ptr(), need.value,
                                             _stream(self.device)))
         return out, lse
+
+    def weigh(self, batch: PagedBatch, q, lse, scale: float | None = None, causal: bool = True) -> None:
+        """Adds the attention that the rows q (with attend's lse, scale and causal) give each position to
+        the cache's weights."""
+        a = _rows(q, "q", self.device)
+        at = _array(lse, "lse", "torch.float32", self.device, q.shape[:2])
+        check(library().jfh_paged_weigh(self.ref, self._of(batch), ctypes.byref(a), at,
+                                        a.head_dim ** -0.5 if scale is None else scale, int(causal), _stream(self.device)))
+
+    def evict(self, batch: PagedBatch, budget: int, n_first: int = 4, n_recent: int = 1) -> None:
+        """Cuts every longer sequence to budget slots per K/V head: the positions below n_first, the
+        n_recent newest, then the heaviest stay; batch.lengths becomes what is left."""
+        need = ctypes.c_size_t()
+        check(library().jfh_paged_evict_workspace(self.ref, self._of(batch), budget, ctypes.byref(need)))
+        space = self._workspace(need.value)
+        check(library().jfh_paged_evict(self.ref, batch.ref, budget, n_first, n_recent,
+                                        None if space is None else space.data_ptr(), need.value, _stream(self.device)))

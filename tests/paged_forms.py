@@ -174,3 +174,56 @@ class Sequences:
                 bound[r, h] += step * (out[r, h].abs() + bound[r, h]) + 2.0**-25
                 lse_bound[r, h] = off[:, 0] + 2.0**-21 + (n + 64) * 2.0**-23 + 2.0**-22 * lse[r, h].abs().nan_to_num(posinf=0)
         return out, lse, bound, lse_bound
+
+    def weigh(self, q, lse, scale, causal=True):
+        """weights (f64) after the rows q with lse [rows, heads] (float32), and their bounds."""
+        group = q.shape[1] // self.kv_heads
+        w, bound = self.weights.double().clone(), torch.zeros(self.weights.shape, dtype=torch.float64)
+        for s in range(len(self.rows)):
+            k, _, there = self.gather(s)
+            sees = self.sees(s, causal, there)
+            r = slice(self.starts[s], self.starts[s + 1])
+            sums, offs = torch.zeros(self.kv_heads, self.lens[s], dtype=torch.float64), torch.zeros(self.kv_heads, self.lens[s])
+            for h in range(q.shape[1]):
+                x, kh, l = q[r, h].double(), k[h // group], lse[r, h].double()[:, None]
+                score = x @ kh.T * scale
+                p = torch.where(sees & (l > -math.inf), torch.exp(score - l), 0.0)
+                # as for attention's scores, and the rounding of lse in base 2
+                off = (self.dim + 2) * 2.0**-24 * scale * (x.abs() @ kh.abs().T) + 2.0**-22 * (score.abs() + l.abs()) + 2.0**-21
+                sums[h // group] += p.sum(0)
+                offs[h // group] += torch.where(p > 0, p * off, 0.0).sum(0)
+            terms = self.rows[s] * group / 16 + 24  # sums of a lane, over lanes and into the total
+            for t in range(self.lens[s]):
+                at = self.slot(s, t)
+                if at is not None:
+                    w[at[0], :, at[1]] += sums[:, t]
+                    bound[at[0], :, at[1]] = offs[:, t] + (terms * sums[:, t] + w[at[0], :, at[1]].abs()) * 2.0**-24
+        return w, bound
+
+    def evict(self, budget, first, recent):
+        """k, v, weights, positions and lengths after a cut."""
+        k, v, w, pos = self.k.clone(), self.v.clone(), self.weights.clone(), self.positions.clone()
+        lens = [min(n, budget) for n in self.lens]
+        for s, n in enumerate(self.lens):
+            if n <= budget:
+                continue
+            at = [self.slot(s, t) for t in range(n)]
+            for h in range(self.kv_heads):
+                there = [t for t in range(n) if at[t] is not None]
+                newest = max((int(self.positions[at[t][0], h, at[t][1]]) for t in there), default=0)
+
+                def order(t):
+                    if at[t] is None:  # holds its place below the budget, never moves
+                        return (0 if t < budget else 3, 0, 0.0, t)
+                    p, weight = int(self.positions[at[t][0], h, at[t][1]]), float(self.weights[at[t][0], h, at[t][1]])
+                    kind = 1 if p < first or p > newest - recent else 2
+                    return (kind, 1, 0.0, t) if math.isnan(weight) else (kind, 0, -weight, t)
+
+                stay = set(sorted(range(n), key=order)[:budget])
+                to = [t for t in range(budget) if t not in stay]
+                come = [t for t in range(budget, n) if t in stay]
+                assert len(to) == len(come)
+                for a, b in zip(to, come):
+                    for x, y in ((k, self.k), (v, self.v), (w, self.weights), (pos, self.positions)):
+                        x[at[a][0], h, at[a][1]] = y[at[b][0], h, at[b][1]]
+        return k, v, w, pos, lens

@@ -305,3 +305,278 @@ def test_attention_of_strided_rows_on_another_stream():
         cache.attend(batch, gpu.unflatten(1, (14, 64))[:, 2:10], 0.125, out=out)
     stream.synchronize()
     within(out.cpu(), want[0], want[2])
+
+
+# ---------------------------------------------------------------- attention weights
+
+@pytest.mark.parametrize("rows,lens,heads,kv,dim,page,more", ATTENDS)
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+def test_weights(rows, lens, heads, kv, dim, page, more, kind):
+    seq = Sequences(rows, lens, kv, dim, page, TYPES[kind], seed=len(lens), **more).poison()
+    q = normal(seq.total, heads, dim, seed=4, std=1.5).to(seq.dtype)
+    scale = dim ** -0.5
+    kp, vp, w, _, table, lengths, starts = seq.to_gpu()
+    cache, batch = jf.PagedCache(kp, vp, w), jf.PagedBatch(table, lengths, starts, seq.max_rows, seq.max_length)
+    for causal in (True, False):
+        lse = seq.attend(q, scale, causal)[1].float()
+        w.copy_(seq.weights)
+        cache.weigh(batch, q.cuda(), lse.cuda(), scale, causal)
+        want, bound = seq.weigh(q, lse, scale, causal)
+        within(w.cpu(), want, bound)
+        assert torch.equal(w.cpu()[bound == 0], seq.weights[bound == 0])
+        again = w.clone()
+        w.copy_(seq.weights)
+        cache.weigh(batch, q.cuda(), lse.cuda(), scale, causal)
+        assert torch.equal(w, again)
+
+
+def test_weights_of_attention_sum_to_its_rows():
+    """What a step adds to all positions of a K/V head is its rows times its heads."""
+    seq = Sequences([50, 3], [400, 77], 2, 128, 16, torch.float16, seed=4)
+    kp, vp, w, _, table, lengths, starts = seq.to_gpu()
+    cache, batch = jf.PagedCache(kp, vp, w), jf.PagedBatch(table, lengths, starts, 50, 400)
+    q = normal(53, 10, 128, seed=1, std=2.0).half().cuda()
+    w.zero_()
+    _, lse = cache.attend(batch, q)
+    cache.weigh(batch, q, lse)
+    per_head = w.double().sum((0, 2)).cpu()
+    # lse and the weights carry the same scores: errors of their sums and exponentials, below 400 terms' worst case
+    assert (per_head - 53 * 5).abs().max() < 53 * 5 * (400 + 64) * 2.0**-23
+
+
+def test_weights_of_the_last_rows_alone():
+    """A prompt's last rows only: a step of fewer rows over the same lengths."""
+    seq = Sequences([8, 8], [300, 90], 1, 64, 16, torch.float16, seed=2)
+    q = normal(200, 4, 64, seed=3).half()
+    part = torch.cat([q[92:100], q[192:200]])
+    lse = seq.attend(part, 0.125)[1].float()
+    kp, vp, w, _, table, lengths, starts = seq.to_gpu()
+    jf.PagedCache(kp, vp, w).weigh(jf.PagedBatch(table, lengths, starts, 8, 300), part.cuda(), lse.cuda(), 0.125)
+    want, bound = seq.weigh(part, lse, 0.125)
+    within(w.cpu(), want, bound)
+
+
+# ---------------------------------------------------------------- cutting
+
+def cut(seq, budget, first, recent):
+    kp, vp, w, pos, table, lengths, starts = seq.to_gpu()
+    batch = jf.PagedBatch(table, lengths, starts, seq.max_rows, seq.max_length)
+    jf.PagedCache(kp, vp, w, pos).evict(batch, budget, first, recent)
+    k, v, ww, wp, lens = seq.evict(budget, first, recent)
+    assert lengths.cpu().tolist() == lens
+    assert torch.equal(pos.cpu(), wp)
+    assert torch.equal(w.cpu().view(torch.int32), ww.view(torch.int32))
+    for got, want in ((kp, k), (vp, v)):
+        assert torch.equal(got.cpu().contiguous().view(torch.int16), want.contiguous().view(torch.int16))
+    return w.cpu(), pos.cpu()
+
+
+CUTS = [
+    # lengths, K/V heads, dim, page, budget, first, recent, what else
+    ([2], 1, 8, 1, 1, 0, 1, {}),
+    ([33, 32, 31], 2, 64, 16, 32, 4, 8, {}),
+    ([4097, 4096, 100], 4, 128, 16, 4096, 4, 256, {}),
+    ([1000, 3000], 2, 72, 8, 700, 0, 0, {"order": "tokens"}),
+    ([1500, 900], 3, 256, 64, 100, 4, 32, {"order": "padded"}),
+    ([500, 70], 2, 64, 16, 64, 40, 40, {}),       # more protected than the budget
+    ([600], 2, 64, 16, 200, 4, 16, {"absent": [(0, 2), (0, 20), (0, 30)]}),
+    ([90], 1, 64, 16, 30, 4, 16, {"absent": [(0, 0), (0, 1)]}),
+    ([40000, 33000], 1, 8, 256, 20000, 16, 1000, {}),  # beyond the keys held in LDS
+    ([2500], 1, 16, 2, 2499, 0, 1, {}),
+    ([5, 1, 0], 2, 32, 4, 3, 1, 1, {}),
+]
+
+
+@pytest.mark.parametrize("lens,kv,dim,page,budget,first,recent,more", CUTS)
+@pytest.mark.parametrize("values", ["spread", "ties", "odd"])
+def test_cut(lens, kv, dim, page, budget, first, recent, more, values):
+    seq = Sequences([0] * len(lens), lens, kv, dim, page, torch.float16, seed=budget, **more)
+    for s in range(len(lens)):  # positions as a cache has them that was cut before: ascending, with gaps
+        for p in range(-(-lens[s] // page)):
+            at = seq.slot(s, p * page)
+            if at is not None:
+                seq.positions[at[0]] = (torch.arange(page, dtype=torch.int32) + p * page) * 2
+    if values == "ties":
+        seq.weights = (seq.weights * 3).floor() - 1
+        seq.weights[seq.weights == 0] *= -1  # -0 and 0 weigh the same
+    if values == "odd":
+        pick = torch.randint(0, 12, seq.weights.shape, generator=torch.Generator().manual_seed(1))
+        for n, x in enumerate((float("nan"), -float("nan"), float("inf"), -float("inf"), -1.0, 1e-42, 3e38)):
+            seq.weights[pick == n] = x
+    cut(seq, budget, first, recent)
+
+
+def test_cut_of_a_cache_in_any_order_protects_by_position():
+    """The newest and the first positions stay wherever their slots are."""
+    seq = Sequences([0], [300], 1, 64, 16, torch.bfloat16, seed=9)
+    order = torch.randperm(300, generator=torch.Generator().manual_seed(2)).int()
+    for t in range(300):
+        at = seq.slot(0, t)
+        seq.positions[at[0], 0, at[1]] = order[t] + 1000
+    _, pos = cut(seq, 40, 1004, 30)
+    left = {int(pos[(*seq.slot(0, t)[:1], 0, seq.slot(0, t)[1])]) for t in range(40)}
+    assert left >= set(range(1000, 1004)) | set(range(1270, 1300))
+
+
+def test_cut_within_the_budget_changes_nothing():
+    seq = Sequences([0, 0], [50, 64], 2, 64, 16, torch.float16, seed=1)
+    cut(seq, 64, 4, 8)
+    cut(seq, 1000, 4, 8)
+
+
+# ---------------------------------------------------------------- together
+
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+def test_prompt_cut_and_decoding(kind):
+    """A prompt in two chunks, its cache cut by the weights of its last rows, then steps of single tokens with the cache
+    held at its budget: every operator on what the ones before it left, each against its definition on those values."""
+    dtype, heads, kv, dim, budget, page = TYPES[kind], 10, 2, 64, 96, 16
+    kw = {"layout": "half", "scaling": "yarn", "factor": 4.0, "original_context": 64}
+    rope = jf.Rope(dim, **kw)
+    seq = Sequences([0, 0], [0, 0], kv, dim, page, dtype, seed=12, wide_table=20)
+    kp, vp, w, pos, table, lengths, starts = seq.to_gpu()
+    cache = jf.PagedCache(kp, vp, w, pos)
+    text = [0, 0]
+    for step, rows in enumerate([[130, 61], [70, 1], [1, 1], [1, 1], [3, 0], [1, 1]]):
+        total = sum(rows)
+        qkv = normal(total, heads + 2 * kv, dim, seed=30 + step, std=1.5).to(dtype)
+        positions = torch.cat([torch.arange(text[s], text[s] + rows[s], dtype=torch.int32) for s in range(2)])
+        seq.rows, seq.starts, seq.total = rows, [0, rows[0], total], total
+        seq.lens = [n + r for n, r in zip(seq.lens, rows)]
+        text = [n + r for n, r in zip(text, rows)]
+        lengths.copy_(ints(seq.lens))
+        starts.copy_(ints(seq.starts))
+        batch = jf.PagedBatch(table, lengths, starts, max(rows), max(seq.lens))
+        gpu = qkv.cuda()
+        q = rope.rotate(gpu[:, :heads], positions.cuda())
+        want, terms = rotate(qkv[:, :heads], positions, dim, **kw)
+        within(q.cpu(), want, rotation_bound(want, terms, dtype))
+
+        want_k, bound, want_v, want_w, want_p = appended(seq, qkv[:, heads:heads + kv], qkv[:, heads + kv:], positions,
+                                                         {"n_rot": dim, **kw}, rope)
+        cache.append(batch, gpu[:, heads:heads + kv], gpu[:, heads + kv:], positions.cuda(), rope)
+        within(kp.cpu(), want_k, bound)
+        assert torch.equal(vp.cpu(), want_v) and torch.equal(w.cpu(), want_w) and torch.equal(pos.cpu(), want_p)
+        seq.k, seq.v, seq.weights, seq.positions = kp.cpu(), vp.cpu(), w.cpu(), pos.cpu()
+
+        out, lse = cache.attend(batch, q)
+        want, want_lse, bound, lse_bound = seq.attend(q.cpu(), dim ** -0.5)
+        within(out.cpu(), want, bound)
+        within(lse.cpu(), want_lse, lse_bound)
+
+        cache.weigh(batch, q, lse)
+        want, bound = seq.weigh(q.cpu(), lse.cpu(), dim ** -0.5)
+        within(w.cpu(), want, bound)
+        seq.weights = w.cpu()
+        if step > 0:
+            cache.evict(batch, budget, 4, 32)
+            k, v, want_w, want_p, seq.lens = seq.evict(budget, 4, 32)
+            assert torch.equal(kp.cpu(), k) and torch.equal(vp.cpu(), v) and torch.equal(w.cpu(), want_w)
+            assert torch.equal(pos.cpu(), want_p) and lengths.cpu().tolist() == seq.lens
+            seq.k, seq.v, seq.weights, seq.positions = k, v, want_w, want_p
+
+
+def test_a_captured_step_replays_with_other_contents():
+    """A decode step with its cut in a graph: lengths, rows and tables of the same tensors change between replays, and
+    eager calls of the same shapes run between them. Every replay equals the eager step."""
+    dtype, heads, kv, dim, budget = torch.float16, 8, 2, 64, 1500
+    rope = jf.Rope(dim)
+    seq = Sequences([1, 1], [1500, 1500], kv, dim, 16, dtype, seed=21, wide_table=10)
+    state = [x.clone() for x in seq.to_gpu()[:4]]
+    _, _, _, _, table, lengths, starts = seq.to_gpu()
+    qkv, positions = torch.zeros(2, heads + 2 * kv, dim, dtype=dtype, device="cuda"), ints([0, 0]).cuda()
+    batch = jf.PagedBatch(table, lengths, starts, 1, 1600)
+
+    def step(kp, vp, w, pos):
+        cache = jf.PagedCache(kp, vp, w, pos)
+        q = rope.rotate(qkv[:, :heads], positions)
+        cache.append(batch, qkv[:, heads:heads + kv], qkv[:, heads + kv:], positions, rope)
+        out, lse = cache.attend(batch, q)
+        cache.weigh(batch, q, lse)
+        cache.evict(batch, budget, 4, 64)
+        return out, lse
+
+    def contents(n):
+        g = torch.Generator().manual_seed(100 + n)
+        qkv.copy_(torch.randn(qkv.shape, generator=g))
+        positions.fill_(1500 + n)
+        lengths.copy_(ints([[1501, 1501], [1501, 700], [3, 1501], [1501, 1501]][n]))
+
+    # positions as the cache's slots
+    for s in range(2):
+        for p in range(table.shape[1]):
+            state[3][int(seq.table[s, p])] = torch.arange(16 * p, 16 * p + 16, dtype=torch.int32, device="cuda")
+    mine = [x.clone() for x in state]
+    graph = torch.cuda.CUDAGraph()
+    contents(0)
+    warm = [x.clone() for x in state]
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step(*warm)
+    torch.cuda.current_stream().wait_stream(side)
+    contents(0)
+    with torch.cuda.graph(graph):
+        out, lse = step(*mine)
+    for n in range(4):
+        contents(n)
+        want_out, want_lse = step(*state)
+        left = lengths.clone()
+        contents(n)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, want_out) and torch.equal(lse, want_lse) and torch.equal(lengths, left)
+        for a, b in zip(mine, state):
+            assert torch.equal(a, b)
+
+
+def test_calls_on_two_streams_do_not_disturb_each_other():
+    seqs = [Sequences([1], [3000], 2, 64, 16, torch.float16, seed=40 + n) for n in range(2)]
+    q = normal(1, 8, 64, seed=1).half()
+    parts, streams = [], [torch.cuda.Stream(), torch.cuda.Stream()]
+    for seq in seqs:
+        kp, vp, _, _, table, lengths, starts = seq.to_gpu()
+        parts.append((jf.PagedCache(kp, vp), jf.PagedBatch(table, lengths, starts, 1, 3000)))
+    gpu = q.cuda()
+    torch.cuda.synchronize()
+    got = [[], []]
+    for _ in range(20):
+        for n in range(2):
+            with torch.cuda.stream(streams[n]):
+                got[n].append(parts[n][0].attend(parts[n][1], gpu)[0])
+    torch.cuda.synchronize()
+    for n in range(2):
+        want, _, bound, _ = seqs[n].attend(q, 0.125)
+        for out in got[n]:
+            within(out.cpu(), want, bound)
+
+
+def test_keys_equal_the_engines():
+    """Keys that an engine's prefill caches are those that append writes: the same pairs, angles and rounding. One layer,
+    float weights; the projected rows come from the engine's own matmul."""
+    import numpy as np
+
+    cfg = jf.ModelConfig(n_layer=1, n_embd=256, n_ff=256, n_head=4, n_head_kv=2, n_vocab=256, n_ctx=128)
+    model = jf.Model.synthesize(cfg, type_linear=jf.Q8_0, type_embd=jf.Q8_0, type_output=jf.Q8_0, seed=5)
+    engine = jf.NativeEngine(model)
+    tokens = [int(t) for t in np.random.default_rng(3).integers(0, 256, 20)]
+    session = engine.create_session(32)
+    session.prefill_greedy(tokens)
+    k, _ = session.read_kv(0, 20)
+    want = torch.from_numpy(k.view(np.float16).copy()).transpose(0, 1).double()  # [position, head, dim]
+
+    x = engine.dequantize_rows("token_embd.weight", 0, 256, 256)[tokens].astype(np.float64)
+    def vector(name):
+        return np.frombuffer(model.tensor_bytes(name), dtype=np.float32).astype(np.float64)
+    x = x / np.sqrt((x * x).mean(-1, keepdims=True) + cfg.rms_eps) * vector("blk.0.attn_norm.weight")
+    rows = engine.matmul("blk.0.attn_k.weight", x.astype(np.float32), 128) + vector("blk.0.attn_k.bias").astype(np.float32)
+    rows = torch.from_numpy(rows.astype(np.float32)).reshape(20, 2, 64).cuda()
+    pages = torch.zeros(2, 2, 16, 64, dtype=torch.float16, device="cuda")
+    cache = jf.PagedCache(pages, torch.zeros_like(pages))
+    batch = jf.PagedBatch(ints([[1, 0]]).cuda(), ints([20]).cuda(), ints([0, 20]).cuda(), 20, 20)
+    cache.append(batch, rows, rows, torch.arange(20, dtype=torch.int32, device="cuda"), jf.Rope(64, base=cfg.rope_base))
+    got = torch.cat([pages[1], pages[0, :, :4]], 1).transpose(0, 1).double().cpu()
+    # the engine rounds its activations to 8-bit codes: a normalization in f32 moves a few of them by one of 127
+    assert (got - want).norm() < 0.01 * want.norm()
+    engine.close()
+    model.close()

@@ -123,6 +123,56 @@ def test_attention_arguments_are_checked():
     check(_attend(b=batch(n_seq=0)))
 
 
+def _weigh(c=None, b=None, q=None, scale=0.125, lse=AT):
+    return jf.library().jfh_paged_weigh(ctypes.byref(c or cache()), ctypes.byref(b or batch()), ctypes.byref(q or rows()),
+                                        lse, scale, 1, None)
+
+
+def _evict(c=None, b=None, budget=8, first=4, recent=2, space=AT, size=1 << 40):
+    return jf.library().jfh_paged_evict(ctypes.byref(c or cache()), ctypes.byref(b or batch()), budget, first, recent, space,
+                                        size, None)
+
+
+@pytest.mark.parametrize("change,match", BAD_CACHES)
+def test_weighed_and_cut_caches_are_checked(change, match):
+    refused(lambda: _weigh(c=cache(**change)), match)
+    refused(lambda: _evict(c=cache(**change)), match)
+
+
+@pytest.mark.parametrize("change,match", BAD_BATCHES)
+def test_weighed_and_cut_batches_are_checked(change, match):
+    refused(lambda: _weigh(b=batch(**change)), match)
+    if "row_starts" not in change and "max_rows" not in change:
+        refused(lambda: _evict(b=batch(**change)), match)
+
+
+def test_weigh_arguments_are_checked():
+    refused(lambda: _weigh(c=cache(weights=None)), "needs weights")
+    refused(lambda: _weigh(lse=None), "lse")
+    refused(lambda: _weigh(scale=0.0), "score scale")
+    refused(lambda: _weigh(q=rows(type=3)), "cache's type")
+    check(_weigh(q=rows(n_rows=0)))
+    check(_weigh(b=batch(max_length=0)))
+
+
+def test_evict_arguments_are_checked():
+    refused(lambda: _evict(c=cache(weights=None)), "weights and positions")
+    refused(lambda: _evict(c=cache(positions=None)), "weights and positions")
+    refused(lambda: _evict(budget=0), "budget")
+    refused(lambda: _evict(budget=1 << 31), "budget")
+    refused(lambda: _evict(first=1 << 31), "protected")
+    refused(lambda: _evict(recent=(1 << 32) - 1), "protected")
+    need = ctypes.c_size_t()
+    check(jf.library().jfh_paged_evict_workspace(ctypes.byref(cache()), ctypes.byref(batch(row_starts=None)), 8,
+                                                 ctypes.byref(need)))
+    assert need.value == 2 * 4 * (1 + 2 * 8) * 4  # lists of 8 moves for 2 sequences of 4 heads
+    refused(lambda: _evict(size=need.value - 1), f"needs {need.value} bytes")
+    refused(lambda: _evict(space=None), "workspace")
+    refused(lambda: _evict(space=AT + 8), "16-byte")
+    check(_evict(budget=64, space=None, size=0))  # no sequence is longer
+    check(_evict(b=batch(n_seq=0)))
+
+
 def test_missing_arguments_are_refused():
     lib = jf.library()
     assert lib.jfh_paged_append(None, ctypes.byref(batch()), ctypes.byref(rows()), ctypes.byref(rows()), None, AT, None).code == 1
