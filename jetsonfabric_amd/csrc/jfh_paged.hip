@@ -12,6 +12,7 @@ namespace {
 using half8 = _Float16 __attribute__((ext_vector_type(8)));
 using bhalf8 = __bf16 __attribute__((ext_vector_type(8)));
 using float4v = float __attribute__((ext_vector_type(4)));
+using float16v = float __attribute__((ext_vector_type(16)));
 
 constexpr float kLn2 = 0.693147180559945309F, kLog2e = 1.44269504088896341F;
 
@@ -212,15 +213,21 @@ template <typename T> struct Values;
 template <> struct Values<_Float16> {
     using v8 = half8;
     static constexpr uint32_t kExponent = 0x7C00;
-    static __device__ __forceinline__ float4v mfma16(v8 a, v8 b, float4v c) {
+    static __device__ __forceinline__ float4v mfma(v8 a, v8 b, float4v c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ float16v mfma(v8 a, v8 b, float16v c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
     }
 };
 template <> struct Values<__bf16> {
     using v8 = bhalf8;
     static constexpr uint32_t kExponent = 0x7F80;
-    static __device__ __forceinline__ float4v mfma16(v8 a, v8 b, float4v c) {
+    static __device__ __forceinline__ float4v mfma(v8 a, v8 b, float4v c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+    }
+    static __device__ __forceinline__ float16v mfma(v8 a, v8 b, float16v c) {
+        return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
     }
 };
 
@@ -239,6 +246,17 @@ __device__ __forceinline__ float groups_sum(float v) {
     return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
+// Over the two lanes l, l ^ 32.
+__device__ __forceinline__ float halves_max(float v) {
+    const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+}
+
+__device__ __forceinline__ float halves_sum(float v) {
+    const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(a[0]) + __uint_as_float(a[1]);
+}
+
 // Whether one of two 16-bit values is infinite or NaN.
 template <typename T>
 __device__ __forceinline__ bool nonfinite(uint32_t two) {
@@ -248,30 +266,48 @@ __device__ __forceinline__ bool nonfinite(uint32_t two) {
 
 // sum + v p where v may hold infinities and NaN in rows that some columns of p do not see: a weight of 0 must leave them
 // out. Their share comes from products of their marks with `seen` (1 where a column sees the row), which count them.
-template <typename T>
-__device__ __forceinline__ float4v weighted_nonfinite(typename Values<T>::v8 v, typename Values<T>::v8 p,
-                                                      typename Values<T>::v8 seen, float4v sum) {
-    typename Values<T>::v8 rest, pos, neg, nan;
+template <typename T, typename Acc>
+__device__ __forceinline__ Acc weighted_nonfinite(typename Values<T>::v8 v, typename Values<T>::v8 p,
+                                                  typename Values<T>::v8 seen, Acc sum) {
+    typename Values<T>::v8 rest, mark[3];
 #pragma unroll
     for (int i = 0; i < 8; ++i) {
         const float x = static_cast<float>(v[i]);
-        const bool finite = fabsf(x) < INFINITY;
-        rest[i] = finite ? v[i] : static_cast<T>(0.0F);
-        pos[i] = static_cast<T>(x == INFINITY ? 1.0F : 0.0F);
-        neg[i] = static_cast<T>(x == -INFINITY ? 1.0F : 0.0F);
-        nan[i] = static_cast<T>(x != x ? 1.0F : 0.0F);
+        rest[i] = fabsf(x) < INFINITY ? v[i] : static_cast<T>(0.0F);
+        mark[0][i] = static_cast<T>(x == INFINITY ? 1.0F : 0.0F);
+        mark[1][i] = static_cast<T>(x == -INFINITY ? 1.0F : 0.0F);
+        mark[2][i] = static_cast<T>(x != x ? 1.0F : 0.0F);
     }
-    const float4v zero{0.0F, 0.0F, 0.0F, 0.0F};
-    const float4v a = Values<T>::mfma16(pos, seen, zero), b = Values<T>::mfma16(neg, seen, zero),
-                  c = Values<T>::mfma16(nan, seen, zero);
-    sum = Values<T>::mfma16(rest, p, sum);
+    constexpr int kSums = sizeof(Acc) / sizeof(float);
+    constexpr float kAdds[3] = {INFINITY, -INFINITY, NAN};
+    sum = Values<T>::mfma(rest, p, sum);
 #pragma unroll
-    for (int r = 0; r < 4; ++r) {
-        if (a[r] > 0.0F) sum[r] += INFINITY;
-        if (b[r] > 0.0F) sum[r] -= INFINITY;
-        if (c[r] > 0.0F) sum[r] = NAN;
+    for (int n = 0; n < 3; ++n) {
+        Acc count;
+#pragma unroll
+        for (int r = 0; r < kSums; ++r) count[r] = 0.0F;
+        count = Values<T>::mfma(mark[n], seen, count);
+#pragma unroll
+        for (int r = 0; r < kSums; ++r) {
+            if (count[r] > 0.0F) sum[r] += kAdds[n];
+        }
     }
     return sum;
+}
+
+// Takes the infinities and NaN out of column e of eight rows of four 16-bit values: 0 in their place, their rows' bits in
+// mark (+inf, -inf, NaN).
+template <typename T>
+__device__ __forceinline__ void take_nonfinite(uint2 (&v)[8], int e, uint8_t (&mark)[3]) {
+    constexpr uint32_t exponent = Values<T>::kExponent, mantissa = 0x7FFFU & ~exponent;
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+        uint32_t& two = e < 2 ? v[j].x : v[j].y;
+        const uint32_t x = two >> (16 * (e % 2)) & 0xFFFFU;
+        if ((x & exponent) != exponent) continue;
+        mark[x & mantissa ? 2 : x >> 15] |= static_cast<uint8_t>(1U << j);
+        two &= ~(0xFFFFU << (16 * (e % 2)));
+    }
 }
 
 // Column c of eight rows of 16-bit values, two to a word.
@@ -440,7 +476,7 @@ __global__ __launch_bounds__(kAttendThreads, HDP * MT <= 128 ? 2 : 1) void k_att
             for (int c = 0; c < KC; ++c) {
                 const v8 q = __builtin_bit_cast(v8, q_lds[mt][c][lane]);
 #pragma unroll
-                for (int u = 0; u < 2; ++u) sc[u] = V::mfma16(__builtin_bit_cast(v8, k[u][c]), q, sc[u]);
+                for (int u = 0; u < 2; ++u) sc[u] = V::mfma(__builtin_bit_cast(v8, k[u][c]), q, sc[u]);
             }
             // scores of keys base + 16 u + 4 g + r, query i
             uint32_t seen = 0xFF;
@@ -477,7 +513,7 @@ __global__ __launch_bounds__(kAttendThreads, HDP * MT <= 128 ? 2 : 1) void k_att
             if (!careful) {
 #pragma unroll
                 for (int c = 0; c < VEC; ++c) {
-                    o[mt][c] = V::mfma16(__builtin_bit_cast(v8, column<VW>(v, c)), p, o[mt][c]);
+                    o[mt][c] = V::mfma(__builtin_bit_cast(v8, column<VW>(v, c)), p, o[mt][c]);
                 }
             } else {
                 v8 seen_mark;
@@ -552,6 +588,287 @@ __global__ __launch_bounds__(kAttendThreads, HDP * MT <= 128 ? 2 : 1) void k_att
                 } else {
                     *reinterpret_cast<float2*>(a.marks + 2 * (static_cast<int64_t>(split) * rows_heads + at)) = float2{now, l};
                 }
+            }
+        }
+    }
+}
+
+// Many query rows: 128 queries of a K/V head per work-group, 32 per wave, over tiles of KT keys that the work-group stages
+// in LDS, double-buffered: while a tile is multiplied, the next one's rows are on their way to registers, and the offsets
+// of the one after it are looked up (pages of any size: one lookup per key).
+//
+// 32x32x16 products: S^T = K Q^T has a query per lane and leaves a lane the scores of keys 8 b + 4 g + r (b = 0..3) of a
+// 32-key block; eight consecutive ones are the B operand of O^T += V^T P^T over 16 keys in that order, so P stays in
+// its lane. V goes to LDS transposed, in pieces of 8 keys in the same order (16-bit permutes on the way), so both
+// operands are 16-byte LDS reads. A row of LDS is one piece longer than its values, so that lanes on consecutive rows spread
+// over the banks, and every read of a tile has one address register and an immediate. Block e of O^T has columns HB n + e
+// (HB blocks), whose rows in LDS follow one another. LDS reads set the bound: 32 queries per wave need a byte of LDS for 16
+// operations, the matrix cores' rate at the LDS's.
+// Statistics and rounding as in k_attend_few.
+constexpr int kTileQueries = 128;
+
+template <int HDP> constexpr int kTileKeys = HDP <= 128 ? 64 : 32;
+
+template <typename T, int HDP>
+__global__ __launch_bounds__(kAttendThreads, HDP <= 128 ? 2 : 1) void k_attend_tile(Attend a, int group) {
+    using V = Values<T>;
+    using v8 = typename V::v8;
+    constexpr int KT = kTileKeys<HDP>;
+    constexpr int KB = KT / 32;     // key blocks of S^T
+    constexpr int KC = HDP / 16;    // products per block of S^T
+    constexpr int HB = HDP / 32;    // column blocks of O^T
+    constexpr int CH = HDP / 8;     // pieces of a K row
+    constexpr int KP = KT * CH / kAttendThreads;  // pieces of K per thread
+    constexpr int VG = KT / 8;      // pieces of a V column
+    constexpr int V4 = HDP / 4;     // threads per piece row: four columns each
+    constexpr int VT = VG * V4;     // threads that stage V
+    static_assert(VT <= kAttendThreads && KT <= 64);
+    constexpr int KS = CH + 1, VS = VG + 1;  // pieces of a row in LDS
+    __shared__ uint4 k_lds[2][KT * KS];
+    __shared__ uint4 v_lds[2][HDP * VS];
+    __shared__ int64_t offsets[3][KT];
+    __shared__ unsigned long long there[3];
+    // of tiles that some query does not see whole: the keys (bits) whose V is +inf, -inf, NaN, by column and piece
+    __shared__ alignas(8) uint8_t marks[2][3][HDP][8];
+    __shared__ bool odd[2][kAttendWaves];
+
+    const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64;
+    const int n = lane % 32, g = lane / 32;
+    const uint32_t pairs = a.cache.n_head_kv * a.batch.n_seq;
+    const uint32_t pair = blockIdx.x % pairs, split = blockIdx.x / pairs % a.splits;
+    const uint32_t h = pair % a.cache.n_head_kv, s = pair / a.cache.n_head_kv;
+    const Span span = sequence_span(a.batch, a.q.rows, s);
+    const int queries = span.rows * group;
+    // the last tile of queries, which sees most, first
+    const int m0 = ((queries + kTileQueries - 1) / kTileQueries - 1 - static_cast<int>(blockIdx.x / pairs / a.splits)) * kTileQueries;
+    if (m0 < 0) return;
+    const int dim = static_cast<int>(a.cache.head_dim);
+    const int first = span.len - span.rows;
+
+    const int wm = m0 + 32 * wave, m = wm + n;
+    const Query query = query_of(min(m, queries - 1), group, h);
+    const int64_t row = span.row0 + query.row;
+    v8 q[KC];
+    {
+        const T* x = static_cast<const T*>(a.q.data) + row * a.q.row_stride + query.head * a.q.head_stride;
+#pragma unroll
+        for (int c = 0; c < KC; ++c) {
+            const int d = 16 * c + 8 * g;
+            uint4 y = *reinterpret_cast<const uint4*>(x + (d < dim ? d : 0));
+            if (d >= dim) y = uint4{0, 0, 0, 0};
+            q[c] = __builtin_bit_cast(v8, y);
+        }
+    }
+    const auto sees = [&](int query_index) {  // slots that a query sees
+        return a.causal ? max(0, first + min(query_index, queries - 1) / group + 1) : span.len;
+    };
+    const int limit = sees(m), least = sees(wm), group_least = sees(m0), end = sees(m0 + kTileQueries - 1);
+
+    const int tiles = (span.len + KT - 1) / KT;
+    const int per = (tiles + static_cast<int>(a.splits) - 1) / static_cast<int>(a.splits);
+    const int t0 = static_cast<int>(split) * per, t1 = min(min(tiles, t0 + per), (end + KT - 1) / KT);
+
+    const T* k_head = static_cast<const T*>(a.cache.k) + h * a.cache.head_stride;
+    const T* v_head = static_cast<const T*>(a.cache.v) + h * a.cache.head_stride;
+
+    const auto look_up = [&](int t) {
+        if (wave != 0) return;
+        int64_t at = -1;
+        const int slot = t * KT + lane;
+        if (lane < KT && slot < end) {
+            const int page = page_of(a.cache, a.batch, s, slot);
+            if (page >= 0) at = slot_offset(a.cache, page, slot);
+        }
+        if (lane < KT) offsets[t % 3][lane] = at;
+        const unsigned long long mask = __ballot(at >= 0);
+        if (lane == 0) there[t % 3] = mask;
+    };
+    uint4 kr[KP];
+    uint2 vr[8];
+    const int v_at = 4 * (tid % V4), v_piece = tid / V4;
+    const auto fetch = [&](int t) {
+        const int64_t* at = offsets[t % 3];
+#pragma unroll
+        for (int p = 0; p < KP; ++p) {
+            const int piece = tid + kAttendThreads * p, d = 8 * (piece % CH);
+            kr[p] = *reinterpret_cast<const uint4*>(k_head + max(at[piece / CH], static_cast<int64_t>(0)) + (d < dim ? d : 0));
+            if (d >= dim) kr[p] = uint4{0, 0, 0, 0};
+        }
+        if (VT == kAttendThreads || tid < VT) {
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const int64_t from = at[16 * (v_piece / 2) + 8 * (j / 4) + 4 * (v_piece % 2) + j % 4];
+                vr[j] = *reinterpret_cast<const uint2*>(v_head + max(from, static_cast<int64_t>(0)) + (v_at < dim ? v_at : 0));
+                if (from < 0 || v_at >= dim) vr[j] = uint2{0, 0};  // a number: its weight is 0
+            }
+        }
+    };
+    const auto stage = [&](int t) {
+        const int b = t % 2;
+#pragma unroll
+        for (int p = 0; p < KP; ++p) {
+            const int piece = tid + kAttendThreads * p, key = piece / CH;
+            k_lds[b][key * KS + piece % CH] = kr[p];
+        }
+        bool any = false;
+        if (VT == kAttendThreads || tid < VT) {
+            if ((t + 1) * KT > group_least) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) any |= nonfinite<T>(vr[j].x) || nonfinite<T>(vr[j].y);
+#pragma unroll
+                for (int e = 0; e < 4; ++e) {
+                    uint8_t mark[3] = {0, 0, 0};
+                    if (any) take_nonfinite<T>(vr, e, mark);
+#pragma unroll
+                    for (int k = 0; k < 3; ++k) marks[b][k][v_at + e][v_piece] = mark[k];
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                const uint32_t pick = e % 2 ? 0x07060302U : 0x05040100U;
+                const auto two = [&](int j) {
+                    return e < 2 ? __builtin_amdgcn_perm(vr[j + 1].x, vr[j].x, pick) : __builtin_amdgcn_perm(vr[j + 1].y, vr[j].y, pick);
+                };
+                v_lds[b][((v_at + e) % HB * 32 + (v_at + e) / HB) * VS + v_piece] = uint4{two(0), two(2), two(4), two(6)};
+            }
+        }
+        any = __ballot(any) != 0;
+        if (lane == 0) odd[b][wave] = any;
+    };
+
+    float16v o[HB];
+#pragma unroll
+    for (int e = 0; e < HB; ++e) {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) o[e][r] = 0.0F;
+    }
+    float top = -INFINITY, sum = 0.0F;
+
+    if (t0 < t1) {
+        look_up(t0);
+        look_up(t0 + 1);
+        __syncthreads();
+        fetch(t0);
+        stage(t0);
+        __syncthreads();
+    }
+    for (int t = t0; t < t1; ++t) {
+        const int b = t % 2, base = t * KT;
+        if (t + 1 < t1) fetch(t + 1);
+        if (t + 2 < t1) look_up(t + 2);
+
+        float16v sc[KB];
+#pragma unroll
+        for (int e = 0; e < KB; ++e) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) sc[e][r] = 0.0F;
+#pragma unroll
+            for (int c = 0; c < KC; ++c) {
+                const uint4 k = k_lds[b][(32 * e + n) * KS + 2 * c + g];
+                sc[e] = V::mfma(__builtin_bit_cast(v8, k), q[c], sc[e]);
+            }
+        }
+        const unsigned long long present = there[t % 3];
+        const bool hidden = base + KT > least;
+        if (hidden || present != (~0ULL >> (64 - KT))) {
+#pragma unroll
+            for (int e = 0; e < KB; ++e) {
+                // keys 32 e + 4 g + 8 (r / 4) + r % 4
+                const uint32_t here = static_cast<uint32_t>(present >> (32 * e + 4 * g));
+                const int left = limit - base - 32 * e - 4 * g;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int key = 8 * (r / 4) + r % 4;
+                    if (key >= left || !(here >> key & 1U)) sc[e][r] = -INFINITY;
+                }
+            }
+        }
+        float most = sc[0][0];
+#pragma unroll
+        for (int e = 0; e < KB; ++e) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) most = fmaxf(most, sc[e][r]);
+        }
+        most = halves_max(most) * a.scale_log2;
+        if (__ballot(most > top + kRescale)) {
+            const float now = fmaxf(top, most);
+            const float shrink = now == -INFINITY ? 1.0F : exp2f(top - now);
+            top = now;
+            sum *= shrink;
+#pragma unroll
+            for (int e = 0; e < HB; ++e) o[e] *= shrink;
+        }
+        const float ref = top == -INFINITY ? 0.0F : top;
+        v8 p[KB][2];
+#pragma unroll
+        for (int e = 0; e < KB; ++e) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const float w = __builtin_amdgcn_exp2f(fmaf(sc[e][r], a.scale_log2, -ref));
+                sum += w;
+                p[e][r / 8][r % 8] = static_cast<T>(w);
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < HB; ++e) {
+#pragma unroll
+            for (int c = 0; c < 2 * KB; ++c) {
+                const uint4 v = v_lds[b][(32 * e + n) * VS + 2 * c + g];
+                o[e] = V::mfma(__builtin_bit_cast(v8, v), p[c / 2][c % 2], o[e]);
+            }
+        }
+        if (hidden && (odd[b][0] || odd[b][1] || odd[b][2] || odd[b][3])) {
+            // what the tile's V has of infinities and NaN, staged as 0, for the queries that see them
+            unsigned long long seen = 0;
+            for (int k = 0; k < KT; ++k) {
+                const int key = 16 * (k / 16) + 8 * (k % 8 / 4) + 4 * (k / 8 % 2) + k % 4;
+                seen |= static_cast<unsigned long long>(base + key < limit && (present >> key & 1ULL)) << k;
+            }
+#pragma unroll
+            for (int e = 0; e < HB; ++e) {
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int d = HB * (8 * (r / 4) + 4 * g + r % 4) + e;
+                    const auto any = [&](int k) {
+                        return (*reinterpret_cast<const unsigned long long*>(marks[b][k][d]) & seen) != 0;
+                    };
+                    if (any(0)) o[e][r] += INFINITY;
+                    if (any(1)) o[e][r] -= INFINITY;
+                    if (any(2)) o[e][r] = NAN;
+                    asm volatile("" ::: "memory");  // one column's marks at a time: the sums leave few registers
+                }
+            }
+        }
+        if (t + 1 < t1) stage(t + 1);
+        __syncthreads();
+    }
+
+    if (m >= queries) return;
+    const float l = halves_sum(sum);
+    const int64_t at = row * a.q.heads + query.head, all = static_cast<int64_t>(a.q.rows) * a.q.heads;
+    const bool whole = a.splits == 1;
+    if (g == 0) {
+        if (!whole) *reinterpret_cast<float2*>(a.marks + 2 * (split * all + at)) = float2{top, l};
+        else if (a.lse) a.lse[at] = top * kLn2 + logf(l);
+    }
+    if (!whole && l == 0.0F) return;  // nothing seen: the join does not read it
+    const float scale = whole ? (l == 0.0F ? 0.0F : 1.0F / l) : 1.0F;
+    // rows 8 b + 4 g + r of the blocks: 4 HB consecutive columns, four at a time
+#pragma unroll
+    for (int b = 0; b < 4; ++b) {
+#pragma unroll
+        for (int f = 0; f < HB; ++f) {
+            const int d = HB * (8 * b + 4 * g) + 4 * f;
+            if (d >= dim) continue;
+            float x[4];
+#pragma unroll
+            for (int e = 0; e < 4; ++e) x[e] = o[(4 * f + e) % HB][4 * b + (4 * f + e) / HB] * scale;
+            if (whole) {
+                T* to = static_cast<T*>(a.out.data) + row * a.out.row_stride + query.head * a.out.head_stride + d;
+                const T y[4] = {static_cast<T>(x[0]), static_cast<T>(x[1]), static_cast<T>(x[2]), static_cast<T>(x[3])};
+                __builtin_memcpy(__builtin_assume_aligned(to, 8), y, 8);
+            } else {
+                *reinterpret_cast<float4v*>(a.partial + (split * all + at) * dim + d) = float4v{x[0], x[1], x[2], x[3]};
             }
         }
     }
@@ -675,7 +992,7 @@ __global__ __launch_bounds__(kWeighThreads) void k_weigh(Weigh a, int group, int
             uint4 y = *reinterpret_cast<const uint4*>(x + (d < dim ? d : 0));
             if (d >= dim) y = uint4{0, 0, 0, 0};
 #pragma unroll
-            for (int u = 0; u < 2; ++u) sc[u] = V::mfma16(__builtin_bit_cast(v8, k[u][c]), __builtin_bit_cast(v8, y), sc[u]);
+            for (int u = 0; u < 2; ++u) sc[u] = V::mfma(__builtin_bit_cast(v8, k[u][c]), __builtin_bit_cast(v8, y), sc[u]);
         }
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
@@ -925,40 +1242,61 @@ hipError_t launch_append(const Rotation* rotation, const Cache& c, const Batch& 
 
 namespace {
 
-// Tiles of 16 queries per work-group: as many as a sequence may have, up to what the registers hold (4; 2 of wide heads).
-uint32_t few_tiles(uint32_t head_dim, uint64_t queries) { return queries <= 16 ? 1 : queries <= 32 || head_dim > 128 ? 2 : 4; }
+// Queries (rows times the heads of a K/V head) of a sequence up to which the waves of a work-group divide its keys.
+constexpr uint32_t kFewQueries = 64;
+
+// How a step's attention is divided: by the most queries that a sequence may have.
+struct Tiling {
+    uint32_t queries;  // of a work-group
+    uint32_t keys;     // that its waves take at a time, all together
+    uint64_t groups;   // work-groups per split
+};
+
+Tiling tiling(const Cache& c, const Batch& b, uint32_t group) {
+    const uint64_t most = static_cast<uint64_t>(b.max_rows) * group;
+    Tiling t;
+    if (most <= kFewQueries) {
+        // tiles of 16 queries: 1, 2 or as many as the registers hold (4; 2 of wide heads)
+        t.queries = most <= 16 ? 16 : most <= 32 || c.head_dim > 128 ? 32 : 64;
+        t.keys = kAttendWaves * kFewKeys;
+    } else {
+        t.queries = kTileQueries;
+        t.keys = c.head_dim <= 128 ? kTileKeys<128> : kTileKeys<256>;
+    }
+    t.groups = (most + t.queries - 1) / t.queries * c.n_head_kv * b.n_seq;
+    return t;
+}
 
 template <typename T, int HDP>
-hipError_t attend_few(const Attend& a, hipStream_t stream) {
+hipError_t attend_of(const Attend& a, hipStream_t stream) {
     const int group = static_cast<int>(a.q.heads / a.cache.n_head_kv);
-    const uint64_t queries = static_cast<uint64_t>(a.batch.max_rows) * group;
-    const uint32_t mt = few_tiles(a.cache.head_dim, queries);
-    const uint64_t groups = (queries + 16 * mt - 1) / (16 * mt) * a.cache.n_head_kv * a.batch.n_seq * a.splits;
+    const Tiling t = tiling(a.cache, a.batch, a.q.heads / a.cache.n_head_kv);
+    const uint64_t groups = t.groups * a.splits;
     if (groups > 0x7FFFFFFF) return hipErrorInvalidConfiguration;
-    const dim3 grid(static_cast<uint32_t>(groups));
-    const dim3 block(kAttendThreads);
-    if (mt == 1) return launch(k_attend_few<T, HDP, 1>, grid, block, stream, a, group);
-    if (mt == 2) return launch(k_attend_few<T, HDP, 2>, grid, block, stream, a, group);
+    const dim3 grid(static_cast<uint32_t>(groups)), block(kAttendThreads);
+    if (t.queries == kTileQueries) return launch(k_attend_tile<T, HDP>, grid, block, stream, a, group);
+    if (t.queries == 16) return launch(k_attend_few<T, HDP, 1>, grid, block, stream, a, group);
+    if (t.queries == 32) return launch(k_attend_few<T, HDP, 2>, grid, block, stream, a, group);
     if constexpr (HDP <= 128) return launch(k_attend_few<T, HDP, 4>, grid, block, stream, a, group);
-    return hipErrorInvalidValue;
+    return hipErrorInvalidConfiguration;
 }
 
 template <typename T>
 hipError_t attend(const Attend& a, hipStream_t stream) {
-    if (a.cache.head_dim <= 64) return attend_few<T, 64>(a, stream);
-    if (a.cache.head_dim <= 128) return attend_few<T, 128>(a, stream);
-    return attend_few<T, 256>(a, stream);
+    if (a.cache.head_dim <= 64) return attend_of<T, 64>(a, stream);
+    if (a.cache.head_dim <= 128) return attend_of<T, 128>(a, stream);
+    return attend_of<T, 256>(a, stream);
 }
 
 }  // namespace
 
 uint32_t attend_splits(const Cache& c, const Batch& b, uint32_t group) {
-    const uint64_t queries = static_cast<uint64_t>(b.max_rows) * group;
-    const uint32_t mt = few_tiles(c.head_dim, queries);
-    const uint64_t groups = c.n_head_kv * static_cast<uint64_t>(b.n_seq) * ((queries + 16 * mt - 1) / (16 * mt));
-    // two work-groups per compute unit; a split of fewer than two tiles per wave costs more than it gains
-    const uint64_t wanted = groups ? (2 * kComputeUnits + groups - 1) / groups : 1;
-    const uint64_t most = b.max_length / (2 * kAttendWaves * kFewKeys);
+    const Tiling t = tiling(c, b, group);
+    if (t.groups == 0) return 1;
+    // two work-groups per compute unit, unless there is one without splits; a split of fewer than two rounds of keys costs
+    // more than it gains
+    if (t.groups >= kComputeUnits) return 1;
+    const uint64_t wanted = (2 * kComputeUnits + t.groups - 1) / t.groups, most = b.max_length / (2 * t.keys);
     return static_cast<uint32_t>(wanted < most ? wanted : most > 0 ? most : 1);
 }
 
