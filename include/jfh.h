@@ -525,9 +525,12 @@ jfh_status jfh_paged_attention(const jfh_paged_cache * cache, const jfh_paged_ba
  * jfh_paged_attention had them (q may hold a part of its rows: the batch's row
  * starts say which, at the sequences' last slots). f32, in one order whatever
  * the launch; a row whose lse is -inf adds nothing. No two sequences may share
- * a page. */
+ * a page. workspace as for jfh_paged_attention. */
+jfh_status jfh_paged_weigh_workspace(const jfh_paged_cache * cache, const jfh_paged_batch * batch, const jfh_rows * q,
+                                     size_t * bytes);
 jfh_status jfh_paged_weigh(const jfh_paged_cache * cache, const jfh_paged_batch * batch, const jfh_rows * q,
-                           const float * lse, float scale, uint32_t causal, void * stream);
+                           const float * lse, float scale, uint32_t causal, void * workspace, size_t workspace_bytes,
+                           void * stream);
 
 /* Cuts every sequence of more than `budget` slots down to `budget`, for each
  * K/V head by itself: of its slots the first `budget` stay in the order

@@ -191,8 +191,9 @@ SIGNATURES = {
                                                POINTER(c_size_t)]),
     "jfh_paged_attention": (Status, [POINTER(PagedCache), POINTER(PagedBatch), POINTER(Rows), c_float, c_uint32,
                                      POINTER(Rows), c_void_p, c_void_p, c_size_t, c_void_p]),
+    "jfh_paged_weigh_workspace": (Status, [POINTER(PagedCache), POINTER(PagedBatch), POINTER(Rows), POINTER(c_size_t)]),
     "jfh_paged_weigh": (Status, [POINTER(PagedCache), POINTER(PagedBatch), POINTER(Rows), c_void_p, c_float, c_uint32,
-                                 c_void_p]),
+                                 c_void_p, c_size_t, c_void_p]),
     "jfh_paged_evict_workspace": (Status, [POINTER(PagedCache), POINTER(PagedBatch), c_uint32, POINTER(c_size_t)]),
     "jfh_paged_evict": (Status, [POINTER(PagedCache), POINTER(PagedBatch), c_uint32, c_uint32, c_uint32, c_void_p,
                                  c_size_t, c_void_p]),

@@ -169,6 +169,17 @@ AttendPlan attend_plan(const paged::Cache& c, const paged::Batch& b, const paged
     return p;
 }
 
+struct WeighPlan {
+    uint32_t splits;
+    size_t bytes;
+};
+
+WeighPlan weigh_plan(const paged::Cache& c, const paged::Batch& b, const paged::Rows& q) {
+    WeighPlan p{b.n_seq ? paged::weigh_splits(c, b, q.heads / c.n_head_kv) : 1, 0};
+    if (p.splits > 1) p.bytes = static_cast<size_t>(p.splits) * c.n_head_kv * b.n_seq * b.max_length * sizeof(float);
+    return p;
+}
+
 // Most positions of a K/V head that move when sequences are cut, and the bytes of the lists that say which.
 uint32_t evict_width(const paged::Batch& b, uint32_t budget) {
     return b.max_length > budget ? std::min(budget, b.max_length - budget) : 0;
@@ -271,8 +282,18 @@ jfh_status jfh_paged_attention(const jfh_paged_cache* cache, const jfh_paged_bat
     });
 }
 
+jfh_status jfh_paged_weigh_workspace(const jfh_paged_cache* cache, const jfh_paged_batch* batch, const jfh_rows* q,
+                                     size_t* bytes) {
+    return guarded([&] {
+        require(bytes != nullptr, "an output for the workspace's size is required");
+        const paged::Cache c = cache_of(cache);
+        const paged::Rows x = attended(q, c, "q");
+        *bytes = weigh_plan(c, batch_of(batch, *cache, true, x.rows), x).bytes;
+    });
+}
+
 jfh_status jfh_paged_weigh(const jfh_paged_cache* cache, const jfh_paged_batch* batch, const jfh_rows* q, const float* lse,
-                           float scale, uint32_t causal, void* stream) {
+                           float scale, uint32_t causal, void* workspace, size_t workspace_bytes, void* stream) {
     return guarded([&] {
         paged::Weigh a{};
         a.cache = cache_of(cache);
@@ -284,6 +305,11 @@ jfh_status jfh_paged_weigh(const jfh_paged_cache* cache, const jfh_paged_batch* 
         if (a.q.rows == 0 || a.batch.n_seq == 0 || a.batch.max_rows == 0 || a.batch.max_length == 0) return;
         require(lse != nullptr && aligned(lse, 4), "lse is required");
         a.lse = lse;
+        const WeighPlan p = weigh_plan(a.cache, a.batch, a.q);
+        require(workspace_bytes >= p.bytes && (p.splits == 1 || workspace) && aligned(workspace, 16),
+                "weighing this step needs " + std::to_string(p.bytes) + " bytes of workspace, 16-byte aligned");
+        a.splits = p.splits;
+        a.partial = static_cast<float*>(workspace);
         const OnDevice guard(cache->device);
         check(paged::launch_weigh(a, static_cast<hipStream_t>(stream)), "weigh positions");
     });

@@ -329,6 +329,14 @@ constexpr int kAttendWaves = 4;
 constexpr int kFewKeys = 32;    // keys of a wave's tile
 constexpr float kRescale = 8.0F;  // a row's running maximum is raised when a tile exceeds it by this (base 2)
 
+// Eight values of a row from column d, 0 from column dim on.
+template <typename T>
+__device__ __forceinline__ typename Values<T>::v8 row_piece(const T* row, int d, int dim) {
+    uint4 x = *reinterpret_cast<const uint4*>(row + (d < dim ? d : 0));
+    if (d >= dim) x = uint4{0, 0, 0, 0};
+    return __builtin_bit_cast(typename Values<T>::v8, x);
+}
+
 // Query m of a K/V head's rows * group queries is head m % group of the sequence's row m / group.
 struct Query {
     int row, head;
@@ -622,7 +630,8 @@ __global__ __launch_bounds__(kAttendThreads, HDP <= 128 ? 2 : 1) void k_attend_t
     constexpr int VG = KT / 8;      // pieces of a V column
     constexpr int V4 = HDP / 4;     // threads per piece row: four columns each
     constexpr int VT = VG * V4;     // threads that stage V
-    static_assert(VT <= kAttendThreads && KT <= 64);
+    static_assert(VT <= kAttendThreads && KT <= 64 && kAttendThreads % CH == 0);
+    constexpr unsigned long long kAllKeys = ~0ULL >> (64 - KT);
     constexpr int KS = CH + 1, VS = VG + 1;  // pieces of a row in LDS
     __shared__ uint4 k_lds[2][KT * KS];
     __shared__ uint4 v_lds[2][HDP * VS];
@@ -673,33 +682,29 @@ __global__ __launch_bounds__(kAttendThreads, HDP <= 128 ? 2 : 1) void k_attend_t
 
     const auto look_up = [&](int t) {
         if (wave != 0) return;
-        int64_t at = -1;
         const int slot = t * KT + lane;
-        if (lane < KT && slot < end) {
-            const int page = page_of(a.cache, a.batch, s, slot);
-            if (page >= 0) at = slot_offset(a.cache, page, slot);
-        }
-        if (lane < KT) offsets[t % 3][lane] = at;
-        const unsigned long long mask = __ballot(at >= 0);
+        const int page = lane < KT && slot < end ? page_of(a.cache, a.batch, s, slot) : -1;
+        // of a row that is not there: any that is
+        if (lane < KT) offsets[t % 3][lane] = page >= 0 ? slot_offset(a.cache, page, slot) : 0;
+        const unsigned long long mask = __ballot(page >= 0);
         if (lane == 0) there[t % 3] = mask;
     };
     uint4 kr[KP];
     uint2 vr[8];
     const int v_at = 4 * (tid % V4), v_piece = tid / V4;
+    const int k_at = 8 * (tid % CH);
+    const T* k_from = k_head + (k_at < dim ? k_at : 0);
+    const T* v_from = v_head + (v_at < dim ? v_at : 0);
     const auto fetch = [&](int t) {
         const int64_t* at = offsets[t % 3];
 #pragma unroll
         for (int p = 0; p < KP; ++p) {
-            const int piece = tid + kAttendThreads * p, d = 8 * (piece % CH);
-            kr[p] = *reinterpret_cast<const uint4*>(k_head + max(at[piece / CH], static_cast<int64_t>(0)) + (d < dim ? d : 0));
-            if (d >= dim) kr[p] = uint4{0, 0, 0, 0};
+            kr[p] = *reinterpret_cast<const uint4*>(k_from + at[(tid + kAttendThreads * p) / CH]);
         }
         if (VT == kAttendThreads || tid < VT) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const int64_t from = at[16 * (v_piece / 2) + 8 * (j / 4) + 4 * (v_piece % 2) + j % 4];
-                vr[j] = *reinterpret_cast<const uint2*>(v_head + max(from, static_cast<int64_t>(0)) + (v_at < dim ? v_at : 0));
-                if (from < 0 || v_at >= dim) vr[j] = uint2{0, 0};  // a number: its weight is 0
+                vr[j] = *reinterpret_cast<const uint2*>(v_from + at[16 * (v_piece / 2) + 8 * (j / 4) + 4 * (v_piece % 2) + j % 4]);
             }
         }
     };
@@ -707,11 +712,19 @@ __global__ __launch_bounds__(kAttendThreads, HDP <= 128 ? 2 : 1) void k_attend_t
         const int b = t % 2;
 #pragma unroll
         for (int p = 0; p < KP; ++p) {
-            const int piece = tid + kAttendThreads * p, key = piece / CH;
-            k_lds[b][key * KS + piece % CH] = kr[p];
+            if (k_at >= dim) kr[p] = uint4{0, 0, 0, 0};
+            k_lds[b][(tid + kAttendThreads * p) / CH * KS + tid % CH] = kr[p];
         }
         bool any = false;
         if (VT == kAttendThreads || tid < VT) {
+            const unsigned long long present = there[t % 3];
+            if (present != kAllKeys || v_at >= dim) {  // what is not there must be a number: its weight is 0
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int key = 16 * (v_piece / 2) + 8 * (j / 4) + 4 * (v_piece % 2) + j % 4;
+                    if (!(present >> key & 1ULL) || v_at >= dim) vr[j] = uint2{0, 0};
+                }
+            }
             if ((t + 1) * KT > group_least) {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) any |= nonfinite<T>(vr[j].x) || nonfinite<T>(vr[j].y);
@@ -762,15 +775,18 @@ __global__ __launch_bounds__(kAttendThreads, HDP <= 128 ? 2 : 1) void k_attend_t
         for (int e = 0; e < KB; ++e) {
 #pragma unroll
             for (int r = 0; r < 16; ++r) sc[e][r] = 0.0F;
+        }
 #pragma unroll
-            for (int c = 0; c < KC; ++c) {
+        for (int c = 0; c < KC; ++c) {
+#pragma unroll
+            for (int e = 0; e < KB; ++e) {
                 const uint4 k = k_lds[b][(32 * e + n) * KS + 2 * c + g];
                 sc[e] = V::mfma(__builtin_bit_cast(v8, k), q[c], sc[e]);
             }
         }
         const unsigned long long present = there[t % 3];
         const bool hidden = base + KT > least;
-        if (hidden || present != (~0ULL >> (64 - KT))) {
+        if (hidden || present != kAllKeys) {
 #pragma unroll
             for (int e = 0; e < KB; ++e) {
                 // keys 32 e + 4 g + 8 (r / 4) + r % 4
@@ -810,9 +826,9 @@ __global__ __launch_bounds__(kAttendThreads, HDP <= 128 ? 2 : 1) void k_attend_t
             }
         }
 #pragma unroll
-        for (int e = 0; e < HB; ++e) {
+        for (int c = 0; c < 2 * KB; ++c) {
 #pragma unroll
-            for (int c = 0; c < 2 * KB; ++c) {
+            for (int e = 0; e < HB; ++e) {
                 const uint4 v = v_lds[b][(32 * e + n) * VS + 2 * c + g];
                 o[e] = V::mfma(__builtin_bit_cast(v8, v), p[c / 2][c % 2], o[e]);
             }
@@ -929,99 +945,220 @@ __global__ __launch_bounds__(kJoinThreads) void k_attend_join(Attend a) {
 // ---------------------------------------------------------------- attention weights
 
 // weights[slot] += sum over the step's queries of a K/V head of exp(scale q k - lse): the columns of the probabilities,
-// summed. A wave owns 32 slots, whose K rows stay in registers as A operands, and goes over the queries 16 at a time; each
-// sum has one owner and one order, so results do not depend on the launch. The sums of 512 queries at a time are added to a
-// total, which keeps the f32 error of long prompts at that of a few hundred terms.
-constexpr int kWeighThreads = 256;
-constexpr int kWeighKeys = 32;   // slots of a wave
-constexpr int kWeighFlush = 32;  // query tiles between additions to the total
+// summed. A wave owns 16 U slots, whose K rows stay in registers as A operands of 16x16x32 products, and goes over the
+// queries. Each sum has one owner and one order, so results do not depend on the launch.
 
+constexpr int kWeighThreads = 256;
+constexpr int kWeighWaves = kWeighThreads / 64;
+constexpr int kFewWeighSlots = 32;  // of a wave
+
+// The K rows of a wave's slots, zeros beyond head_dim; where their weights lie, -1 for slots that are not there.
+template <typename T, int U, int KC>
+__device__ __forceinline__ void weighed_rows(const Weigh& a, uint32_t s, uint32_t h, int len, int base,
+                                             typename Values<T>::v8 (&k)[U][KC], int64_t (&index)[U]) {
+    const int i = threadIdx.x % 16, g = threadIdx.x % 64 / 16;
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+        const int slot = base + 16 * u + i;
+        const int page = slot < len ? page_of(a.cache, a.batch, s, slot) : -1;
+        index[u] = page >= 0 ? slot_index(a.cache, page, h, slot) : -1;
+        const T* row = static_cast<const T*>(a.cache.k) + h * a.cache.head_stride + (page >= 0 ? slot_offset(a.cache, page, slot) : 0);
+#pragma unroll
+        for (int c = 0; c < KC; ++c) k[u][c] = row_piece<T>(row, 32 * c + 8 * g, static_cast<int>(a.cache.head_dim));
+    }
+}
+
+// sum += the weights of 16 queries (lane i's: its lse in base 2, the slots it sees) for the wave's slots from `base`. All
+// seen: every query sees every one of the slots.
+template <typename T, bool ALL_SEEN, int U, int KC>
+__device__ __forceinline__ void weigh_queries(const Weigh& a, int base, const typename Values<T>::v8 (&k)[U][KC],
+                                              const typename Values<T>::v8 (&q)[KC], float ref, int limit, float4v (&sum)[U]) {
+    const int g = threadIdx.x % 64 / 16;
+    float4v sc[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) sc[u] = float4v{0.0F, 0.0F, 0.0F, 0.0F};
+#pragma unroll
+    for (int c = 0; c < KC; ++c) {
+#pragma unroll
+        for (int u = 0; u < U; ++u) sc[u] = Values<T>::mfma(k[u][c], q[c], sc[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const float p = __builtin_amdgcn_exp2f(fmaf(sc[u][r], a.scale_log2, -ref));
+            sum[u][r] += ALL_SEEN || base + 16 * u + 4 * g + r < limit ? p : 0.0F;
+        }
+    }
+}
+
+// Few queries: the K rows' bytes bound the call. 32 slots per wave, the queries' operands straight from memory.
 template <typename T, int HDP>
-__global__ __launch_bounds__(kWeighThreads) void k_weigh(Weigh a, int group, int blocks) {
-    using V = Values<T>;
-    using v8 = typename V::v8;
-    constexpr int KC = HDP / 32;
+__global__ __launch_bounds__(kWeighThreads) void k_weigh_few(Weigh a, int group, int blocks) {
+    using v8 = typename Values<T>::v8;
+    constexpr int KC = HDP / 32, U = kFewWeighSlots / 16;
     const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
     const int i = lane % 16, g = lane / 16;
     const uint32_t pair = blockIdx.x / blocks;
     const uint32_t h = pair % a.cache.n_head_kv, s = pair / a.cache.n_head_kv;
     const Span span = sequence_span(a.batch, a.q.rows, s);
-    const int base = (static_cast<int>(blockIdx.x % blocks) * (kWeighThreads / 64) + wave) * kWeighKeys;
+    const int base = (static_cast<int>(blockIdx.x % blocks) * kWeighWaves + wave) * kFewWeighSlots;
     const int queries = span.rows * group;
     if (base >= span.len || queries == 0) return;
-    const int dim = static_cast<int>(a.cache.head_dim), first = span.len - span.rows;
+    const int first = span.len - span.rows;
 
-    int64_t at[2], index[2];
-    uint32_t present[2];
-    uint4 k[2][KC];
+    int64_t index[U];
+    v8 k[U][KC];
+    weighed_rows<T>(a, s, h, span.len, base, k, index);
+    float4v sum[U];
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-        const int slot = base + 16 * u + i;
-        const int page = slot < span.len ? page_of(a.cache, a.batch, s, slot) : -1;
-        at[u] = page >= 0 ? slot_offset(a.cache, page, slot) : 0;
-        index[u] = page >= 0 ? slot_index(a.cache, page, h, slot) : 0;
-        present[u] = static_cast<uint32_t>(__ballot(page >= 0)) & 0xFFFFU;
-        const T* row = static_cast<const T*>(a.cache.k) + h * a.cache.head_stride + at[u];
+    for (int u = 0; u < U; ++u) sum[u] = float4v{0.0F, 0.0F, 0.0F, 0.0F};
+    // from the first row that sees slot `base`
+    for (int m0 = a.causal ? max(0, base - first) * group / 16 * 16 : 0; m0 < queries; m0 += 16) {
+        const Query query = query_of(min(m0 + i, queries - 1), group, h);
+        const int64_t row = span.row0 + query.row;
+        const T* x = static_cast<const T*>(a.q.data) + row * a.q.row_stride + query.head * a.q.head_stride;
+        v8 q[KC];
 #pragma unroll
-        for (int c = 0; c < KC; ++c) {
-            const int d = 32 * c + 8 * g;
-            k[u][c] = *reinterpret_cast<const uint4*>(row + (d < dim ? d : 0));
-            if (d >= dim) k[u][c] = uint4{0, 0, 0, 0};
-        }
-    }
-
-    float4v total[2], part[2];
-#pragma unroll
-    for (int u = 0; u < 2; ++u) total[u] = part[u] = float4v{0.0F, 0.0F, 0.0F, 0.0F};
-    // the first row that sees slot `base`
-    const int from = a.causal ? max(0, base - first) * group / 16 * 16 : 0;
-    int tiles = 0;
-    for (int m0 = from; m0 < queries; m0 += 16) {
-        const int m = m0 + i;
-        const Query q = query_of(min(m, queries - 1), group, h);
-        const int64_t row = span.row0 + q.row;
-        const T* x = static_cast<const T*>(a.q.data) + row * a.q.row_stride + q.head * a.q.head_stride;
-        const float lse = a.lse[row * a.q.heads + q.head];
+        for (int c = 0; c < KC; ++c) q[c] = row_piece<T>(x, 32 * c + 8 * g, static_cast<int>(a.cache.head_dim));
+        const float lse = a.lse[row * a.q.heads + query.head];
         // a row that saw nothing adds nothing
-        const int limit = m >= queries || lse == -INFINITY ? 0 : a.causal ? first + q.row + 1 : span.len;
-        const float ref = lse * kLog2e;
-        float4v sc[2] = {float4v{0.0F, 0.0F, 0.0F, 0.0F}, float4v{0.0F, 0.0F, 0.0F, 0.0F}};
-#pragma unroll
-        for (int c = 0; c < KC; ++c) {
-            const int d = 32 * c + 8 * g;
-            uint4 y = *reinterpret_cast<const uint4*>(x + (d < dim ? d : 0));
-            if (d >= dim) y = uint4{0, 0, 0, 0};
-#pragma unroll
-            for (int u = 0; u < 2; ++u) sc[u] = V::mfma(__builtin_bit_cast(v8, k[u][c]), __builtin_bit_cast(v8, y), sc[u]);
-        }
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const float p = __builtin_amdgcn_exp2f(fmaf(sc[u][r], a.scale_log2, -ref));
-                part[u][r] += base + 16 * u + 4 * g + r < limit ? p : 0.0F;
-            }
-        }
-        if (++tiles % kWeighFlush == 0) {
-#pragma unroll
-            for (int u = 0; u < 2; ++u) {
-                total[u] += part[u];
-                part[u] = float4v{0.0F, 0.0F, 0.0F, 0.0F};
-            }
-        }
+        const int limit = m0 + i >= queries || lse == -INFINITY ? 0 : a.causal ? first + query.row + 1 : span.len;
+        weigh_queries<T, false>(a, base, k, q, lse * kLog2e, limit, sum);
     }
 #pragma unroll
-    for (int u = 0; u < 2; ++u) {
-        total[u] += part[u];
+    for (int u = 0; u < U; ++u) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            float x = total[u][r];
+            float x = sum[u][r];
 #pragma unroll
             for (int o = 1; o < 16; o *= 2) x += __shfl_xor(x, o);
             const int64_t to = __shfl(index[u], 4 * g + r);
-            if (i == 0 && (present[u] >> (4 * g + r) & 1U)) a.cache.weights[to] += x;
+            if (i == 0 && to >= 0) a.cache.weights[to] += x;
         }
     }
+}
+
+// Many queries: products and exponentials bound the call, after the traffic of Q, which every work-group reads for its
+// slots. So a work-group has 256 slots (128 of wide heads) and stages 64 queries at a time in LDS for its four waves,
+// double-buffered; where that leaves the chip idle, the queries are divided into `splits` parts, whose sums go to the
+// workspace and are added in order.
+template <int HDP> constexpr int kWeighTiles = HDP <= 128 ? 4 : 2;  // 16-slot tiles of a wave
+
+template <typename T, int HDP>
+__global__ __launch_bounds__(kWeighThreads, 2) void k_weigh_many(Weigh a, int group, int blocks) {
+    using v8 = typename Values<T>::v8;
+    constexpr int KC = HDP / 32, U = kWeighTiles<HDP>, CH = HDP / 8, QS = CH + 1, QT = 64, KP = QT * CH / kWeighThreads;
+    __shared__ uint4 q_lds[2][QT * QS];
+    __shared__ float refs[2][QT];
+    __shared__ int limits[2][QT];
+    const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64;
+    const int i = lane % 16, g = lane / 16;
+    const uint32_t split = blockIdx.x / blocks % a.splits, pair = blockIdx.x / blocks / a.splits;
+    const uint32_t h = pair % a.cache.n_head_kv, s = pair / a.cache.n_head_kv;
+    const Span span = sequence_span(a.batch, a.q.rows, s);
+    const int group_base = static_cast<int>(blockIdx.x % blocks) * kWeighWaves * 16 * U, base = group_base + wave * 16 * U;
+    const int queries = span.rows * group;
+    if (group_base >= span.len) return;
+    const int first = span.len - span.rows, dim = static_cast<int>(a.cache.head_dim);
+
+    int64_t index[U];
+    v8 k[U][KC];
+    weighed_rows<T>(a, s, h, span.len, base, k, index);
+
+    // the split's queries, in whole tiles, from the first row that sees the work-group's first slot
+    const int from = a.causal ? max(0, group_base - first) * group / QT : 0;
+    const int tiles = (queries + QT - 1) / QT - from, per = (tiles + static_cast<int>(a.splits) - 1) / static_cast<int>(a.splits);
+    const int t0 = from + min(static_cast<int>(split) * per, tiles), t1 = from + min(static_cast<int>(split + 1) * per, tiles);
+
+    // the thread's pieces of a tile: rows tid / CH + p (256 / CH), advanced by a tile at a time
+    uint4 staged[KP];
+    int at_row[KP], at_head[KP];
+    const int row_step = QT / group, head_step = QT - row_step * group;
+#pragma unroll
+    for (int p = 0; p < KP; ++p) {
+        const Query query = query_of(QT * t0 + (tid + kWeighThreads * p) / CH, group, 0);
+        at_row[p] = query.row;
+        at_head[p] = query.head;
+    }
+    const auto fetch = [&] {
+#pragma unroll
+        for (int p = 0; p < KP; ++p) {
+            const int64_t row = span.row0 + min(at_row[p], span.rows - 1), head = static_cast<int>(h) * group + at_head[p];
+            const int d = 8 * (tid % CH);
+            staged[p] = __builtin_bit_cast(uint4, row_piece<T>(static_cast<const T*>(a.q.data) + row * a.q.row_stride +
+                                                                   head * a.q.head_stride, d, dim));
+            at_row[p] += row_step;
+            at_head[p] += head_step;
+            if (at_head[p] >= group) at_head[p] -= group, ++at_row[p];
+        }
+    };
+    const auto stage = [&](int t) {
+        const int b = t % 2;
+#pragma unroll
+        for (int p = 0; p < KP; ++p) q_lds[b][(tid + kWeighThreads * p) / CH * QS + tid % CH] = staged[p];
+        if (tid < QT) {
+            const int m = QT * t + tid;
+            const Query query = query_of(min(m, queries - 1), group, h);
+            const float lse = a.lse[(span.row0 + query.row) * static_cast<int64_t>(a.q.heads) + query.head];
+            // a row that saw nothing adds nothing
+            limits[b][tid] = m >= queries || lse == -INFINITY ? 0 : a.causal ? first + query.row + 1 : span.len;
+            refs[b][tid] = lse * kLog2e;
+        }
+    };
+
+    float4v sum[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) sum[u] = float4v{0.0F, 0.0F, 0.0F, 0.0F};
+    if (t0 < t1) {
+        fetch();
+        stage(t0);
+    }
+    __syncthreads();
+    for (int t = t0; t < t1; ++t) {
+        const int b = t % 2;
+        if (t + 1 < t1) fetch();
+        const auto weigh = [&](auto all_seen) {
+#pragma unroll
+            for (int w = 0; w < QT / 16; ++w) {
+                v8 q[KC];
+#pragma unroll
+                for (int c = 0; c < KC; ++c) q[c] = __builtin_bit_cast(v8, q_lds[b][(16 * w + i) * QS + 4 * c + g]);
+                weigh_queries<T, all_seen>(a, base, k, q, refs[b][16 * w + i], limits[b][16 * w + i], sum);
+            }
+        };
+        if (__ballot(limits[b][lane % QT] < base + 16 * U) == 0) weigh(std::true_type{});
+        else weigh(std::false_type{});
+        if (t + 1 < t1) stage(t + 1);
+        __syncthreads();
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            float x = sum[u][r];
+#pragma unroll
+            for (int o = 1; o < 16; o *= 2) x += __shfl_xor(x, o);
+            const int64_t to = __shfl(index[u], 4 * g + r);
+            const int slot = base + 16 * u + 4 * g + r;
+            if (i != 0 || slot >= span.len) continue;
+            if (a.splits > 1) a.partial[(static_cast<int64_t>(split) * a.cache.n_head_kv * a.batch.n_seq + pair) * a.batch.max_length + slot] = x;
+            else if (to >= 0) a.cache.weights[to] += x;
+        }
+    }
+}
+
+__global__ __launch_bounds__(kWeighThreads) void k_weigh_join(Weigh a, int blocks) {
+    const uint32_t pair = blockIdx.x / blocks;
+    const uint32_t h = pair % a.cache.n_head_kv, s = pair / a.cache.n_head_kv;
+    const int slot = static_cast<int>(blockIdx.x % blocks) * kWeighThreads + threadIdx.x;
+    if (slot >= span_length(a.batch, s)) return;
+    const int page = page_of(a.cache, a.batch, s, slot);
+    if (page < 0) return;
+    const int64_t all = static_cast<int64_t>(a.cache.n_head_kv) * a.batch.n_seq;
+    float x = 0.0F;
+    for (uint32_t n = 0; n < a.splits; ++n) x += a.partial[(n * all + pair) * a.batch.max_length + slot];
+    a.cache.weights[slot_index(a.cache, page, h, slot)] += x;
 }
 
 // ---------------------------------------------------------------- cutting a cache
@@ -1308,27 +1445,56 @@ hipError_t launch_attend(const Attend& a, hipStream_t stream) {
 
 namespace {
 
+// How a step's weights are divided: by the most queries that a sequence may have.
+struct WeighTiling {
+    bool few;
+    int blocks;       // work-groups that a sequence's slots take, per K/V head
+    uint64_t groups;  // work-groups per split
+};
+
+WeighTiling weigh_tiling(const Cache& c, const Batch& b, uint32_t group) {
+    WeighTiling t;
+    t.few = static_cast<uint64_t>(b.max_rows) * group <= kFewQueries;
+    const uint32_t slots = kWeighWaves * (t.few ? kFewWeighSlots : 16 * (c.head_dim <= 128 ? kWeighTiles<128> : kWeighTiles<256>));
+    t.blocks = static_cast<int>((b.max_length + slots - 1) / slots);
+    t.groups = static_cast<uint64_t>(t.blocks) * c.n_head_kv * b.n_seq;
+    return t;
+}
+
 template <typename T, int HDP>
-hipError_t weigh_few(const Weigh& a, hipStream_t stream) {
-    constexpr int kSlots = kWeighThreads / 64 * kWeighKeys;
+hipError_t weigh_of(const Weigh& a, hipStream_t stream) {
     const int group = static_cast<int>(a.q.heads / a.cache.n_head_kv);
-    const int blocks = static_cast<int>((a.batch.max_length + kSlots - 1) / kSlots);
-    const uint64_t groups = static_cast<uint64_t>(blocks) * a.cache.n_head_kv * a.batch.n_seq;
+    const WeighTiling t = weigh_tiling(a.cache, a.batch, a.q.heads / a.cache.n_head_kv);
+    const uint64_t groups = t.groups * a.splits;
     if (groups > 0x7FFFFFFF) return hipErrorInvalidConfiguration;
-    return launch(k_weigh<T, HDP>, dim3(static_cast<uint32_t>(groups)), dim3(kWeighThreads), stream, a, group, blocks);
+    return launch(t.few ? k_weigh_few<T, HDP> : k_weigh_many<T, HDP>, dim3(static_cast<uint32_t>(groups)),
+                  dim3(kWeighThreads), stream, a, group, t.blocks);
 }
 
 template <typename T>
 hipError_t weigh(const Weigh& a, hipStream_t stream) {
-    if (a.cache.head_dim <= 64) return weigh_few<T, 64>(a, stream);
-    if (a.cache.head_dim <= 128) return weigh_few<T, 128>(a, stream);
-    return weigh_few<T, 256>(a, stream);
+    if (a.cache.head_dim <= 64) return weigh_of<T, 64>(a, stream);
+    if (a.cache.head_dim <= 128) return weigh_of<T, 128>(a, stream);
+    return weigh_of<T, 256>(a, stream);
 }
 
 }  // namespace
 
+uint32_t weigh_splits(const Cache& c, const Batch& b, uint32_t group) {
+    const WeighTiling t = weigh_tiling(c, b, group);
+    if (t.few || t.groups == 0) return 1;
+    // two work-groups per compute unit, of eight tiles of 32 queries at least
+    const uint64_t wanted = (2 * kComputeUnits + t.groups - 1) / t.groups, most = static_cast<uint64_t>(b.max_rows) * group / 256;
+    return static_cast<uint32_t>(wanted < most ? wanted : most > 0 ? most : 1);
+}
+
 hipError_t launch_weigh(const Weigh& a, hipStream_t stream) {
-    return a.cache.type == kF16 ? weigh<_Float16>(a, stream) : weigh<__bf16>(a, stream);
+    const hipError_t e = a.cache.type == kF16 ? weigh<_Float16>(a, stream) : weigh<__bf16>(a, stream);
+    if (e != hipSuccess || a.splits == 1) return e;
+    const int blocks = static_cast<int>((a.batch.max_length + kWeighThreads - 1) / kWeighThreads);
+    const uint64_t groups = static_cast<uint64_t>(blocks) * a.cache.n_head_kv * a.batch.n_seq;
+    if (groups > 0x7FFFFFFF) return hipErrorInvalidConfiguration;
+    return launch(k_weigh_join, dim3(static_cast<uint32_t>(groups)), dim3(kWeighThreads), stream, a, blocks);
 }
 
 hipError_t launch_evict(const Evict& a, hipStream_t stream) {

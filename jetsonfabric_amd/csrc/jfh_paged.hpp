@@ -120,8 +120,9 @@ struct Weigh {
     Batch batch;
     Rows q;
     const float* lse;
+    float* partial;  // [splits][sequences * K/V heads][max_length]
     float scale_log2;
-    uint32_t causal;
+    uint32_t causal, splits;
 };
 
 struct Evict {
@@ -135,6 +136,9 @@ struct Evict {
 // Parts that a step's keys are divided into, each a work-group of its own per K/V head and tile of query rows; more than
 // one where the tiles do not fill the chip.
 uint32_t attend_splits(const Cache& c, const Batch& b, uint32_t group);
+
+// Parts that a step's queries are divided into when their weights are added up.
+uint32_t weigh_splits(const Cache& c, const Batch& b, uint32_t group);
 
 hipError_t launch_rotate(const Rotation& r, const Rows& x, const int32_t* positions, const Rows& y, hipStream_t stream);
 hipError_t launch_append(const Rotation* r, const Cache& c, const Batch& b, const Rows& k, const Rows& v,

@@ -185,8 +185,12 @@ class PagedCache:
         the cache's weights."""
         a = _rows(q, "q", self.device)
         at = _array(lse, "lse", "torch.float32", self.device, q.shape[:2])
-        check(library().jfh_paged_weigh(self.ref, self._of(batch), ctypes.byref(a), at,
-                                        a.head_dim ** -0.5 if scale is None else scale, int(causal), _stream(self.device)))
+        need = ctypes.c_size_t()
+        check(library().jfh_paged_weigh_workspace(self.ref, self._of(batch), ctypes.byref(a), ctypes.byref(need)))
+        space = self._workspace(need.value)
+        check(library().jfh_paged_weigh(self.ref, batch.ref, ctypes.byref(a), at,
+                                        a.head_dim ** -0.5 if scale is None else scale, int(causal),
+                                        None if space is None else space.data_ptr(), need.value, _stream(self.device)))
 
     def evict(self, batch: PagedBatch, budget: int, n_first: int = 4, n_recent: int = 1) -> None:
         """Cuts every longer sequence to budget slots per K/V head: the positions below n_first, the

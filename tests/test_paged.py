@@ -123,9 +123,9 @@ def test_attention_arguments_are_checked():
     check(_attend(b=batch(n_seq=0)))
 
 
-def _weigh(c=None, b=None, q=None, scale=0.125, lse=AT):
+def _weigh(c=None, b=None, q=None, scale=0.125, lse=AT, space=AT, size=1 << 40):
     return jf.library().jfh_paged_weigh(ctypes.byref(c or cache()), ctypes.byref(b or batch()), ctypes.byref(q or rows()),
-                                        lse, scale, 1, None)
+                                        lse, scale, 1, space, size, None)
 
 
 def _evict(c=None, b=None, budget=8, first=4, recent=2, space=AT, size=1 << 40):
@@ -151,6 +151,14 @@ def test_weigh_arguments_are_checked():
     refused(lambda: _weigh(lse=None), "lse")
     refused(lambda: _weigh(scale=0.0), "score scale")
     refused(lambda: _weigh(q=rows(type=3)), "cache's type")
+    many = {"q": rows(n_rows=4000, n_head=28), "b": batch(n_seq=1, max_rows=4000)}
+    need = ctypes.c_size_t()
+    check(jf.library().jfh_paged_weigh_workspace(ctypes.byref(cache()), ctypes.byref(many["b"]), ctypes.byref(many["q"]),
+                                                 ctypes.byref(need)))
+    assert need.value > 0
+    refused(lambda: _weigh(**many, size=need.value - 1), f"needs {need.value} bytes")
+    refused(lambda: _weigh(**many, space=None), "workspace")
+    refused(lambda: _weigh(**many, space=AT + 8), "16-byte")
     check(_weigh(q=rows(n_rows=0)))
     check(_weigh(b=batch(max_length=0)))
 
