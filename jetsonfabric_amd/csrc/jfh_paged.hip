@@ -1164,11 +1164,14 @@ __global__ __launch_bounds__(kWeighThreads) void k_weigh_join(Weigh a, int block
 // ---------------------------------------------------------------- cutting a cache
 
 // What stays of a K/V head's slots: the `budget` first in the order (protected, heavier, lower slot). One work-group per
-// sequence and K/V head turns the order into 32-bit keys, finds the budget-th largest by its bytes (four counts of 256
-// bins), and lists the slots below the budget that go and those above that stay, both ascending: the latter move into the
-// former, the others stay where they are. Integer counts and scans only, so the lists do not depend on the launch.
+// sequence and K/V head turns the order into 32-bit keys in LDS, finds the budget-th largest by its digits (counts of 2048
+// bins: 11, 11 and 10 bits), and lists the slots below the budget that go and those above that stay, both ascending: the
+// latter move into the former, the others stay where they are. Integer counts and scans only, so the lists do not depend
+// on the launch. Latency bounds it: the passes over weights and positions have BATCH slots per thread in flight, and
+// read caches of up to 8192 slots once.
 constexpr int kSelectThreads = 1024;
-constexpr int kSelectKeys = 32768;  // keys kept in LDS; later slots' are computed again
+constexpr int kSelectBins = 2048;
+constexpr int kSelectFew = 8192, kSelectMany = 36864;  // keys in LDS; later slots' are computed again where they are used
 
 // Order of weights as unsigned integers, 1 for NaN (nothing is lighter), 0 free.
 __device__ __forceinline__ uint32_t weight_key(float w) {
@@ -1177,132 +1180,199 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
     return b >> 31 ? ~b : b | 0x80000000U;
 }
 
+// Inclusive sum over the lanes of a wave: within rows of 16, then from row to row.
+__device__ __forceinline__ int wave_sum_upto(int v) {
+    v += __builtin_amdgcn_update_dpp(0, v, 0x111, 0xF, 0xF, false);  // row_shr 1, 2, 4, 8
+    v += __builtin_amdgcn_update_dpp(0, v, 0x112, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x114, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x118, 0xF, 0xF, false);
+    v += __builtin_amdgcn_update_dpp(0, v, 0x142, 0xA, 0xF, false);  // the last of rows 0 and 2 to rows 1 and 3
+    v += __builtin_amdgcn_update_dpp(0, v, 0x143, 0xC, 0xF, false);  // that of row 1 to rows 2 and 3
+    return v;
+}
+
 // Exclusive sum over the work-group of two counts; `all` gets their totals.
-__device__ __forceinline__ int2 exclusive_sum(int2 v, int2 (*waves), int2* all) {
+__device__ __forceinline__ int2 exclusive_sum(int2 v, int2* waves, int2* all) {
     const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
-    int2 x = v;
-#pragma unroll
-    for (int o = 1; o < 64; o *= 2) {
-        const int a = __shfl_up(x.x, o), b = __shfl_up(x.y, o);
-        if (lane >= o) x.x += a, x.y += b;
-    }
+    const int2 x{wave_sum_upto(v.x), wave_sum_upto(v.y)};
     __syncthreads();
     if (lane == 63) waves[wave] = x;
     __syncthreads();
     int2 before{0, 0}, sum{0, 0};
+#pragma unroll
     for (int w = 0; w < kSelectThreads / 64; ++w) {
+        const int2 y = waves[w];
         if (w == wave) before = sum;
-        sum.x += waves[w].x;
-        sum.y += waves[w].y;
+        sum.x += y.x;
+        sum.y += y.y;
     }
     *all = sum;
     return int2{before.x + x.x - v.x, before.y + x.y - v.y};
 }
 
+template <int CAP, int BATCH>
 __global__ __launch_bounds__(kSelectThreads) void k_evict_select(Evict a) {
-    __shared__ uint32_t keys[kSelectKeys];
-    __shared__ uint32_t bins[256];
+    constexpr bool kStay = CAP <= BATCH * kSelectThreads;  // the first batch, in registers from pass to pass
+    __shared__ uint32_t keys[CAP];
+    __shared__ uint32_t bins[kSelectBins];
     __shared__ int2 waves[kSelectThreads / 64];
     __shared__ uint32_t found[2];
+    const int tid = threadIdx.x;
     const uint32_t h = blockIdx.x % a.cache.n_head_kv, s = blockIdx.x / a.cache.n_head_kv;
     int32_t* list = a.lists + static_cast<int64_t>(blockIdx.x) * (1 + 2 * static_cast<int64_t>(a.width));
     const int len = span_length(a.batch, s), budget = a.budget;
     if (len <= budget) {
-        if (threadIdx.x == 0) list[0] = -1;
+        if (tid == 0) list[0] = -1;
         return;
     }
+    // where the weights and positions of the thread's next slots lie, -1 on absent pages
+    const auto look_up = [&](int t0, int64_t (&at)[BATCH]) {
+        int page[BATCH];
+#pragma unroll
+        for (int e = 0; e < BATCH; ++e) page[e] = page_of(a.cache, a.batch, s, min(t0 + e * kSelectThreads, len - 1));
+#pragma unroll
+        for (int e = 0; e < BATCH; ++e) {
+            const int t = min(t0 + e * kSelectThreads, len - 1);
+            at[e] = page[e] >= 0 ? slot_index(a.cache, page[e], h, t) : -1;
+        }
+    };
 
     // the newest position
     int newest = INT32_MIN;
-    for (int t = threadIdx.x; t < len; t += kSelectThreads) {
-        const int page = page_of(a.cache, a.batch, s, t);
-        if (page >= 0) newest = max(newest, a.cache.positions[slot_index(a.cache, page, h, t)]);
+    int64_t first_at[kStay ? BATCH : 1];
+    int first_p[kStay ? BATCH : 1];
+    float first_w[kStay ? BATCH : 1];
+    for (int t0 = tid; t0 < len; t0 += BATCH * kSelectThreads) {
+        int64_t at[BATCH];
+        look_up(t0, at);
+        int p[BATCH];
+#pragma unroll
+        for (int e = 0; e < BATCH; ++e) p[e] = a.cache.positions[max(at[e], static_cast<int64_t>(0))];
+        if constexpr (kStay) {
+            if (t0 == tid) {
+#pragma unroll
+                for (int e = 0; e < BATCH; ++e) {
+                    first_at[e] = at[e];
+                    first_p[e] = p[e];
+                    first_w[e] = a.cache.weights[max(at[e], static_cast<int64_t>(0))];
+                }
+            }
+        }
+#pragma unroll
+        for (int e = 0; e < BATCH; ++e) newest = max(newest, at[e] >= 0 ? p[e] : INT32_MIN);
     }
 #pragma unroll
     for (int o = 32; o; o /= 2) newest = max(newest, __shfl_xor(newest, o));
-    if (threadIdx.x % 64 == 0) waves[threadIdx.x / 64].x = newest;
+    if (tid % 64 == 0) waves[tid / 64].x = newest;
     __syncthreads();
+#pragma unroll
     for (int w = 0; w < kSelectThreads / 64; ++w) newest = max(newest, waves[w].x);
-
-    // protected slots; an absent page's slots below the budget count among them, as nothing can take their place
     const int64_t recent = static_cast<int64_t>(newest) - a.recent;
-    int held = 0;
-    const auto safe = [&](int page, int t) {
-        if (page < 0) return t < budget;
-        const int p = a.cache.positions[slot_index(a.cache, page, h, t)];
-        return p < a.first || p > recent;
-    };
-    for (int t = threadIdx.x; t < len; t += kSelectThreads) held += safe(page_of(a.cache, a.batch, s, t), t);
-    int2 all;
-    exclusive_sum(int2{held, 0}, waves, &all);
-    const bool crowded = all.x >= budget;  // some of the protected go too, and nothing else stays
 
-    const auto key_of = [&](int t) {
-        const int page = page_of(a.cache, a.batch, s, t);
-        const bool keep = safe(page, t);
-        if (page < 0 || (keep && !crowded)) return keep ? 0xFFFFFFFFU : 0U;
-        return crowded && !keep ? 0U : weight_key(a.cache.weights[slot_index(a.cache, page, h, t)]);
+    // Protected slots have the largest key, and so have an absent page's slots below the budget, whose place nothing can
+    // take; its others have 0. Where that is more than the budget (`crowded`), protected slots are in the order of their
+    // weights and the others at 0.
+    const auto key_of = [&](int t, int64_t at, int p, float w, bool crowded, bool& keep) {
+        keep = at < 0 ? t < budget : p < a.first || p > recent;
+        if (at < 0 || (keep && !crowded)) return keep ? 0xFFFFFFFFU : 0U;
+        return crowded && !keep ? 0U : weight_key(w);
     };
-    for (int t = threadIdx.x; t < min(len, kSelectKeys); t += kSelectThreads) keys[t] = key_of(t);
-    const auto key_at = [&](int t) { return t < kSelectKeys ? keys[t] : key_of(t); };
+    const auto fill = [&](bool crowded) {
+        int held = 0;
+        for (int t0 = tid; t0 < len; t0 += BATCH * kSelectThreads) {
+            int64_t at[BATCH];
+            int p[BATCH];
+            float w[BATCH];
+            if (kStay && t0 == tid) {
+#pragma unroll
+                for (int e = 0; e < BATCH; ++e) at[e] = first_at[e % (kStay ? BATCH : 1)], p[e] = first_p[e % (kStay ? BATCH : 1)], w[e] = first_w[e % (kStay ? BATCH : 1)];
+            } else {
+                look_up(t0, at);
+#pragma unroll
+                for (int e = 0; e < BATCH; ++e) {
+                    p[e] = a.cache.positions[max(at[e], static_cast<int64_t>(0))];
+                    w[e] = a.cache.weights[max(at[e], static_cast<int64_t>(0))];
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < BATCH; ++e) {
+                const int t = t0 + e * kSelectThreads;
+                if (t >= len) continue;
+                bool keep;
+                const uint32_t k = key_of(t, at[e], p[e], w[e], crowded, keep);
+                held += keep;
+                if (t < CAP) keys[t] = k;
+            }
+        }
+        return held;
+    };
+    int2 all;
+    exclusive_sum(int2{fill(false), 0}, waves, &all);
+    const bool crowded = all.x >= budget;
+    if (crowded) fill(true);
+    const auto key_at = [&](int t) {
+        if (t < CAP) return keys[t];
+        const int page = page_of(a.cache, a.batch, s, t);
+        const int64_t at = page >= 0 ? slot_index(a.cache, page, h, t) : -1;
+        bool keep;
+        return key_of(t, at, at < 0 ? 0 : a.cache.positions[at], at < 0 ? 0.0F : a.cache.weights[at], crowded, keep);
+    };
 
     uint32_t prefix = 0, mask = 0;
     int need = budget;
-    for (int shift = 24; shift >= 0; shift -= 8) {
+    for (int shift = 21; shift >= 0; shift -= shift == 21 ? 11 : 10) {  // 21, 10, 0
+        const uint32_t digit = shift ? 2047U : 1023U;
+        for (int e = tid; e < kSelectBins; e += kSelectThreads) bins[e] = 0;
         __syncthreads();
-        if (threadIdx.x < 256) bins[threadIdx.x] = 0;
-        __syncthreads();
-        for (int t = threadIdx.x; t < len; t += kSelectThreads) {
+#pragma unroll 4
+        for (int t = tid; t < len; t += kSelectThreads) {
             const uint32_t k = key_at(t);
-            if ((k & mask) == prefix) atomicAdd(&bins[k >> shift & 255U], 1U);
+            if ((k & mask) == prefix) atomicAdd(&bins[k >> shift & digit], 1U);
         }
         __syncthreads();
-        if (threadIdx.x < 64) {  // lane l has bins 255 - 4 l downwards
-            int own[4], sum = 0;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) sum += own[e] = static_cast<int>(bins[255 - 4 * threadIdx.x - e]);
-            int upto = sum;
-#pragma unroll
-            for (int o = 1; o < 64; o *= 2) {
-                const int v = __shfl_up(upto, o);
-                if (static_cast<int>(threadIdx.x) >= o) upto += v;
-            }
-            int above = upto - sum;
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                if (above < need && above + own[e] >= need) found[0] = 255 - 4 * threadIdx.x - e, found[1] = above;
-                above += own[e];
-            }
+        // thread l has bins 2047 - 2 l and 2046 - 2 l: those of larger keys come first
+        const int hi = static_cast<int>(bins[kSelectBins - 1 - 2 * tid]), lo = static_cast<int>(bins[kSelectBins - 2 - 2 * tid]);
+        const int above = exclusive_sum(int2{hi + lo, 0}, waves, &all).x;
+        if (above < need && above + hi + lo >= need) {
+            const bool upper = above + hi >= need;
+            found[0] = kSelectBins - (upper ? 1 : 2) - 2 * tid;
+            found[1] = upper ? above : above + hi;
         }
         __syncthreads();
         prefix |= found[0] << shift;
-        mask |= 255U << shift;
+        mask |= digit << shift;
         need -= static_cast<int>(found[1]);
     }
 
-    // `need` of the slots with key `prefix` stay, the lowest; a thread owns a run of slots (odd, for the LDS banks)
-    const int run = ((len + kSelectThreads - 1) / kSelectThreads) | 1;
-    const int t0 = min(static_cast<int>(threadIdx.x) * run, len), t1 = min(t0 + run, len);
-    int equal = 0;
-    for (int t = t0; t < t1; ++t) equal += key_at(t) == prefix;
-    const int before = exclusive_sum(int2{equal, 0}, waves, &all).x;
+    // `need` of the slots with key `prefix` stay, the lowest. A thread owns a run of slots (an odd number, for the LDS
+    // banks) as bits of two words; sequences beyond 63 slots per thread take several rounds.
+    int equals = 0;      // of earlier rounds
     int2 moves{0, 0};
-    int rank = before;
-    for (int t = t0; t < t1; ++t) {
-        const uint32_t k = key_at(t);
-        const bool stays = k > prefix || (k == prefix && rank++ < need);
-        moves.x += t < budget && !stays;
-        moves.y += t >= budget && stays;
+    for (int round = 0; round < len; round += 63 * kSelectThreads) {
+        const int upto = min(len - round, 63 * kSelectThreads);
+        const int run = ((upto + kSelectThreads - 1) / kSelectThreads) | 1;
+        const int t0 = round + min(tid * run, upto), count = min(run, round + upto - t0);
+        unsigned long long larger = 0, equal = 0;
+#pragma unroll 8
+        for (int e = 0; e < count; ++e) {
+            const uint32_t k = key_at(t0 + e);
+            larger |= static_cast<unsigned long long>(k > prefix) << e;
+            equal |= static_cast<unsigned long long>(k == prefix) << e;
+        }
+        int room = need - equals - exclusive_sum(int2{__popcll(equal), 0}, waves, &all).x;
+        equals += all.x;
+        unsigned long long stays = larger;
+        for (unsigned long long left = equal; left && room > 0; left &= left - 1, --room) stays |= left & -left;
+        const int below = clamped(budget - t0, 0, count);  // of the run
+        const unsigned long long inside = (1ULL << below) - 1, owned = (1ULL << count) - 1;
+        unsigned long long goes = ~stays & inside, comes = stays & owned & ~inside;
+        const int2 before = exclusive_sum(int2{__popcll(goes), __popcll(comes)}, waves, &all);
+        for (int n = moves.x + before.x; goes; goes &= goes - 1) list[1 + n++] = t0 + __ffsll(goes) - 1;
+        for (int n = moves.y + before.y; comes; comes &= comes - 1) list[1 + a.width + n++] = t0 + __ffsll(comes) - 1;
+        moves.x += all.x;
+        moves.y += all.y;
     }
-    int2 to = exclusive_sum(moves, waves, &all);
-    if (threadIdx.x == 0) list[0] = all.x;
-    rank = before;
-    for (int t = t0; t < t1; ++t) {
-        const uint32_t k = key_at(t);
-        const bool stays = k > prefix || (k == prefix && rank++ < need);
-        if (t < budget && !stays) list[1 + to.x++] = t;
-        if (t >= budget && stays) list[1 + a.width + to.y++] = t;
-    }
+    if (tid == 0) list[0] = moves.x;
 }
 
 // 16 threads per moving position: its K and V rows, its weight and its position.
@@ -1501,7 +1571,8 @@ hipError_t launch_evict(const Evict& a, hipStream_t stream) {
     const uint64_t pairs = static_cast<uint64_t>(a.cache.n_head_kv) * a.batch.n_seq;
     const int chunks = (a.width + kMoveSlots - 1) / kMoveSlots;
     if (pairs * static_cast<uint64_t>(chunks) > 0x7FFFFFFF) return hipErrorInvalidConfiguration;
-    const hipError_t e = launch(k_evict_select, dim3(static_cast<uint32_t>(pairs)), dim3(kSelectThreads), stream, a);
+    // the larger LDS takes a compute unit for one work-group
+    const hipError_t e = launch(a.batch.max_length <= kSelectFew ? k_evict_select<kSelectFew, 8> : k_evict_select<kSelectMany, 16>, dim3(static_cast<uint32_t>(pairs)), dim3(kSelectThreads), stream, a);
     if (e != hipSuccess) return e;
     return launch(k_evict_move, dim3(static_cast<uint32_t>(pairs) * chunks), dim3(kMoveThreads), stream, a, chunks);
 }

@@ -382,6 +382,7 @@ CUTS = [
     ([600], 2, 64, 16, 200, 4, 16, {"absent": [(0, 2), (0, 20), (0, 30)]}),
     ([90], 1, 64, 16, 30, 4, 16, {"absent": [(0, 0), (0, 1)]}),
     ([40000, 33000], 1, 8, 256, 20000, 16, 1000, {}),  # beyond the keys held in LDS
+    ([70000], 1, 8, 1024, 66000, 16, 1000, {}),        # more than one round of the lists
     ([2500], 1, 16, 2, 2499, 0, 1, {}),
     ([5, 1, 0], 2, 32, 4, 3, 1, 1, {}),
 ]
