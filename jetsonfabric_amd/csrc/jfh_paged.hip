@@ -264,50 +264,23 @@ __device__ __forceinline__ bool nonfinite(uint32_t two) {
     return (two & e) == e || (two & (e << 16)) == (e << 16);
 }
 
-// sum + v p where v may hold infinities and NaN in rows that some columns of p do not see: a weight of 0 must leave them
-// out. Their share comes from products of their marks with `seen` (1 where a column sees the row), which count them.
-template <typename T, typename Acc>
-__device__ __forceinline__ Acc weighted_nonfinite(typename Values<T>::v8 v, typename Values<T>::v8 p,
-                                                  typename Values<T>::v8 seen, Acc sum) {
-    typename Values<T>::v8 rest, mark[3];
-#pragma unroll
-    for (int i = 0; i < 8; ++i) {
-        const float x = static_cast<float>(v[i]);
-        rest[i] = fabsf(x) < INFINITY ? v[i] : static_cast<T>(0.0F);
-        mark[0][i] = static_cast<T>(x == INFINITY ? 1.0F : 0.0F);
-        mark[1][i] = static_cast<T>(x == -INFINITY ? 1.0F : 0.0F);
-        mark[2][i] = static_cast<T>(x != x ? 1.0F : 0.0F);
-    }
-    constexpr int kSums = sizeof(Acc) / sizeof(float);
-    constexpr float kAdds[3] = {INFINITY, -INFINITY, NAN};
-    sum = Values<T>::mfma(rest, p, sum);
-#pragma unroll
-    for (int n = 0; n < 3; ++n) {
-        Acc count;
-#pragma unroll
-        for (int r = 0; r < kSums; ++r) count[r] = 0.0F;
-        count = Values<T>::mfma(mark[n], seen, count);
-#pragma unroll
-        for (int r = 0; r < kSums; ++r) {
-            if (count[r] > 0.0F) sum[r] += kAdds[n];
-        }
-    }
-    return sum;
+// Takes an infinity or NaN out of a half of two 16-bit values: 0 in its place, bit j in mark (+inf, -inf, NaN).
+template <typename T>
+__device__ __forceinline__ void take_nonfinite(uint32_t& two, int half, int j, uint32_t (&mark)[3]) {
+    constexpr uint32_t exponent = Values<T>::kExponent, mantissa = 0x7FFFU & ~exponent;
+    const uint32_t x = two >> (16 * half) & 0xFFFFU;
+    const bool odd = (x & exponent) == exponent, nan = odd && (x & mantissa) != 0;
+    mark[0] |= static_cast<uint32_t>(odd && !nan && !(x >> 15)) << j;
+    mark[1] |= static_cast<uint32_t>(odd && !nan && (x >> 15)) << j;
+    mark[2] |= static_cast<uint32_t>(nan) << j;
+    if (odd) two &= half ? 0x0000FFFFU : 0xFFFF0000U;
 }
 
-// Takes the infinities and NaN out of column e of eight rows of four 16-bit values: 0 in their place, their rows' bits in
-// mark (+inf, -inf, NaN).
-template <typename T>
-__device__ __forceinline__ void take_nonfinite(uint2 (&v)[8], int e, uint8_t (&mark)[3]) {
-    constexpr uint32_t exponent = Values<T>::kExponent, mantissa = 0x7FFFU & ~exponent;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-        uint32_t& two = e < 2 ? v[j].x : v[j].y;
-        const uint32_t x = two >> (16 * (e % 2)) & 0xFFFFU;
-        if ((x & exponent) != exponent) continue;
-        mark[x & mantissa ? 2 : x >> 15] |= static_cast<uint8_t>(1U << j);
-        two &= ~(0xFFFFU << (16 * (e % 2)));
-    }
+// A sum to which visible infinities and NaN belong (any positive weight of theirs gives the same).
+__device__ __forceinline__ float with_nonfinite(float sum, bool pos, bool neg, bool nan) {
+    if (pos) sum += INFINITY;
+    if (neg) sum -= INFINITY;
+    return nan ? NAN : sum;
 }
 
 // Column c of eight rows of 16-bit values, two to a word.
@@ -346,17 +319,22 @@ __device__ __forceinline__ Query query_of(int m, int group, uint32_t kv_head) {
     return Query{row, static_cast<int>(kv_head) * group + (m - row * group)};
 }
 
-// Few query rows: o = softmax(scale q K^T) V for up to 16 MT queries of a K/V head, 4 waves that divide its keys.
+// Few query rows: o = softmax(scale q K^T) V for up to 16 MT QG queries of a K/V head. Its 8 waves (4 of wide heads) divide
+// the keys; with QG = 2 those of either half have half of the queries, as one wave's registers hold 32.
 //
-// The bytes of K and V bound it. A wave takes tiles of 32 keys from global memory to registers, in the layout of the
-// rows: S^T = K Q^T on 16x16x32 products has a K row's 16 bytes per lane as its A operand. O^T += V^T P^T wants 8 keys of
-// one column per lane; lane (i, g) loads rows 16 u + 4 g + r (u = 0, 1, r = 0..3), columns VEC i .. VEC i + VEC - 1, and
-// 16-bit permutes of those rows give the operands of VEC products, the c-th of columns VEC i + c. The keys of lane group g
-// are those whose scores the group holds after S^T, so P needs no exchange between lanes. No LDS on the way.
+// The bytes of K and V bound it where there are enough of them, and their latency elsewhere. A wave takes tiles of 32 keys
+// from global memory to registers, in the layout of the rows: S^T = K Q^T on 16x16x32 products has a K row's 16 bytes per
+// lane as its A operand. O^T += V^T P^T wants 8 keys of one column per lane; lane (i, g) loads rows 16 u + 4 g + r (u = 0,
+// 1, r = 0..3), columns VEC i .. VEC i + VEC - 1, and 16-bit permutes of those rows give the operands of VEC products, the
+// c-th of columns VEC i + c. The keys of lane group g are those whose scores the group holds after S^T, so P needs no
+// exchange between lanes. No LDS on the way: the next tile's K is requested as soon as the scores are there, its V after
+// the product with P, and the pages of the one after it are looked up meanwhile.
 // Running maximum and sum are f32, base 2; P is rounded to the cache's type for the product (half a step per weight, as
 // the output), its sum is not. A row's maximum is raised only when a tile exceeds it by 2^8: P stays far below 65504.
-template <typename T, int HDP, int MT>
-__global__ __launch_bounds__(kAttendThreads, HDP * MT <= 128 ? 2 : 1) void k_attend_few(Attend a, int group) {
+template <int HDP> constexpr int kFewWaves = HDP <= 128 ? 8 : 4;
+
+template <typename T, int HDP, int MT, int QG>
+__global__ __launch_bounds__(64 * kFewWaves<HDP>) void k_attend_few(Attend a, int group) {
     using V = Values<T>;
     using v8 = typename V::v8;
     constexpr int VEC = HDP / 16;   // columns per lane of V
@@ -364,26 +342,88 @@ __global__ __launch_bounds__(kAttendThreads, HDP * MT <= 128 ? 2 : 1) void k_att
     constexpr int VW = VEC / 2;     // words per lane and V row
     constexpr int kChunk = VW < 4 ? VW : 4;  // words of one load
     constexpr int OS = HDP + 4;     // floats per query of the waves' sums in LDS
-    __shared__ float part_o[kAttendWaves][16][OS];
-    __shared__ float part_m[kAttendWaves][16], part_l[kAttendWaves][16];
-    __shared__ uint4 q_lds[MT][KC][64];
+    constexpr int kWaves = kFewWaves<HDP>, kThreads = 64 * kWaves, KW = kWaves / QG;  // waves that divide the keys
+    __shared__ float part_o[kWaves][16][OS];
+    __shared__ float part_m[kWaves][16], part_l[kWaves][16];
+    __shared__ uint4 q_lds[QG * MT][KC][64];
 
-    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
+    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, half = wave / KW;
     const int i = lane % 16, g = lane / 16;
     const uint32_t pairs = a.cache.n_head_kv * a.batch.n_seq;  // K/V heads of sequences
     const uint32_t split = blockIdx.x % a.splits, pair = blockIdx.x / a.splits % pairs;
     const uint32_t h = pair % a.cache.n_head_kv, s = pair / a.cache.n_head_kv;
-    const int m0 = static_cast<int>(blockIdx.x / a.splits / pairs) * 16 * MT;
+    const int group_m0 = static_cast<int>(blockIdx.x / a.splits / pairs) * 16 * MT * QG, m0 = group_m0 + 16 * MT * half;
     const Span span = sequence_span(a.batch, a.q.rows, s);
     const int queries = span.rows * group;
-    if (m0 >= queries) return;
+    if (group_m0 >= queries) return;
     const int dim = static_cast<int>(a.cache.head_dim);
     const int first = span.len - span.rows;  // slot of row 0
+    const auto sees = [&](int m) { return a.causal ? max(0, first + m / group + 1) : span.len; };  // slots of query m
+    // seen by all queries of the wave, by any
+    const int least = sees(min(m0, queries - 1)), end = m0 < queries ? sees(min(queries, m0 + 16 * MT) - 1) : 0;
+
+    // the split's tiles: equal parts of the sequence's
+    const int tiles = (span.len + kFewKeys - 1) / kFewKeys;
+    const int per = (tiles + static_cast<int>(a.splits) - 1) / static_cast<int>(a.splits);
+    const int t0 = static_cast<int>(split) * per, t1 = min(min(tiles, t0 + per), (end + kFewKeys - 1) / kFewKeys);
+
+    const T* k_head = static_cast<const T*>(a.cache.k) + h * a.cache.head_stride;
+    const T* v_head = static_cast<const T*>(a.cache.v) + h * a.cache.head_stride;
+
+    // Offsets of the lane's K rows of a tile and a bit per key that is there: in use, and on a page.
+    struct Keys {
+        int64_t at[2];
+        uint32_t present;  // bit 16 u + e: key 16 u + e
+    };
+    const auto look_up = [&](int t) {
+        Keys x;
+        x.present = 0;
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+            const int slot = t * kFewKeys + 16 * u + i;
+            const int page = slot < end ? page_of(a.cache, a.batch, s, slot) : -1;
+            x.at[u] = page >= 0 ? slot_offset(a.cache, page, slot) : 0;  // of a row that is not there: any that is
+            x.present |= (static_cast<uint32_t>(__ballot(page >= 0)) & 0xFFFFU) << (16 * u);
+        }
+        return x;
+    };
+    v8 k[2][KC];
+    uint32_t v[8][VW];
+    const auto fetch_k = [&](const Keys& x) {
+#pragma unroll
+        for (int u = 0; u < 2; ++u) {
+#pragma unroll
+            for (int c = 0; c < KC; ++c) {
+                const int d = 32 * c + 8 * g;
+                k[u][c] = *reinterpret_cast<const v8*>(k_head + x.at[u] + (d < dim ? d : 0));
+            }
+        }
+    };
+    const auto fetch_v = [&](const Keys& x) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            const T* row = v_head + __shfl(x.at[j / 4], 4 * g + j % 4);
+#pragma unroll
+            for (int w = 0; w < VW; w += kChunk) {
+                const int d = VEC * i + 2 * w;
+                __builtin_memcpy(&v[j][w], __builtin_assume_aligned(row + (d < dim ? d : 0), 4 * kChunk), 4 * kChunk);
+            }
+        }
+    };
+
+    int t = t0 + wave % KW;
+    Keys now{}, next{};
+    if (t < t1) {
+        now = look_up(t);
+        fetch_k(now);
+        fetch_v(now);
+        if (t + KW < t1) next = look_up(t + KW);
+    }
 
     // queries to LDS in operand order, zeros behind the last one and beyond head_dim
-    for (int t = threadIdx.x; t < MT * KC * 64; t += kAttendThreads) {
-        const int l = t % 64, c = t / 64 % KC, mt = t / 64 / KC;
-        const int m = m0 + 16 * mt + l % 16, d = 32 * c + 8 * (l / 16);
+    for (int e = threadIdx.x; e < QG * MT * KC * 64; e += kThreads) {
+        const int l = e % 64, c = e / 64 % KC, mt = e / 64 / KC;
+        const int m = group_m0 + 16 * mt + l % 16, d = 32 * c + 8 * (l / 16);
         uint4 x{0, 0, 0, 0};
         if (m < queries && d < dim) {
             const Query q = query_of(m, group, h);
@@ -394,22 +434,9 @@ __global__ __launch_bounds__(kAttendThreads, HDP * MT <= 128 ? 2 : 1) void k_att
     }
     __syncthreads();
 
-    int limit[MT];  // slots that the lane's query sees: 0 .. limit - 1
-    int least = span.len;
+    int limit[MT];
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-        const int m = m0 + 16 * mt + i;
-        limit[mt] = m < queries && a.causal ? max(0, first + m / group + 1) : span.len;
-    }
-    if (a.causal) least = max(0, first + m0 / group + 1);
-    const int last = min(queries, m0 + 16 * MT) - 1;
-    const int end = a.causal ? max(0, first + last / group + 1) : span.len;  // slots that any query here sees
-
-    // the split's tiles: equal parts of the sequence's
-    const int tiles = (span.len + kFewKeys - 1) / kFewKeys;
-    const int per = (tiles + static_cast<int>(a.splits) - 1) / static_cast<int>(a.splits);
-    const int t0 = static_cast<int>(split) * per, t1 = min(min(tiles, t0 + per), (end + kFewKeys - 1) / kFewKeys);
-
+    for (int mt = 0; mt < MT; ++mt) limit[mt] = sees(min(m0 + 16 * mt + i, queries - 1));
     float4v o[MT][VEC];
     float top[MT], sum[MT];
 #pragma unroll
@@ -420,50 +447,83 @@ __global__ __launch_bounds__(kAttendThreads, HDP * MT <= 128 ? 2 : 1) void k_att
         for (int c = 0; c < VEC; ++c) o[mt][c] = float4v{0.0F, 0.0F, 0.0F, 0.0F};
     }
 
-    const T* k_head = static_cast<const T*>(a.cache.k) + h * a.cache.head_stride;
-    const T* v_head = static_cast<const T*>(a.cache.v) + h * a.cache.head_stride;
-
-    for (int t = t0 + wave; t < t1; t += kAttendWaves) {
+    for (; t < t1; t += KW) {
         const int base = t * kFewKeys;
-        // offsets of the lane's K rows; -1: not in use, or on an absent page
-        int64_t at[2];
-        uint32_t present[2];
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const int slot = base + 16 * u + i;
-            at[u] = -1;
-            if (slot < end) {
-                const int page = page_of(a.cache, a.batch, s, slot);
-                if (page >= 0) at[u] = slot_offset(a.cache, page, slot);
-            }
-            present[u] = static_cast<uint32_t>(__ballot(at[u] >= 0)) & 0xFFFFU;
-        }
-        const bool all_present = (present[0] & present[1]) == 0xFFFFU;
+        const bool whole = now.present == 0xFFFFFFFFU;
         const bool hidden = base + kFewKeys > least;  // some query here does not see some of the tile
-        uint4 k[2][KC];
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-            const T* row = k_head + max(at[u], static_cast<int64_t>(0));
+        if (dim < HDP) {  // beyond head_dim Q is 0, and what it meets must be a number
 #pragma unroll
             for (int c = 0; c < KC; ++c) {
-                const int d = 32 * c + 8 * g;
-                k[u][c] = *reinterpret_cast<const uint4*>(row + (d < dim ? d : 0));
-                if (d >= dim) k[u][c] = uint4{0, 0, 0, 0};
+                if (32 * c + 8 * g >= dim) k[0][c] = k[1][c] = __builtin_bit_cast(v8, uint4{0, 0, 0, 0});
             }
         }
-        uint32_t v[8][VW];
+        float4v sc[MT][2];
 #pragma unroll
-        for (int j = 0; j < 8; ++j) {
-            const int64_t row = __shfl(at[j / 4], 4 * g + j % 4);
+        for (int mt = 0; mt < MT; ++mt) sc[mt][0] = sc[mt][1] = float4v{0.0F, 0.0F, 0.0F, 0.0F};
 #pragma unroll
-            for (int w = 0; w < VW; w += kChunk) {
-                const int d = VEC * i + 2 * w;
-                const T* from = v_head + max(row, static_cast<int64_t>(0)) + (d < dim ? d : 0);
-                __builtin_memcpy(&v[j][w], __builtin_assume_aligned(from, 4 * kChunk), 4 * kChunk);
-                // what is not there must be a number: its weight is 0
-                if (row < 0 || d >= dim) {
+        for (int c = 0; c < KC; ++c) {
 #pragma unroll
-                    for (int e = 0; e < kChunk; ++e) v[j][w + e] = 0;
+            for (int mt = 0; mt < MT; ++mt) {
+                const v8 q = __builtin_bit_cast(v8, q_lds[half * MT + mt][c][lane]);
+                sc[mt][0] = V::mfma(k[0][c], q, sc[mt][0]);
+                sc[mt][1] = V::mfma(k[1][c], q, sc[mt][1]);
+            }
+        }
+        if (t + KW < t1) fetch_k(next);
+
+        // scores of keys base + 16 u + 4 g + r, query i
+        uint32_t seen[MT];
+        if (!whole || hidden) {
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+                seen[mt] = 0;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int e = 16 * (j / 4) + 4 * g + j % 4;
+                    const bool see = (now.present >> e & 1U) && base + e < limit[mt];
+                    seen[mt] |= static_cast<uint32_t>(see) << j;
+                    if (!see) sc[mt][j / 4][j % 4] = -INFINITY;
+                }
+            }
+        }
+        float most[MT];
+        bool rise = false;
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+            most[mt] = sc[mt][0][0];
+#pragma unroll
+            for (int j = 1; j < 8; ++j) most[mt] = fmaxf(most[mt], sc[mt][j / 4][j % 4]);
+            most[mt] = groups_max(most[mt]) * a.scale_log2;
+            rise |= most[mt] > top[mt] + kRescale;
+        }
+        if (__ballot(rise)) {
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+                const float to = fmaxf(top[mt], most[mt]);
+                const float shrink = to == -INFINITY ? 1.0F : exp2f(top[mt] - to);
+                top[mt] = to;
+                sum[mt] *= shrink;
+#pragma unroll
+                for (int c = 0; c < VEC; ++c) o[mt][c] *= shrink;
+            }
+        }
+        v8 p[MT];
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+            const float ref = top[mt] == -INFINITY ? 0.0F : top[mt];
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float w = __builtin_amdgcn_exp2f(fmaf(sc[mt][j / 4][j % 4], a.scale_log2, -ref));
+                sum[mt] += w;
+                p[mt][j] = static_cast<T>(w);
+            }
+        }
+        if (!whole || dim < HDP) {  // what is not there must be a number: its weight is 0
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+#pragma unroll
+                for (int w = 0; w < VW; ++w) {
+                    if (!(now.present >> (16 * (j / 4) + 4 * g + j % 4) & 1U) || VEC * i + 2 * w >= dim) v[j][w] = 0;
                 }
             }
         }
@@ -475,128 +535,103 @@ __global__ __launch_bounds__(kAttendThreads, HDP * MT <= 128 ? 2 : 1) void k_att
                 for (int w = 0; w < VW; ++w) odd |= nonfinite<T>(v[j][w]);
             }
         }
-        const bool careful = __ballot(odd) != 0;
-
+        // rare: marks of the infinities and NaN of V, taken out for the product, go to LDS by column, a byte per lane group
+        uint32_t* marks = reinterpret_cast<uint32_t*>(part_o[wave]);  // [3][HDP], the wave's own until the loop ends
+        const bool any_odd = __ballot(odd) != 0;
+        if (any_odd) {
 #pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-            float4v sc[2] = {float4v{0.0F, 0.0F, 0.0F, 0.0F}, float4v{0.0F, 0.0F, 0.0F, 0.0F}};
+            for (int c = 0; c < VEC; ++c) {
+                uint32_t mark[3] = {0, 0, 0};
 #pragma unroll
-            for (int c = 0; c < KC; ++c) {
-                const v8 q = __builtin_bit_cast(v8, q_lds[mt][c][lane]);
+                for (int j = 0; j < 8; ++j) take_nonfinite<T>(v[j][c / 2], c % 2, j, mark);
 #pragma unroll
-                for (int u = 0; u < 2; ++u) sc[u] = V::mfma(__builtin_bit_cast(v8, k[u][c]), q, sc[u]);
+                for (int n = 0; n < 3; ++n) reinterpret_cast<uint8_t*>(marks + n * HDP + VEC * i + c)[g] = static_cast<uint8_t>(mark[n]);
             }
-            // scores of keys base + 16 u + 4 g + r, query i
-            uint32_t seen = 0xFF;
-            if (!all_present || hidden) {
-                seen = 0;
+        }
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const int u = j / 4, e = 4 * g + j % 4;
-                    const bool sees = (present[u] >> e & 1U) && base + 16 * u + e < limit[mt];
-                    seen |= static_cast<uint32_t>(sees) << j;
-                    if (!sees) sc[u][j % 4] = -INFINITY;
-                }
-            }
-            float most = sc[0][0];
+        for (int c = 0; c < VEC; ++c) {
+            const v8 x = __builtin_bit_cast(v8, column<VW>(v, c));
 #pragma unroll
-            for (int j = 1; j < 8; ++j) most = fmaxf(most, sc[j / 4][j % 4]);
-            most = groups_max(most) * a.scale_log2;
-            if (__ballot(most > top[mt] + kRescale)) {
-                const float now = fmaxf(top[mt], most);
-                const float shrink = now == -INFINITY ? 1.0F : exp2f(top[mt] - now);
-                top[mt] = now;
-                sum[mt] *= shrink;
+            for (int mt = 0; mt < MT; ++mt) o[mt][c] = V::mfma(x, p[mt], o[mt][c]);
+        }
+        if (any_odd) {
+            asm volatile("" ::: "memory");
 #pragma unroll
-                for (int c = 0; c < VEC; ++c) o[mt][c] *= shrink;
-            }
-            const float ref = top[mt] == -INFINITY ? 0.0F : top[mt];
-            v8 p;
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float w = __builtin_amdgcn_exp2f(fmaf(sc[j / 4][j % 4], a.scale_log2, -ref));
-                sum[mt] += w;
-                p[j] = static_cast<T>(w);
-            }
-            if (!careful) {
+            for (int mt = 0; mt < MT; ++mt) {
+                // the query's keys: bit 8 g + j
+                uint32_t see = seen[mt] << (8 * g);
+                see |= __shfl_xor(see, 16);
+                see |= __shfl_xor(see, 32);
 #pragma unroll
                 for (int c = 0; c < VEC; ++c) {
-                    o[mt][c] = V::mfma(__builtin_bit_cast(v8, column<VW>(v, c)), p, o[mt][c]);
-                }
-            } else {
-                v8 seen_mark;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) seen_mark[j] = static_cast<T>(seen >> j & 1U ? 1.0F : 0.0F);
-#pragma unroll
-                for (int c = 0; c < VEC; ++c) {
-                    o[mt][c] = weighted_nonfinite<T>(__builtin_bit_cast(v8, column<VW>(v, c)), p, seen_mark, o[mt][c]);
+                    for (int r = 0; r < 4; ++r) {
+                        const int d = VEC * (4 * g + r) + c;
+                        o[mt][c][r] = with_nonfinite(o[mt][c][r], marks[d] & see, marks[HDP + d] & see, marks[2 * HDP + d] & see);
+                        asm volatile("" ::: "memory");  // one column's marks at a time: the sums leave few registers
+                    }
                 }
             }
+        }
+        if (t + KW < t1) {
+            fetch_v(next);
+            now = next;
+            if (t + 2 * KW < t1) next = look_up(t + 2 * KW);
         }
     }
 
     // the waves' sums, 16 queries at a time
-    const int rows_heads = static_cast<int>(a.q.rows * a.q.heads);
+    const int64_t all = static_cast<int64_t>(a.q.rows) * a.q.heads;
+    const bool complete = a.splits == 1;
+#pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
-        if (m0 + 16 * mt >= queries) break;
+        if (group_m0 + 16 * mt >= queries) break;
         __syncthreads();
+        const float wave_l = groups_sum(sum[mt]);
+        if (g == 0) part_m[wave][i] = top[mt], part_l[wave][i] = wave_l;
+        // lane (i, g) holds columns VEC (4 g + r) + c of query i
 #pragma unroll
-        for (int n = 0; n < MT; ++n) {
-            if (n != mt) continue;
-            const float l = groups_sum(sum[n]);
-            if (g == 0) part_m[wave][i] = top[n], part_l[wave][i] = l;
-            // lane (i, g) holds columns VEC (4 g + r) + c of query i
+        for (int r = 0; r < 4; ++r) {
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-#pragma unroll
-                for (int c = 0; c < VEC; c += 4) {
-                    *reinterpret_cast<float4v*>(&part_o[wave][i][VEC * (4 * g + r) + c]) =
-                        float4v{o[n][c][r], o[n][c + 1][r], o[n][c + 2][r], o[n][c + 3][r]};
-                }
+            for (int c = 0; c < VEC; c += 4) {
+                *reinterpret_cast<float4v*>(&part_o[wave][i][VEC * (4 * g + r) + c]) =
+                    float4v{o[mt][c][r], o[mt][c + 1][r], o[mt][c + 2][r], o[mt][c + 3][r]};
             }
         }
         __syncthreads();
-        // 16 threads per query
-        const int n = threadIdx.x / 16, m = m0 + 16 * mt + n;
-        if (m < queries) {
-            float now = part_m[0][n];
+        // the threads of a half of the waves share out its 16 queries
+        constexpr int kPer = 4 * KW;
+        const int n = threadIdx.x % (64 * KW) / kPer, m = m0 + 16 * mt + n, w0 = half * KW;
+        if (m >= queries) continue;
+        float high = part_m[w0][n];
 #pragma unroll
-            for (int w = 1; w < kAttendWaves; ++w) now = fmaxf(now, part_m[w][n]);
-            float share[kAttendWaves], l = 0.0F;
+        for (int w = 1; w < KW; ++w) high = fmaxf(high, part_m[w0 + w][n]);
+        float share[KW], l = 0.0F;
 #pragma unroll
-            for (int w = 0; w < kAttendWaves; ++w) {
-                share[w] = split_share(part_m[w][n], part_l[w][n], now);
-                l += part_l[w][n] * share[w];
-            }
-            const Query q = query_of(m, group, h);
-            const int64_t row = span.row0 + q.row;
-            const int64_t at = row * a.q.heads + q.head;
-            const bool whole = a.splits == 1;
-            const float scale = !whole ? 1.0F : l == 0.0F ? 0.0F : 1.0F / l;
-            for (int d = threadIdx.x % 16 * 8; d < dim; d += 128) {
-                float x[8];
+        for (int w = 0; w < KW; ++w) {
+            share[w] = split_share(part_m[w0 + w][n], part_l[w0 + w][n], high);
+            l += part_l[w0 + w][n] * share[w];
+        }
+        const Query q = query_of(m, group, h);
+        const int64_t row = span.row0 + q.row, at = row * a.q.heads + q.head;
+        const float scale = !complete ? 1.0F : l == 0.0F ? 0.0F : 1.0F / l;
+        for (int d = threadIdx.x % kPer * 8; d < dim; d += 8 * kPer) {
+            float x[8];
 #pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    x[e] = 0.0F;
+            for (int e = 0; e < 8; ++e) {
+                x[e] = 0.0F;
 #pragma unroll
-                    for (int w = 0; w < kAttendWaves; ++w) {
-                        if (share[w] != 0.0F) x[e] += part_o[w][n][d + e] * share[w];
-                    }
-                    x[e] *= scale;
+                for (int w = 0; w < KW; ++w) {
+                    if (share[w] != 0.0F) x[e] += part_o[w0 + w][n][d + e] * share[w];
                 }
-                if (whole) {
-                    store(a.out.data, row * a.out.row_stride + q.head * a.out.head_stride + d, a.out.type, x);
-                } else {
-                    store(a.partial, (static_cast<int64_t>(split) * rows_heads + at) * dim + d, kF32, x);
-                }
+                x[e] *= scale;
             }
-            if (threadIdx.x % 16 == 0) {
-                if (whole) {
-                    if (a.lse) a.lse[at] = now * kLn2 + logf(l);
-                } else {
-                    *reinterpret_cast<float2*>(a.marks + 2 * (static_cast<int64_t>(split) * rows_heads + at)) = float2{now, l};
-                }
-            }
+            if (complete) store(a.out.data, row * a.out.row_stride + q.head * a.out.head_stride + d, a.out.type, x);
+            else if (l != 0.0F) store(a.partial, (split * all + at) * dim + d, kF32, x);
+        }
+        if (threadIdx.x % kPer == 0) {
+            if (!complete) *reinterpret_cast<float2*>(a.marks + 2 * (split * all + at)) = float2{high, l};
+            else if (a.lse) a.lse[at] = high * kLn2 + logf(l);
         }
     }
 }
@@ -730,10 +765,13 @@ __global__ __launch_bounds__(kAttendThreads, HDP <= 128 ? 2 : 1) void k_attend_t
                 for (int j = 0; j < 8; ++j) any |= nonfinite<T>(vr[j].x) || nonfinite<T>(vr[j].y);
 #pragma unroll
                 for (int e = 0; e < 4; ++e) {
-                    uint8_t mark[3] = {0, 0, 0};
-                    if (any) take_nonfinite<T>(vr, e, mark);
+                    uint32_t mark[3] = {0, 0, 0};
+                    if (any) {
 #pragma unroll
-                    for (int k = 0; k < 3; ++k) marks[b][k][v_at + e][v_piece] = mark[k];
+                        for (int j = 0; j < 8; ++j) take_nonfinite<T>(e < 2 ? vr[j].x : vr[j].y, e % 2, j, mark);
+                    }
+#pragma unroll
+                    for (int k = 0; k < 3; ++k) marks[b][k][v_at + e][v_piece] = static_cast<uint8_t>(mark[k]);
                 }
             }
 #pragma unroll
@@ -848,9 +886,7 @@ __global__ __launch_bounds__(kAttendThreads, HDP <= 128 ? 2 : 1) void k_attend_t
                     const auto any = [&](int k) {
                         return (*reinterpret_cast<const unsigned long long*>(marks[b][k][d]) & seen) != 0;
                     };
-                    if (any(0)) o[e][r] += INFINITY;
-                    if (any(1)) o[e][r] -= INFINITY;
-                    if (any(2)) o[e][r] = NAN;
+                    o[e][r] = with_nonfinite(o[e][r], any(0), any(1), any(2));
                     asm volatile("" ::: "memory");  // one column's marks at a time: the sums leave few registers
                 }
             }
@@ -1449,8 +1485,10 @@ hipError_t launch_append(const Rotation* rotation, const Cache& c, const Batch& 
 
 namespace {
 
-// Queries (rows times the heads of a K/V head) of a sequence up to which the waves of a work-group divide its keys.
-constexpr uint32_t kFewQueries = 64;
+// Queries (rows times the heads of a K/V head) of a sequence up to which the waves of a work-group divide its keys: what
+// their registers hold.
+constexpr uint32_t few_queries(uint32_t head_dim) { return head_dim <= 128 ? 64 : 16; }
+constexpr uint32_t kFewQueries = 64;  // up to which a wave that adds up weights has slots of its own
 
 // How a step's attention is divided: by the most queries that a sequence may have.
 struct Tiling {
@@ -1462,10 +1500,9 @@ struct Tiling {
 Tiling tiling(const Cache& c, const Batch& b, uint32_t group) {
     const uint64_t most = static_cast<uint64_t>(b.max_rows) * group;
     Tiling t;
-    if (most <= kFewQueries) {
-        // tiles of 16 queries: 1, 2 or as many as the registers hold (4; 2 of wide heads)
-        t.queries = most <= 16 ? 16 : most <= 32 || c.head_dim > 128 ? 32 : 64;
-        t.keys = kAttendWaves * kFewKeys;
+    if (most <= few_queries(c.head_dim)) {
+        t.queries = most <= 16 ? 16 : most <= 32 ? 32 : 64;
+        t.keys = (c.head_dim > 128 ? kFewWaves<256> : most <= 32 ? kFewWaves<128> : kFewWaves<128> / 2) * kFewKeys;
     } else {
         t.queries = kTileQueries;
         t.keys = c.head_dim <= 128 ? kTileKeys<128> : kTileKeys<256>;
@@ -1480,12 +1517,13 @@ hipError_t attend_of(const Attend& a, hipStream_t stream) {
     const Tiling t = tiling(a.cache, a.batch, a.q.heads / a.cache.n_head_kv);
     const uint64_t groups = t.groups * a.splits;
     if (groups > 0x7FFFFFFF) return hipErrorInvalidConfiguration;
-    const dim3 grid(static_cast<uint32_t>(groups)), block(kAttendThreads);
-    if (t.queries == kTileQueries) return launch(k_attend_tile<T, HDP>, grid, block, stream, a, group);
-    if (t.queries == 16) return launch(k_attend_few<T, HDP, 1>, grid, block, stream, a, group);
-    if (t.queries == 32) return launch(k_attend_few<T, HDP, 2>, grid, block, stream, a, group);
-    if constexpr (HDP <= 128) return launch(k_attend_few<T, HDP, 4>, grid, block, stream, a, group);
-    return hipErrorInvalidConfiguration;
+    const dim3 grid(static_cast<uint32_t>(groups)), few(64 * kFewWaves<HDP>);
+    if (t.queries == kTileQueries) return launch(k_attend_tile<T, HDP>, grid, dim3(kAttendThreads), stream, a, group);
+    if constexpr (HDP <= 128) {
+        if (t.queries == 64) return launch(k_attend_few<T, HDP, 2, 2>, grid, few, stream, a, group);
+        if (t.queries == 32) return launch(k_attend_few<T, HDP, 2, 1>, grid, few, stream, a, group);
+    }
+    return launch(k_attend_few<T, HDP, 1, 1>, grid, few, stream, a, group);
 }
 
 template <typename T>

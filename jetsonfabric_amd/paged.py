@@ -19,39 +19,46 @@ __all__ = ["Rope", "PagedCache", "PagedBatch"]
 _TYPES = {"torch.float32": 1, "torch.float16": 2, "torch.bfloat16": 3}
 _LAYOUTS = {"half": 0, "interleaved": 1}
 _SCALINGS = {"none": 0, "linear": 1, "ntk": 2, "yarn": 3}
+_codes: dict = {}  # torch dtype -> jfh_value_type
 
 
 def _type(x, name: str) -> int:
-    t = _TYPES.get(str(x.dtype))
+    t = _codes.get(x.dtype)
     if t is None:
-        raise ValueError(f"{name} holds {x.dtype}: float32, float16 and bfloat16 are supported")
+        t = _TYPES.get(str(x.dtype))
+        if t is None:
+            raise ValueError(f"{name} holds {x.dtype}: float32, float16 and bfloat16 are supported")
+        _codes[x.dtype] = t
     return t
 
 
 def _rows(x, name: str, device: int) -> _capi.Rows:
     """A tensor [rows, heads, head dim] of any strides whose heads are contiguous."""
-    if x.dim() != 3:
+    shape, stride = x.shape, x.stride()
+    if len(shape) != 3:
         raise ValueError(f"{name} must be [rows, heads, head dim]")
-    if not x.is_cuda or x.get_device() != device:
+    if x.get_device() != device or device < 0:
         raise ValueError(f"{name} must be on GPU {device}")
-    rows, heads, dim = x.shape
-    row_stride, head_stride, one = x.stride()
-    if one != 1 and dim > 1:
+    if stride[2] != 1 and shape[2] > 1:
         raise ValueError(f"the values of a head of {name} must be contiguous")
-    return _capi.Rows(x.data_ptr(), row_stride, head_stride, rows, heads, dim, _type(x, name))
+    return _capi.Rows(x.data_ptr(), stride[0], stride[1], shape[0], shape[1], shape[2], _type(x, name))
 
 
 def _array(x, name: str, dtype: str, device: int, shape: tuple | None = None) -> int:
     """Address of a contiguous device array."""
-    if str(x.dtype) != dtype or not x.is_cuda or x.get_device() != device or not x.is_contiguous():
+    if x.dtype is not getattr(_torch(), dtype) or x.get_device() != device or device < 0 or not x.is_contiguous():
         raise ValueError(f"{name} must be a contiguous {dtype} tensor on GPU {device}")
     if shape is not None and x.shape != shape:
         raise ValueError(f"{name} must have shape {list(shape)}, not {list(x.shape)}")
     return x.data_ptr()
 
 
+def _torch():
+    return sys.modules["torch"]  # there once the caller has a tensor
+
+
 def _stream(device: int) -> int:
-    return sys.modules["torch"].cuda.current_stream(device).cuda_stream
+    return _torch().cuda.current_stream(device).cuda_stream
 
 
 class Rope:
@@ -91,10 +98,10 @@ class Rope:
         """x [rows, heads, head dim] rotated by positions (int32 [rows]) into out, which may be x or
         have another type; a new tensor like x by default. Returns out."""
         if out is None:
-            out = sys.modules["torch"].empty_like(x)
+            out = _torch().empty_like(x)
         device = x.get_device()
         a, b = _rows(x, "x", device), _rows(out, "out", device)
-        at = _array(positions, "positions", "torch.int32", device, (x.shape[0],))
+        at = _array(positions, "positions", "int32", device, (x.shape[0],))
         check(library().jfh_rope_rotate(self._h, ctypes.byref(a), at, ctypes.byref(b), device, _stream(device)))
         return out
 
@@ -111,10 +118,11 @@ class PagedBatch:
         n = table.shape[0]
         self.table, self.lengths, self.row_starts = table, lengths, row_starts
         self.device = device
-        self.c = _capi.PagedBatch(_array(table, "table", "torch.int32", device),
-                                  _array(lengths, "lengths", "torch.int32", device, (n,)),
-                                  _array(row_starts, "row_starts", "torch.int32", device, (n + 1,)), n, table.shape[1],
+        self.c = _capi.PagedBatch(_array(table, "table", "int32", device),
+                                  _array(lengths, "lengths", "int32", device, (n,)),
+                                  _array(row_starts, "row_starts", "int32", device, (n + 1,)), n, table.shape[1],
                                   max_rows, max_length)
+        self.workspaces: dict = {}
         self.ref = ctypes.byref(self.c)
 
 
@@ -137,66 +145,70 @@ class PagedCache:
         self.device = device
         self.c = _capi.PagedCache(
             k.data_ptr(), v.data_ptr(),
-            None if weights is None else _array(weights, "weights", "torch.float32", device, meta),
-            None if positions is None else _array(positions, "positions", "torch.int32", device, meta),
+            None if weights is None else _array(weights, "weights", "float32", device, meta),
+            None if positions is None else _array(positions, "positions", "int32", device, meta),
             k.stride(0), k.stride(1), k.stride(2), pages, page_size, heads, dim, _type(k, "k"), device)
         self.ref = ctypes.byref(self.c)
+        self.shape = (heads, dim, page_size)
 
     def _of(self, batch: PagedBatch):
         if batch.device != self.device:
             raise ValueError(f"the batch is on GPU {batch.device}, the cache on GPU {self.device}")
         return batch.ref
 
-    def _workspace(self, size: int):
-        # of torch's allocator: ordered by the current stream, and a captured graph's own
-        return sys.modules["torch"].empty(size, dtype=sys.modules["torch"].uint8, device=self.k.device) if size else None
+    def _workspace(self, batch: PagedBatch, call: str, *args):
+        """Address and size of a call's workspace (and the tensor that holds it), from torch's allocator:
+        ordered by the current stream, and a captured graph's own. Its size goes by the shapes alone."""
+        key = (call, self.shape, *((a.n_rows, a.n_head) if isinstance(a, _capi.Rows) else a for a in args))
+        size = batch.workspaces.get(key)
+        if size is None:
+            need = ctypes.c_size_t()
+            check(getattr(library(), f"jfh_paged_{call}_workspace")(
+                self.ref, batch.ref, *(ctypes.byref(a) if isinstance(a, _capi.Rows) else a for a in args), ctypes.byref(need)))
+            size = batch.workspaces[key] = need.value
+        if size == 0:
+            return None, 0, None
+        space = _torch().empty(size, dtype=_torch().uint8, device=self.k.device)
+        return space.data_ptr(), size, space
 
     def append(self, batch: PagedBatch, k, v, positions=None, rope: Rope | None = None) -> None:
         """Writes a step's rows k and v [rows, K/V heads, head dim] at its sequences' last slots, k
         rotated by rope; positions int32 [rows]."""
         a, b = _rows(k, "k", self.device), _rows(v, "v", self.device)
-        at = None if positions is None else _array(positions, "positions", "torch.int32", self.device, (k.shape[0],))
+        at = None if positions is None else _array(positions, "positions", "int32", self.device, (k.shape[0],))
         check(library().jfh_paged_append(self.ref, self._of(batch), ctypes.byref(a), ctypes.byref(b),
                                          None if rope is None else rope.handle, at, _stream(self.device)))
 
     def attend(self, batch: PagedBatch, q, scale: float | None = None, causal: bool = True, out=None, lse=None):
         """softmax(scale q K^T) V of a step's rows q [rows, heads, head dim] over their sequences' slots
         (scale 1 / sqrt(head dim) by default) and ln sum exp of the scores, float32 [rows, heads].
-        Returns (out, lse), written where they are given; rows of no sequence are left as they were,
-        zeros in new tensors."""
-        torch = sys.modules["torch"]
+        Returns (out, lse), new tensors where they are not given; rows of no sequence are not written."""
+        torch = _torch()
         if out is None:
-            out = torch.zeros_like(q)
+            out = torch.empty_like(q)
         if lse is None:
-            lse = torch.zeros(q.shape[:2], dtype=torch.float32, device=q.device)
+            lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
         a, b = _rows(q, "q", self.device), _rows(out, "out", self.device)
-        at = _array(lse, "lse", "torch.float32", self.device, q.shape[:2])
-        need = ctypes.c_size_t()
-        check(library().jfh_paged_attention_workspace(self.ref, self._of(batch), ctypes.byref(a), ctypes.byref(need)))
-        space = self._workspace(need.value)
-        check(library().jfh_paged_attention(self.ref, batch.ref, ctypes.byref(a),
-                                            a.head_dim ** -0.5 if scale is None else scale, int(causal), ctypes.byref(b),
-                                            at, None if space is None else space.data_ptr(), need.value,
-                                            _stream(self.device)))
+        at = _array(lse, "lse", "float32", self.device, q.shape[:2])
+        ref = self._of(batch)
+        space, size, _held = self._workspace(batch, "attention", a)
+        check(library().jfh_paged_attention(self.ref, ref, ctypes.byref(a), a.head_dim ** -0.5 if scale is None else scale,
+                                            int(causal), ctypes.byref(b), at, space, size, _stream(self.device)))
         return out, lse
 
     def weigh(self, batch: PagedBatch, q, lse, scale: float | None = None, causal: bool = True) -> None:
         """Adds the attention that the rows q (with attend's lse, scale and causal) give each position to
         the cache's weights."""
         a = _rows(q, "q", self.device)
-        at = _array(lse, "lse", "torch.float32", self.device, q.shape[:2])
-        need = ctypes.c_size_t()
-        check(library().jfh_paged_weigh_workspace(self.ref, self._of(batch), ctypes.byref(a), ctypes.byref(need)))
-        space = self._workspace(need.value)
-        check(library().jfh_paged_weigh(self.ref, batch.ref, ctypes.byref(a), at,
-                                        a.head_dim ** -0.5 if scale is None else scale, int(causal),
-                                        None if space is None else space.data_ptr(), need.value, _stream(self.device)))
+        at = _array(lse, "lse", "float32", self.device, q.shape[:2])
+        ref = self._of(batch)
+        space, size, _held = self._workspace(batch, "weigh", a)
+        check(library().jfh_paged_weigh(self.ref, ref, ctypes.byref(a), at, a.head_dim ** -0.5 if scale is None else scale,
+                                        int(causal), space, size, _stream(self.device)))
 
     def evict(self, batch: PagedBatch, budget: int, n_first: int = 4, n_recent: int = 1) -> None:
         """Cuts every longer sequence to budget slots per K/V head: the positions below n_first, the
         n_recent newest, then the heaviest stay; batch.lengths becomes what is left."""
-        need = ctypes.c_size_t()
-        check(library().jfh_paged_evict_workspace(self.ref, self._of(batch), budget, ctypes.byref(need)))
-        space = self._workspace(need.value)
-        check(library().jfh_paged_evict(self.ref, batch.ref, budget, n_first, n_recent,
-                                        None if space is None else space.data_ptr(), need.value, _stream(self.device)))
+        ref = self._of(batch)
+        space, size, _held = self._workspace(batch, "evict", budget)
+        check(library().jfh_paged_evict(self.ref, ref, budget, n_first, n_recent, space, size, _stream(self.device)))
