@@ -319,8 +319,8 @@ __device__ __forceinline__ Query query_of(int m, int group, uint32_t kv_head) {
     return Query{row, static_cast<int>(kv_head) * group + (m - row * group)};
 }
 
-// Few query rows: o = softmax(scale q K^T) V for up to 16 MT QG queries of a K/V head. Its 8 waves (4 of wide heads) divide
-// the keys; with QG = 2 those of either half have half of the queries, as one wave's registers hold 32.
+// Few query rows: o = softmax(scale q K^T) V for up to 16 MT queries of a K/V head, 8 waves (4 of wide heads) that divide its
+// keys.
 //
 // The bytes of K and V bound it where there are enough of them, and their latency elsewhere. A wave takes tiles of 32 keys
 // from global memory to registers, in the layout of the rows: S^T = K Q^T on 16x16x32 products has a K row's 16 bytes per
@@ -333,7 +333,7 @@ __device__ __forceinline__ Query query_of(int m, int group, uint32_t kv_head) {
 // the output), its sum is not. A row's maximum is raised only when a tile exceeds it by 2^8: P stays far below 65504.
 template <int HDP> constexpr int kFewWaves = HDP <= 128 ? 8 : 4;
 
-template <typename T, int HDP, int MT, int QG>
+template <typename T, int HDP, int MT>
 __global__ __launch_bounds__(64 * kFewWaves<HDP>) void k_attend_few(Attend a, int group) {
     using V = Values<T>;
     using v8 = typename V::v8;
@@ -342,30 +342,29 @@ __global__ __launch_bounds__(64 * kFewWaves<HDP>) void k_attend_few(Attend a, in
     constexpr int VW = VEC / 2;     // words per lane and V row
     constexpr int kChunk = VW < 4 ? VW : 4;  // words of one load
     constexpr int OS = HDP + 4;     // floats per query of the waves' sums in LDS
-    constexpr int kWaves = kFewWaves<HDP>, kThreads = 64 * kWaves, KW = kWaves / QG;  // waves that divide the keys
+    constexpr int kWaves = kFewWaves<HDP>, kThreads = 64 * kWaves;
     __shared__ float part_o[kWaves][16][OS];
     __shared__ float part_m[kWaves][16], part_l[kWaves][16];
-    __shared__ uint4 q_lds[QG * MT][KC][64];
+    __shared__ uint4 q_lds[MT][KC][64];
 
-    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64, half = wave / KW;
+    const int lane = threadIdx.x % 64, wave = threadIdx.x / 64;
     const int i = lane % 16, g = lane / 16;
     const uint32_t pairs = a.cache.n_head_kv * a.batch.n_seq;  // K/V heads of sequences
     const uint32_t split = blockIdx.x % a.splits, pair = blockIdx.x / a.splits % pairs;
     const uint32_t h = pair % a.cache.n_head_kv, s = pair / a.cache.n_head_kv;
-    const int group_m0 = static_cast<int>(blockIdx.x / a.splits / pairs) * 16 * MT * QG, m0 = group_m0 + 16 * MT * half;
+    const int m0 = static_cast<int>(blockIdx.x / a.splits / pairs) * 16 * MT;
     const Span span = sequence_span(a.batch, a.q.rows, s);
     const int queries = span.rows * group;
-    if (group_m0 >= queries) return;
+    if (m0 >= queries) return;
     const int dim = static_cast<int>(a.cache.head_dim);
     const int first = span.len - span.rows;  // slot of row 0
     const auto sees = [&](int m) { return a.causal ? max(0, first + m / group + 1) : span.len; };  // slots of query m
-    // seen by all queries of the wave, by any
-    const int least = sees(min(m0, queries - 1)), end = m0 < queries ? sees(min(queries, m0 + 16 * MT) - 1) : 0;
+    const int least = sees(m0), end = sees(min(queries, m0 + 16 * MT) - 1);  // seen by all queries here, by any
 
-    // the split's tiles: equal parts of the sequence's
+    // the split's tiles: equal parts of the sequence's, whole rounds of the waves
     const int tiles = (span.len + kFewKeys - 1) / kFewKeys;
-    const int per = (tiles + static_cast<int>(a.splits) - 1) / static_cast<int>(a.splits);
-    const int t0 = static_cast<int>(split) * per, t1 = min(min(tiles, t0 + per), (end + kFewKeys - 1) / kFewKeys);
+    const int per = (tiles + static_cast<int>(a.splits) * kWaves - 1) / (static_cast<int>(a.splits) * kWaves) * kWaves;
+    const int t0 = min(static_cast<int>(split) * per, tiles), t1 = min(min(tiles, t0 + per), (end + kFewKeys - 1) / kFewKeys);
 
     const T* k_head = static_cast<const T*>(a.cache.k) + h * a.cache.head_stride;
     const T* v_head = static_cast<const T*>(a.cache.v) + h * a.cache.head_stride;
@@ -411,19 +410,19 @@ __global__ __launch_bounds__(64 * kFewWaves<HDP>) void k_attend_few(Attend a, in
         }
     };
 
-    int t = t0 + wave % KW;
+    int t = t0 + wave;
     Keys now{}, next{};
     if (t < t1) {
         now = look_up(t);
         fetch_k(now);
         fetch_v(now);
-        if (t + KW < t1) next = look_up(t + KW);
+        if (t + kWaves < t1) next = look_up(t + kWaves);
     }
 
     // queries to LDS in operand order, zeros behind the last one and beyond head_dim
-    for (int e = threadIdx.x; e < QG * MT * KC * 64; e += kThreads) {
+    for (int e = threadIdx.x; e < MT * KC * 64; e += kThreads) {
         const int l = e % 64, c = e / 64 % KC, mt = e / 64 / KC;
-        const int m = group_m0 + 16 * mt + l % 16, d = 32 * c + 8 * (l / 16);
+        const int m = m0 + 16 * mt + l % 16, d = 32 * c + 8 * (l / 16);
         uint4 x{0, 0, 0, 0};
         if (m < queries && d < dim) {
             const Query q = query_of(m, group, h);
@@ -447,7 +446,7 @@ __global__ __launch_bounds__(64 * kFewWaves<HDP>) void k_attend_few(Attend a, in
         for (int c = 0; c < VEC; ++c) o[mt][c] = float4v{0.0F, 0.0F, 0.0F, 0.0F};
     }
 
-    for (; t < t1; t += KW) {
+    for (; t < t1; t += kWaves) {
         const int base = t * kFewKeys;
         const bool whole = now.present == 0xFFFFFFFFU;
         const bool hidden = base + kFewKeys > least;  // some query here does not see some of the tile
@@ -464,12 +463,12 @@ __global__ __launch_bounds__(64 * kFewWaves<HDP>) void k_attend_few(Attend a, in
         for (int c = 0; c < KC; ++c) {
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) {
-                const v8 q = __builtin_bit_cast(v8, q_lds[half * MT + mt][c][lane]);
+                const v8 q = __builtin_bit_cast(v8, q_lds[mt][c][lane]);
                 sc[mt][0] = V::mfma(k[0][c], q, sc[mt][0]);
                 sc[mt][1] = V::mfma(k[1][c], q, sc[mt][1]);
             }
         }
-        if (t + KW < t1) fetch_k(next);
+        if (t + kWaves < t1) fetch_k(next);
 
         // scores of keys base + 16 u + 4 g + r, query i
         uint32_t seen[MT];
@@ -573,10 +572,10 @@ __global__ __launch_bounds__(64 * kFewWaves<HDP>) void k_attend_few(Attend a, in
                 }
             }
         }
-        if (t + KW < t1) {
+        if (t + kWaves < t1) {
             fetch_v(next);
             now = next;
-            if (t + 2 * KW < t1) next = look_up(t + 2 * KW);
+            if (t + 2 * kWaves < t1) next = look_up(t + 2 * kWaves);
         }
     }
 
@@ -585,7 +584,7 @@ __global__ __launch_bounds__(64 * kFewWaves<HDP>) void k_attend_few(Attend a, in
     const bool complete = a.splits == 1;
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
-        if (group_m0 + 16 * mt >= queries) break;
+        if (m0 + 16 * mt >= queries) break;
         __syncthreads();
         const float wave_l = groups_sum(sum[mt]);
         if (g == 0) part_m[wave][i] = top[mt], part_l[wave][i] = wave_l;
@@ -599,18 +598,17 @@ __global__ __launch_bounds__(64 * kFewWaves<HDP>) void k_attend_few(Attend a, in
             }
         }
         __syncthreads();
-        // the threads of a half of the waves share out its 16 queries
-        constexpr int kPer = 4 * KW;
-        const int n = threadIdx.x % (64 * KW) / kPer, m = m0 + 16 * mt + n, w0 = half * KW;
+        constexpr int kPer = kThreads / 16;  // threads of a query
+        const int n = threadIdx.x / kPer, m = m0 + 16 * mt + n;
         if (m >= queries) continue;
-        float high = part_m[w0][n];
+        float high = part_m[0][n];
 #pragma unroll
-        for (int w = 1; w < KW; ++w) high = fmaxf(high, part_m[w0 + w][n]);
-        float share[KW], l = 0.0F;
+        for (int w = 1; w < kWaves; ++w) high = fmaxf(high, part_m[w][n]);
+        float share[kWaves], l = 0.0F;
 #pragma unroll
-        for (int w = 0; w < KW; ++w) {
-            share[w] = split_share(part_m[w0 + w][n], part_l[w0 + w][n], high);
-            l += part_l[w0 + w][n] * share[w];
+        for (int w = 0; w < kWaves; ++w) {
+            share[w] = split_share(part_m[w][n], part_l[w][n], high);
+            l += part_l[w][n] * share[w];
         }
         const Query q = query_of(m, group, h);
         const int64_t row = span.row0 + q.row, at = row * a.q.heads + q.head;
@@ -621,8 +619,8 @@ __global__ __launch_bounds__(64 * kFewWaves<HDP>) void k_attend_few(Attend a, in
             for (int e = 0; e < 8; ++e) {
                 x[e] = 0.0F;
 #pragma unroll
-                for (int w = 0; w < KW; ++w) {
-                    if (share[w] != 0.0F) x[e] += part_o[w0 + w][n][d + e] * share[w];
+                for (int w = 0; w < kWaves; ++w) {
+                    if (share[w] != 0.0F) x[e] += part_o[w][n][d + e] * share[w];
                 }
                 x[e] *= scale;
             }
@@ -926,52 +924,69 @@ __global__ __launch_bounds__(kAttendThreads, HDP <= 128 ? 2 : 1) void k_attend_t
     }
 }
 
-// Joins the splits of one row and head: 32 (head dims up to 128: 16) threads hold a partial's columns 8 each, the others
-// take other splits. Rows of no sequence are left as they are.
+// Joins the splits of a row and head: 32 (head dims up to 128: 16) threads hold a partial's columns 8 each, `takers` such
+// groups take every takers-th split of a row and head, and a work-group has as many rows and heads as that leaves room for.
+// Rows of no sequence are left as they are. Latency bounds short joins, so a thread's first partial and marks are requested
+// before anything else is known; what no split wrote is not used.
 constexpr int kJoinThreads = 256;
 
-__global__ __launch_bounds__(kJoinThreads) void k_attend_join(Attend a) {
+__global__ __launch_bounds__(kJoinThreads) void k_attend_join(Attend a, int takers) {
     __shared__ float part[16][kMaxHeadDim];
-    __shared__ float part_l[16];
-    const int64_t at = blockIdx.x, all = static_cast<int64_t>(a.q.rows) * a.q.heads;
-    const int row = static_cast<int>(at / a.q.heads), head = static_cast<int>(at % a.q.heads);
-    Span span;
-    if (sequence_of(a.batch, a.q.rows, row, &span) < 0) return;
+    __shared__ float2 part_mark[16];
+    const int64_t all = static_cast<int64_t>(a.q.rows) * a.q.heads;
     const int dim = static_cast<int>(a.cache.head_dim), splits = static_cast<int>(a.splits);
+    const int wide = dim <= 128 ? 16 : 32, unit = threadIdx.x / wide, d = threadIdx.x % wide * 8;
+    const int taker = unit % takers, joins = kJoinThreads / wide / takers;
+    const int64_t at = min(blockIdx.x * static_cast<int64_t>(joins) + unit / takers, all - 1);
     const float2* marks = reinterpret_cast<const float2*>(a.marks) + at;
-    float now = -INFINITY;
-    for (int s = threadIdx.x % 64; s < splits; s += 64) now = fmaxf(now, marks[s * all].x);
-#pragma unroll
-    for (int o = 32; o; o /= 2) now = fmaxf(now, __shfl_xor(now, o));
+    float2 mark{-INFINITY, 0.0F};
+    float y[8] = {};
+    if (taker < splits) {
+        mark = marks[taker * all];
+        if (d < dim) load(a.partial, (taker * all + at) * dim + d, kF32, y);
+    }
+    const int row = static_cast<int>(at / a.q.heads), head = static_cast<int>(at - row * static_cast<int64_t>(a.q.heads));
+    Span span;
+    const bool owned = sequence_of(a.batch, a.q.rows, row, &span) >= 0 && blockIdx.x * static_cast<int64_t>(joins) + unit / takers < all;
 
-    const int wide = dim <= 128 ? 16 : 32, takers = kJoinThreads / wide;
-    const int d = threadIdx.x % wide * 8, taker = threadIdx.x / wide;
-    float x[8] = {}, l = 0.0F;
-    for (int s = taker; s < splits; s += takers) {
-        const float2 mark = marks[s * all];
-        if (mark.y == 0.0F) continue;
-        const float share = split_share(mark.x, mark.y, now);
-        l += mark.y * share;
-        if (d < dim) {
-            float y[8];
-            load(a.partial, (s * all + at) * dim + d, kF32, y);
+    float x[8] = {}, top = -INFINITY, l = 0.0F;
+    if (owned) {
+        for (int s = taker; s < splits; s += takers) {
+            if (s != taker) {
+                mark = marks[s * all];
+                if (d < dim) load(a.partial, (s * all + at) * dim + d, kF32, y);
+            }
+            if (mark.y == 0.0F) continue;  // nothing seen: the split wrote no sums
+            const float high = fmaxf(top, mark.x), before = split_share(top, l, high), share = split_share(mark.x, mark.y, high);
+            top = high;
+            l = l * before + mark.y * share;
 #pragma unroll
-            for (int e = 0; e < 8; ++e) x[e] += y[e] * share;
+            for (int e = 0; e < 8; ++e) x[e] = x[e] * before + y[e] * share;
         }
     }
-    if (d < dim) store(part[taker], d, kF32, x);
-    if (d == 0) part_l[taker] = l;
-    __syncthreads();
-    if (static_cast<int>(threadIdx.x) >= wide) return;
-    l = 0.0F;
-    for (int t = 0; t < takers; ++t) l += part_l[t];
-    if (d == 0 && a.lse) a.lse[at] = now * kLn2 + logf(l);
-    if (d >= dim) return;
-    for (int e = 0; e < 8; ++e) x[e] = 0.0F;
-    for (int t = 0; t < takers; ++t) {
+    if (takers > 1) {
+        if (d < dim) store(part[unit], d, kF32, x);
+        if (d == 0) part_mark[unit] = float2{top, l};
+        __syncthreads();
+        if (taker != 0 || !owned) return;
+        for (int t = 0; t < takers; ++t) top = fmaxf(top, part_mark[unit + t].x);
+        l = 0.0F;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) x[e] += part[t][d + e];
+        for (int e = 0; e < 8; ++e) x[e] = 0.0F;
+        for (int t = 0; t < takers; ++t) {
+            const float2 other = part_mark[unit + t];
+            const float share = split_share(other.x, other.y, top);
+            if (other.y == 0.0F) continue;
+            l += other.y * share;
+            if (d < dim) {
+#pragma unroll
+                for (int e = 0; e < 8; ++e) x[e] += part[unit + t][d + e] * share;
+            }
+        }
     }
+    if (!owned) return;
+    if (d == 0 && a.lse) a.lse[at] = top * kLn2 + logf(l);
+    if (d >= dim) return;
     const float scale = l == 0.0F ? 0.0F : 1.0F / l;
 #pragma unroll
     for (int e = 0; e < 8; ++e) x[e] *= scale;
@@ -1486,8 +1501,8 @@ hipError_t launch_append(const Rotation* rotation, const Cache& c, const Batch& 
 namespace {
 
 // Queries (rows times the heads of a K/V head) of a sequence up to which the waves of a work-group divide its keys: what
-// their registers hold.
-constexpr uint32_t few_queries(uint32_t head_dim) { return head_dim <= 128 ? 64 : 16; }
+// their registers hold. (45 queries at 4096 positions: 26 us with 64 here, half for either half of the waves; 22 on tiles.)
+constexpr uint32_t few_queries(uint32_t head_dim) { return head_dim <= 128 ? 32 : 16; }
 constexpr uint32_t kFewQueries = 64;  // up to which a wave that adds up weights has slots of its own
 
 // How a step's attention is divided: by the most queries that a sequence may have.
@@ -1501,8 +1516,8 @@ Tiling tiling(const Cache& c, const Batch& b, uint32_t group) {
     const uint64_t most = static_cast<uint64_t>(b.max_rows) * group;
     Tiling t;
     if (most <= few_queries(c.head_dim)) {
-        t.queries = most <= 16 ? 16 : most <= 32 ? 32 : 64;
-        t.keys = (c.head_dim > 128 ? kFewWaves<256> : most <= 32 ? kFewWaves<128> : kFewWaves<128> / 2) * kFewKeys;
+        t.queries = most <= 16 ? 16 : 32;
+        t.keys = (c.head_dim > 128 ? kFewWaves<256> : kFewWaves<128>) * kFewKeys;
     } else {
         t.queries = kTileQueries;
         t.keys = c.head_dim <= 128 ? kTileKeys<128> : kTileKeys<256>;
@@ -1520,10 +1535,9 @@ hipError_t attend_of(const Attend& a, hipStream_t stream) {
     const dim3 grid(static_cast<uint32_t>(groups)), few(64 * kFewWaves<HDP>);
     if (t.queries == kTileQueries) return launch(k_attend_tile<T, HDP>, grid, dim3(kAttendThreads), stream, a, group);
     if constexpr (HDP <= 128) {
-        if (t.queries == 64) return launch(k_attend_few<T, HDP, 2, 2>, grid, few, stream, a, group);
-        if (t.queries == 32) return launch(k_attend_few<T, HDP, 2, 1>, grid, few, stream, a, group);
+        if (t.queries == 32) return launch(k_attend_few<T, HDP, 2>, grid, few, stream, a, group);
     }
-    return launch(k_attend_few<T, HDP, 1, 1>, grid, few, stream, a, group);
+    return launch(k_attend_few<T, HDP, 1>, grid, few, stream, a, group);
 }
 
 template <typename T>
@@ -1538,17 +1552,33 @@ hipError_t attend(const Attend& a, hipStream_t stream) {
 uint32_t attend_splits(const Cache& c, const Batch& b, uint32_t group) {
     const Tiling t = tiling(c, b, group);
     if (t.groups == 0) return 1;
-    // two work-groups per compute unit, unless there is one without splits; a split of fewer than two rounds of keys costs
-    // more than it gains
-    if (t.groups >= kComputeUnits) return 1;
-    const uint64_t wanted = (2 * kComputeUnits + t.groups - 1) / t.groups, most = b.max_length / (2 * t.keys);
-    return static_cast<uint32_t>(wanted < most ? wanted : most > 0 ? most : 1);
+    // Work-groups that run at once: one per compute unit of the few-query form, two of the tiles. Splits that fill the chip
+    // once or, with few queries, twice (the second rounds even out sequences of different lengths: eight rows over up to
+    // 32701 positions 113 us, 140 in one round), whichever takes fewer rounds of keys in a row; of two rounds at least, as
+    // partial sums cost more than shorter ones gain.
+    const bool few = t.queries != kTileQueries;
+    const uint64_t resident = few ? kComputeUnits : 2 * kComputeUnits, least = 2;
+    if (t.groups >= resident) return 1;
+    const uint64_t rounds = (b.max_length + t.keys - 1) / t.keys;
+    uint64_t best = 1, cost = ~0ULL;
+    for (uint64_t fill = 1; fill <= (few ? 2 : 1); ++fill) {
+        const uint64_t wanted = fill * resident / t.groups, even = (rounds + wanted - 1) / wanted, per = even > least ? even : least;
+        const uint64_t splits = (rounds + per - 1) / per, takes = (t.groups * splits + resident - 1) / resident * per;
+        if (splits > 0 && takes <= cost) best = splits, cost = takes;
+    }
+    return static_cast<uint32_t>(best);
 }
 
 hipError_t launch_attend(const Attend& a, hipStream_t stream) {
     const hipError_t e = a.cache.type == kF16 ? attend<_Float16>(a, stream) : attend<__bf16>(a, stream);
     if (e != hipSuccess || a.splits == 1) return e;
-    return launch(k_attend_join, dim3(a.q.rows * a.q.heads), dim3(kJoinThreads), stream, a);
+    // as many takers as splits, in powers of two, up to a work-group's units
+    const uint32_t units = a.cache.head_dim <= 128 ? 16 : 8;
+    uint32_t takers = 1;
+    while (2 * takers <= a.splits && takers < units) takers *= 2;
+    const uint64_t joins = units / takers, all = static_cast<uint64_t>(a.q.rows) * a.q.heads;
+    return launch(k_attend_join, dim3(static_cast<uint32_t>((all + joins - 1) / joins)), dim3(kJoinThreads), stream, a,
+                  static_cast<int>(takers));
 }
 
 namespace {
