@@ -1500,9 +1500,12 @@ hipError_t launch_append(const Rotation* rotation, const Cache& c, const Batch& 
 
 namespace {
 
-// Queries (rows times the heads of a K/V head) of a sequence up to which the waves of a work-group divide its keys: what
-// their registers hold. (45 queries at 4096 positions: 26 us with 64 here, half for either half of the waves; 22 on tiles.)
-constexpr uint32_t few_queries(uint32_t head_dim) { return head_dim <= 128 ? 32 : 16; }
+// Queries (rows times the heads of a K/V head) of a sequence up to which the waves of a work-group divide its keys: 16,
+// one tile of scores, and 32 where there are so many positions that the bytes of K and V alone count (21 queries, 32 K/V
+// heads of sequences of 30000 positions: 102 us, 116 on tiles; of 4000: 29, 26 on tiles).
+uint32_t few_queries(const Cache& c, const Batch& b) {
+    return c.head_dim <= 128 && static_cast<uint64_t>(c.n_head_kv) * b.n_seq * b.max_length >= (1U << 19) ? 32 : 16;
+}
 constexpr uint32_t kFewQueries = 64;  // up to which a wave that adds up weights has slots of its own
 
 // How a step's attention is divided: by the most queries that a sequence may have.
@@ -1515,7 +1518,7 @@ struct Tiling {
 Tiling tiling(const Cache& c, const Batch& b, uint32_t group) {
     const uint64_t most = static_cast<uint64_t>(b.max_rows) * group;
     Tiling t;
-    if (most <= few_queries(c.head_dim)) {
+    if (most <= few_queries(c, b)) {
         t.queries = most <= 16 ? 16 : 32;
         t.keys = (c.head_dim > 128 ? kFewWaves<256> : kFewWaves<128>) * kFewKeys;
     } else {
@@ -1552,19 +1555,21 @@ hipError_t attend(const Attend& a, hipStream_t stream) {
 uint32_t attend_splits(const Cache& c, const Batch& b, uint32_t group) {
     const Tiling t = tiling(c, b, group);
     if (t.groups == 0) return 1;
-    // Work-groups that run at once: one per compute unit of the few-query form, two of the tiles. Splits that fill the chip
-    // once or, with few queries, twice (the second rounds even out sequences of different lengths: eight rows over up to
-    // 32701 positions 113 us, 140 in one round), whichever takes fewer rounds of keys in a row; of two rounds at least, as
-    // partial sums cost more than shorter ones gain.
+    // Rounds of keys in a row set the time, counted in halves: a work-group's beginning and end take about three halves,
+    // the join four (of 256 keys; eight of a tile's 64). Work-groups that run at once: one per compute unit of the
+    // few-query form, two of the tiles. No splits, or so many as fill the chip once, or, of long few-query calls, twice
+    // where that costs little, and 128 at most, for the join: the second rounds even out sequences of different lengths (eight rows over up to 32701
+    // positions 113 us, 140 in one round; 32 K/V heads of sequences of 4000, equal: 22 in one, 29 in two short ones).
     const bool few = t.queries != kTileQueries;
-    const uint64_t resident = few ? kComputeUnits : 2 * kComputeUnits, least = 2;
+    const uint64_t resident = few ? kComputeUnits : 2 * kComputeUnits, least = t.queries <= 16 ? 1 : 2;
     if (t.groups >= resident) return 1;
     const uint64_t rounds = (b.max_length + t.keys - 1) / t.keys;
-    uint64_t best = 1, cost = ~0ULL;
+    uint64_t best = 1, cost = 2 * rounds + 3;
     for (uint64_t fill = 1; fill <= (few ? 2 : 1); ++fill) {
-        const uint64_t wanted = fill * resident / t.groups, even = (rounds + wanted - 1) / wanted, per = even > least ? even : least;
-        const uint64_t splits = (rounds + per - 1) / per, takes = (t.groups * splits + resident - 1) / resident * per;
-        if (splits > 0 && takes <= cost) best = splits, cost = takes;
+        const uint64_t fills = fill * resident / t.groups, wanted = fills < 128 ? fills : 128, even = (rounds + wanted - 1) / wanted, per = even > least ? even : least;
+        const uint64_t splits = (rounds + per - 1) / per, turns = (t.groups * splits + resident - 1) / resident;
+        const uint64_t takes = turns * (2 * per + 3) + (few ? 4 : 8);
+        if (splits > 1 && (takes < cost || (best > 1 && per >= 8 && 10 * takes <= 11 * cost))) best = splits, cost = takes;
     }
     return static_cast<uint32_t>(best);
 }
