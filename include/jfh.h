@@ -505,7 +505,8 @@ jfh_status jfh_paged_append(const jfh_paged_cache * cache, const jfh_paged_batch
  * h / (n_head / n_head_kv). With causal, row r of a sequence's n sees its slots
  * 0 .. lengths - n + r, otherwise all of them. q and out have the cache's type
  * and head_dim, 16-byte aligned, strides in multiples of 8 values; lse (device,
- * float [n_rows][n_head], may be NULL) receives ln sum exp(scale q K^T). A row
+ * float [n_rows][n_head], may be NULL) receives ln sum exp(scale q K^T). out may
+ * be q itself, and overlaps it in no other way. A row
  * that sees nothing gives 0 and -inf; what a row does not see does not reach
  * it, infinities and NaN included; rows of no sequence are left as they were.
  * Sums are f32, the weights are rounded to the cache's type for their product

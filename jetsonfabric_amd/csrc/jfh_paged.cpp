@@ -23,6 +23,9 @@ constexpr uint64_t kMaxIndex = 0x7FFFFFFF;
 void check(hipError_t e, const char* what) {
     if (e == hipSuccess) return;
     (void) hipGetLastError();  // it is reported here: the next call's launch is not to find it
+    if (e == hipErrorInvalidConfiguration) {
+        throw jfh::Error(jfh::Status::InvalidArgument, std::string(what) + ": the step takes more threads than a launch holds");
+    }
     throw jfh::Error(jfh::Status::DeviceError, std::string(what) + ": " + hipGetErrorString(e));
 }
 
@@ -52,6 +55,7 @@ paged::Rows rows_of(const jfh_rows* x, const char* name) {
     require(x->n_rows <= kMaxIndex, n + " has more rows than a step can hold");
     require(x->n_head > 0 && x->n_head <= 65536 && x->head_dim > 0 && x->head_dim <= 65536,
             n + " rows have no heads, no values or too many");
+    require(static_cast<uint64_t>(x->n_head) * x->head_dim <= 1U << 24, n + " rows hold too many values");
     require(x->row_stride >= 0 && x->head_stride >= 0, n + " rows have a negative stride");
     require(x->n_rows == 0 || (x->data != nullptr && aligned(x->data, x->type == JFH_VALUE_F32 ? 4 : 2)),
             n + " rows are missing or not aligned to their values");
@@ -151,7 +155,9 @@ paged::Rows attended(const jfh_rows* x, const paged::Cache& c, const char* name)
 
 float score_scale(float scale) {
     require(std::isfinite(scale) && scale > 0.0F, "the score scale must be above 0");
-    return static_cast<float>(static_cast<double>(scale) / std::log(2.0));
+    const float base2 = static_cast<float>(static_cast<double>(scale) / std::log(2.0));
+    require(std::isfinite(base2), "the score scale is too large");
+    return base2;
 }
 
 struct AttendPlan {

@@ -21,6 +21,8 @@ enum : uint32_t { kF32 = 1, kF16 = 2, kBF16 = 3 };
 template <typename... KArgs, typename... Args>
 hipError_t launch(void (*kernel)(KArgs...), dim3 grid, dim3 block, hipStream_t stream, const Args&... args) {
     static_assert((std::is_same_v<KArgs, Args> && ...), "arguments are passed by address");
+    // a launch holds fewer than 2^32 threads
+    if (static_cast<uint64_t>(grid.x) * block.x > 0xFFFFFFFFULL) return hipErrorInvalidConfiguration;
     void* p[] = {const_cast<void*>(static_cast<const void*>(&args))...};
     return hipLaunchKernel(reinterpret_cast<const void*>(kernel), grid, block, p, 0, stream);
 }
@@ -1418,12 +1420,13 @@ __global__ __launch_bounds__(kSelectThreads) void k_evict_select(Evict a) {
         const unsigned long long inside = (1ULL << below) - 1, owned = (1ULL << count) - 1;
         unsigned long long goes = ~stays & inside, comes = stays & owned & ~inside;
         const int2 before = exclusive_sum(int2{__popcll(goes), __popcll(comes)}, waves, &all);
-        for (int n = moves.x + before.x; goes; goes &= goes - 1) list[1 + n++] = t0 + __ffsll(goes) - 1;
-        for (int n = moves.y + before.y; comes; comes &= comes - 1) list[1 + a.width + n++] = t0 + __ffsll(comes) - 1;
+        // the lists hold what a cache that nobody else writes can need
+        for (int n = moves.x + before.x; goes && n < a.width; goes &= goes - 1) list[1 + n++] = t0 + __ffsll(goes) - 1;
+        for (int n = moves.y + before.y; comes && n < a.width; comes &= comes - 1) list[1 + a.width + n++] = t0 + __ffsll(comes) - 1;
         moves.x += all.x;
         moves.y += all.y;
     }
-    if (tid == 0) list[0] = moves.x;
+    if (tid == 0) list[0] = min(min(moves.x, moves.y), a.width);
 }
 
 // 16 threads per moving position: its K and V rows, its weight and its position.

@@ -225,6 +225,9 @@ ATTENDS = [
     ([3], [40], 16, 16, 8, 8, {}),
     ([1], [9000], 4, 1, 72, 1, {}),
     ([20], [65], 3, 1, 256, 16, {}),
+    ([1], [40000], 2, 1, 64, 16, {}),       # more than 64 splits
+    ([40, 3], [9000, 5], 2, 1, 64, 32, {}),  # of tiles
+    ([3], [20000], 8, 1, 128, 64, {}),
 ]
 
 
@@ -305,6 +308,18 @@ def test_attention_of_strided_rows_on_another_stream():
         cache.attend(batch, gpu.unflatten(1, (14, 64))[:, 2:10], 0.125, out=out)
     stream.synchronize()
     within(out.cpu(), want[0], want[2])
+
+
+@pytest.mark.parametrize("rows,length", [(1, 40), (2, 5000), (60, 90), (30, 9000)])
+def test_attention_in_place(rows, length):
+    seq = Sequences([rows], [length], 2, 64, 16, torch.float16, seed=7)
+    q = normal(rows, 8, 64, seed=3).half()
+    want, _, bound, _ = seq.attend(q, 0.125)
+    kp, vp, _, _, table, lengths, starts = seq.to_gpu()
+    gpu = q.cuda()
+    out, _ = jf.PagedCache(kp, vp).attend(jf.PagedBatch(table, lengths, starts, rows, length), gpu, out=gpu)
+    assert out is gpu
+    within(gpu.cpu(), want, bound)
 
 
 # ---------------------------------------------------------------- attention weights
@@ -423,6 +438,31 @@ def test_cut_within_the_budget_changes_nothing():
     seq = Sequences([0, 0], [50, 64], 2, 64, 16, torch.float16, seed=1)
     cut(seq, 64, 4, 8)
     cut(seq, 1000, 4, 8)
+
+
+def test_offsets_beyond_32_bits():
+    """Pages further apart than 2^32 values: every operator on them gives what it gives on neighbouring pages."""
+    far, shape = (1 << 32) + 1024, (3, 2, 16, 64)
+    seq = Sequences([5], [40], 2, 64, 16, torch.float16, seed=3, extra_pages=0)
+    near = seq.to_gpu()
+    pools = [torch.empty(2 * far + 2 * 16 * 64, dtype=torch.float16, device="cuda").as_strided(shape, (far, 1024, 64, 1))
+             for _ in range(2)]
+    for x, y in zip(pools, near):
+        x.copy_(y)
+    rows = normal(5, 12, 64, seed=1).half().cuda()
+    positions = torch.arange(35, 40, dtype=torch.int32, device="cuda")
+    got = []
+    for k, v in (near[:2], pools):
+        w, pos, lengths = near[2].clone(), near[3].clone(), near[5].clone()
+        cache, batch = jf.PagedCache(k, v, w, pos), jf.PagedBatch(near[4], lengths, near[6], 5, 40)
+        cache.append(batch, rows[:, 8:10], rows[:, 10:], positions, jf.Rope(64))
+        out, lse = cache.attend(batch, rows[:, :8])
+        many, _ = cache.attend(batch, rows[:, :8].repeat(1, 5, 1))
+        cache.weigh(batch, rows[:, :8], lse)
+        cache.evict(batch, 20, 2, 4)
+        got.append([out, lse, many, k.contiguous(), v.contiguous(), w, pos, lengths])
+    for x, y in zip(*got):
+        assert torch.equal(x, y)
 
 
 # ---------------------------------------------------------------- together

@@ -70,7 +70,7 @@ def test_batches_are_checked(change, match):
     ({"data": None}, "k rows are missing"), ({"data": AT + 1}, "aligned"), ({"type": 1, "data": AT + 2}, "aligned"),
     ({"type": 0}, "value type"), ({"type": 4}, "value type"), ({"n_head": 3}, "heads and head dim"),
     ({"head_dim": 32}, "heads and head dim"), ({"n_head": 0}, "no heads"), ({"row_stride": -1}, "negative stride"),
-    ({"n_rows": 4}, "same rows"), ({"n_rows": 1 << 31}, "more rows")])
+    ({"n_rows": 4}, "same rows"), ({"n_rows": 1 << 31}, "more rows"), ({"n_head": 65536, "head_dim": 512}, "too many values")])
 def test_appended_rows_are_checked(change, match):
     refused(lambda: _append(k=rows(**change)), match)
 
@@ -108,7 +108,7 @@ def test_attention_rows_are_checked(change, match):
 
 
 def test_attention_arguments_are_checked():
-    for scale in (0.0, -1.0, float("nan"), float("inf")):
+    for scale in (0.0, -1.0, float("nan"), float("inf"), 3e38):
         refused(lambda: _attend(scale=scale), "score scale")
     refused(lambda: _attend(lse=AT + 2), "lse")
     long = {"b": batch(n_seq=1, table_stride=4096, max_length=65536), "c": cache(page_size=16)}
@@ -254,3 +254,15 @@ def test_tensors_are_checked():
     with pytest.raises(ValueError, match="GPU"):
         jf.PagedBatch(torch.zeros(1, 4, dtype=torch.int32), torch.zeros(1, dtype=torch.int32),
                       torch.zeros(2, dtype=torch.int32), 1, 64)
+
+
+def test_calls_without_a_gpu_are_device_errors():
+    import torch
+
+    if torch.cuda.is_available():
+        pytest.skip("a GPU is present")
+    calls = [_append, _attend, _weigh, _evict, lambda: _rotate(rows(), rows(data=AT + 4096))]
+    for call in calls:
+        with pytest.raises(jf.JfhError) as e:
+            check(call())
+        assert e.value.code == 6
