@@ -1377,10 +1377,14 @@ __global__ __launch_bounds__(kSelectThreads) void k_evict_select(Evict a) {
         const uint32_t digit = shift ? 2047U : 1023U;
         for (int e = tid; e < kSelectBins; e += kSelectThreads) bins[e] = 0;
         __syncthreads();
-#pragma unroll 4
-        for (int t = tid; t < len; t += kSelectThreads) {
-            const uint32_t k = key_at(t);
+        const auto count = [&](uint32_t k) {
             if ((k & mask) == prefix) atomicAdd(&bins[k >> shift & digit], 1U);
+        };
+        if (len <= CAP) {
+#pragma unroll 8
+            for (int t = tid; t < len; t += kSelectThreads) count(keys[t]);
+        } else {
+            for (int t = tid; t < len; t += kSelectThreads) count(key_at(t));
         }
         __syncthreads();
         // thread l has bins 2047 - 2 l and 2046 - 2 l: those of larger keys come first
@@ -1406,11 +1410,15 @@ __global__ __launch_bounds__(kSelectThreads) void k_evict_select(Evict a) {
         const int run = ((upto + kSelectThreads - 1) / kSelectThreads) | 1;
         const int t0 = round + min(tid * run, upto), count = min(run, round + upto - t0);
         unsigned long long larger = 0, equal = 0;
-#pragma unroll 8
-        for (int e = 0; e < count; ++e) {
-            const uint32_t k = key_at(t0 + e);
+        const auto compare = [&](int e, uint32_t k) {
             larger |= static_cast<unsigned long long>(k > prefix) << e;
             equal |= static_cast<unsigned long long>(k == prefix) << e;
+        };
+        if (len <= CAP) {
+#pragma unroll 8
+            for (int e = 0; e < count; ++e) compare(e, keys[t0 + e]);
+        } else {
+            for (int e = 0; e < count; ++e) compare(e, key_at(t0 + e));
         }
         int room = need - equals - exclusive_sum(int2{__popcll(equal), 0}, waves, &all).x;
         equals += all.x;
