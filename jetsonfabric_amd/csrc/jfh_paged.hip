@@ -877,8 +877,8 @@ __global__ __launch_bounds__(kAttendThreads, HDP <= 128 ? 2 : 1) void k_attend_t
                 o[e] = V::mfma(__builtin_bit_cast(v8, v), p[c / 2][c % 2], o[e]);
             }
         }
-        if (hidden && (odd[b][0] || odd[b][1] || odd[b][2] || odd[b][3])) {
-            // what the tile's V has of infinities and NaN, staged as 0, for the queries that see them
+        if (base + KT > group_least && (odd[b][0] || odd[b][1] || odd[b][2] || odd[b][3])) {
+            // what the tile's V has of infinities and NaN, staged as 0 for all waves, for the queries that see them
             unsigned long long seen = 0;
             for (int k = 0; k < KT; ++k) {
                 const int key = 16 * (k / 16) + 8 * (k % 8 / 4) + 4 * (k / 8 % 2) + k % 4;

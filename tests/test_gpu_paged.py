@@ -271,6 +271,29 @@ def test_attention_does_not_take_hidden_infinities(kind, rows):
     assert torch.isnan(lse[4:]).all() and torch.isfinite(lse[:4]).all()
 
 
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("heads,rows,length", [(1, 200, 200), (1, 150, 333), (4, 130, 130)])
+def test_attention_takes_the_infinities_that_it_sees(heads, rows, length, dim):
+    """Rows far behind an infinite V, which see all of its tile, have it as the rows near it do."""
+    seq = Sequences([rows], [length], 1, dim, 16, torch.float16, seed=4)
+    q = normal(rows, heads, dim, seed=5).half()
+    want, _, bound, _ = seq.attend(q, 0.05)
+    odd = {3: (length - rows + 5, float("inf")), 9: (length - rows + 70, -float("inf")), 11: (length - rows + 100, float("nan"))}
+    for column, (t, x) in odd.items():
+        at = seq.slot(0, t)
+        seq.v[at[0], 0, at[1], column] = x
+    kp, vp, _, _, table, lengths, starts = seq.to_gpu()
+    out, _ = jf.PagedCache(kp, vp).attend(jf.PagedBatch(table, lengths, starts, rows, length), q.cuda(), 0.05)
+    out = out.cpu()
+    plain = [c for c in range(dim) if c not in odd]
+    within(out[..., plain], want[..., plain], bound[..., plain])
+    for column, (t, x) in odd.items():
+        first = t - (length - rows)
+        within(out[:first, :, column], want[:first, :, column], bound[:first, :, column])
+        left = out[first:, :, column]
+        assert torch.isnan(left).all() if x != x else (left == x).all()
+
+
 def test_attention_of_infinite_queries_and_scores():
     seq = Sequences([3, 1], [40, 50], 1, 64, 16, torch.float16, seed=1)
     q = normal(4, 2, 64, seed=2).half()
