@@ -149,7 +149,7 @@ paged::Rows attended(const jfh_rows* x, const paged::Cache& c, const char* name)
     require(r.heads % c.n_head_kv == 0, n + "'s heads must be a multiple of the cache's");
     require(aligned(r.data, 16) && r.row_stride % 8 == 0 && r.head_stride % 8 == 0,
             n + " must be 16-byte aligned, with strides in multiples of 8 values");
-    require(static_cast<uint64_t>(r.rows) * r.heads <= kMaxIndex, n + " has more rows than a step can hold");
+    require(static_cast<uint64_t>(r.rows) * r.heads <= kMaxIndex / 2, n + " has more rows than a step can hold");
     return r;
 }
 

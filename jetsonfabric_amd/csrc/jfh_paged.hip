@@ -302,9 +302,6 @@ __device__ __forceinline__ float split_share(float m, float l, float now) {
     return l == 0.0F ? 0.0F : m == -INFINITY ? 1.0F : exp2f(m - now);
 }
 
-constexpr int kAttendThreads = 256;
-constexpr int kAttendWaves = 4;
-constexpr int kFewKeys = 32;    // keys of a wave's tile
 constexpr float kRescale = 8.0F;  // a row's running maximum is raised when a tile exceeds it by this (base 2)
 
 // Eight values of a row from column d, 0 from column dim on.
@@ -338,6 +335,7 @@ __device__ __forceinline__ Query query_of(int m, int group, uint32_t kv_head) {
 // the output), its sum is not. A row's maximum is raised only when a tile exceeds it by 2^8: P stays far below 65504.
 // Eight rows of 40 heads over 4087 to 32701 positions, bf16: 108 us and 5 for the join, 5.4 TB/s of K and V; one row over
 // 257: 11.7 us, the latency of its dependent loads.
+constexpr int kFewKeys = 32;  // keys of a wave's tile
 template <int HDP> constexpr int kFewWaves = HDP <= 128 ? 8 : 4;
 
 template <typename T, int HDP, int MT>
@@ -650,16 +648,18 @@ __global__ __launch_bounds__(64 * kFewWaves<HDP>) void k_attend_few(Attend a, in
 // its lane. V goes to LDS transposed, in pieces of 8 keys in the same order (16-bit permutes on the way), so both
 // operands are 16-byte LDS reads. A row of LDS is one piece longer than its values, so that lanes on consecutive rows spread
 // over the banks, and every read of a tile has one address register and an immediate. Block e of O^T has columns HB n + e
-// (HB blocks), whose rows in LDS follow one another. LDS reads set the bound: 32 queries per wave need a byte of LDS for 16
-// operations, the matrix cores' rate at the LDS's.
+// (HB blocks), whose rows in LDS follow one another. 32 queries per wave need a byte of LDS for 16 operations, which the
+// LDS gives at the matrix cores' rate; 64 would need half, and twice the registers.
 // Statistics and rounding as in k_attend_few. 2048 rows of 28 heads over 8192 positions of 4 K/V heads of 128 values, f16:
 // 270 us, 780 TFLOP/s; products and the softmax's instructions share the time, 36 % and 45 % of a SIMD's cycles.
-constexpr int kTileQueries = 128;
+constexpr int kTileThreads = 256;
+constexpr int kTileWaves = kTileThreads / 64;
+constexpr int kTileQueries = 32 * kTileWaves;
 
 template <int HDP> constexpr int kTileKeys = HDP <= 128 ? 64 : 32;
 
 template <typename T, int HDP>
-__global__ __launch_bounds__(kAttendThreads, HDP <= 128 ? 2 : 1) void k_attend_tile(Attend a, int group) {
+__global__ __launch_bounds__(kTileThreads, HDP <= 128 ? 2 : 1) void k_attend_tile(Attend a, int group) {
     using V = Values<T>;
     using v8 = typename V::v8;
     constexpr int KT = kTileKeys<HDP>;
@@ -667,11 +667,11 @@ __global__ __launch_bounds__(kAttendThreads, HDP <= 128 ? 2 : 1) void k_attend_t
     constexpr int KC = HDP / 16;    // products per block of S^T
     constexpr int HB = HDP / 32;    // column blocks of O^T
     constexpr int CH = HDP / 8;     // pieces of a K row
-    constexpr int KP = KT * CH / kAttendThreads;  // pieces of K per thread
+    constexpr int KP = KT * CH / kTileThreads;  // pieces of K per thread
     constexpr int VG = KT / 8;      // pieces of a V column
     constexpr int V4 = HDP / 4;     // threads per piece row: four columns each
     constexpr int VT = VG * V4;     // threads that stage V
-    static_assert(VT <= kAttendThreads && KT <= 64 && kAttendThreads % CH == 0);
+    static_assert(VT <= kTileThreads && KT <= 64 && kTileThreads % CH == 0);
     constexpr unsigned long long kAllKeys = ~0ULL >> (64 - KT);
     constexpr int KS = CH + 1, VS = VG + 1;  // pieces of a row in LDS
     __shared__ uint4 k_lds[2][KT * KS];
@@ -680,7 +680,7 @@ __global__ __launch_bounds__(kAttendThreads, HDP <= 128 ? 2 : 1) void k_attend_t
     __shared__ unsigned long long there[3];
     // of tiles that some query does not see whole: the keys (bits) whose V is +inf, -inf, NaN, by column and piece
     __shared__ alignas(8) uint8_t marks[2][3][HDP][8];
-    __shared__ bool odd[2][kAttendWaves];
+    __shared__ bool odd[2][kTileWaves];
 
     const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64;
     const int n = lane % 32, g = lane / 32;
@@ -740,9 +740,9 @@ __global__ __launch_bounds__(kAttendThreads, HDP <= 128 ? 2 : 1) void k_attend_t
         const int64_t* at = offsets[t % 3];
 #pragma unroll
         for (int p = 0; p < KP; ++p) {
-            kr[p] = *reinterpret_cast<const uint4*>(k_from + at[(tid + kAttendThreads * p) / CH]);
+            kr[p] = *reinterpret_cast<const uint4*>(k_from + at[(tid + kTileThreads * p) / CH]);
         }
-        if (VT == kAttendThreads || tid < VT) {
+        if (VT == kTileThreads || tid < VT) {
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
                 vr[j] = *reinterpret_cast<const uint2*>(v_from + at[16 * (v_piece / 2) + 8 * (j / 4) + 4 * (v_piece % 2) + j % 4]);
@@ -754,10 +754,10 @@ __global__ __launch_bounds__(kAttendThreads, HDP <= 128 ? 2 : 1) void k_attend_t
 #pragma unroll
         for (int p = 0; p < KP; ++p) {
             if (k_at >= dim) kr[p] = uint4{0, 0, 0, 0};
-            k_lds[b][(tid + kAttendThreads * p) / CH * KS + tid % CH] = kr[p];
+            k_lds[b][(tid + kTileThreads * p) / CH * KS + tid % CH] = kr[p];
         }
         bool any = false;
-        if (VT == kAttendThreads || tid < VT) {
+        if (VT == kTileThreads || tid < VT) {
             const unsigned long long present = there[t % 3];
             if (present != kAllKeys || v_at >= dim) {  // what is not there must be a number: its weight is 0
 #pragma unroll
@@ -1345,7 +1345,10 @@ __global__ __launch_bounds__(kSelectThreads) void k_evict_select(Evict a) {
             float w[BATCH];
             if (kStay && t0 == tid) {
 #pragma unroll
-                for (int e = 0; e < BATCH; ++e) at[e] = first_at[e % (kStay ? BATCH : 1)], p[e] = first_p[e % (kStay ? BATCH : 1)], w[e] = first_w[e % (kStay ? BATCH : 1)];
+                for (int e = 0; e < BATCH; ++e) {
+                    const int f = kStay ? e : 0;
+                    at[e] = first_at[f], p[e] = first_p[f], w[e] = first_w[f];
+                }
             } else {
                 look_up(t0, at);
 #pragma unroll
@@ -1525,7 +1528,6 @@ namespace {
 uint32_t few_queries(const Cache& c, const Batch& b) {
     return c.head_dim <= 128 && static_cast<uint64_t>(c.n_head_kv) * b.n_seq * b.max_length >= (1U << 19) ? 32 : 16;
 }
-constexpr uint32_t kFewQueries = 64;  // up to which a wave that adds up weights has slots of its own
 
 // How a step's attention is divided: by the most queries that a sequence may have.
 struct Tiling {
@@ -1555,7 +1557,7 @@ hipError_t attend_of(const Attend& a, hipStream_t stream) {
     const uint64_t groups = t.groups * a.splits;
     if (groups > 0x7FFFFFFF) return hipErrorInvalidConfiguration;
     const dim3 grid(static_cast<uint32_t>(groups)), few(64 * kFewWaves<HDP>);
-    if (t.queries == kTileQueries) return launch(k_attend_tile<T, HDP>, grid, dim3(kAttendThreads), stream, a, group);
+    if (t.queries == kTileQueries) return launch(k_attend_tile<T, HDP>, grid, dim3(kTileThreads), stream, a, group);
     if constexpr (HDP <= 128) {
         if (t.queries == 32) return launch(k_attend_few<T, HDP, 2>, grid, few, stream, a, group);
     }
@@ -1577,15 +1579,17 @@ uint32_t attend_splits(const Cache& c, const Batch& b, uint32_t group) {
     // Rounds of keys in a row set the time, counted in halves: a work-group's beginning and end take about three halves,
     // the join four (of 256 keys; eight of a tile's 64). Work-groups that run at once: one per compute unit of the
     // few-query form, two of the tiles. No splits, or so many as fill the chip once, or, of long few-query calls, twice
-    // where that costs little, and 128 at most, for the join: the second rounds even out sequences of different lengths (eight rows over up to 32701
-    // positions 113 us, 140 in one round; 32 K/V heads of sequences of 4000, equal: 22 in one, 29 in two short ones).
+    // where that costs little, and 128 at most, for the join: the second rounds even out sequences of different lengths
+    // (eight rows over up to 32701 positions 113 us, 140 in one round; 32 K/V heads of sequences of 4000, equal: 22 in
+    // one, 29 in two short ones).
     const bool few = t.queries != kTileQueries;
     const uint64_t resident = few ? kComputeUnits : 2 * kComputeUnits, least = t.queries <= 16 ? 1 : 2;
     if (t.groups >= resident) return 1;
     const uint64_t rounds = (b.max_length + t.keys - 1) / t.keys;
     uint64_t best = 1, cost = 2 * rounds + 3;
     for (uint64_t fill = 1; fill <= (few ? 2 : 1); ++fill) {
-        const uint64_t fills = fill * resident / t.groups, wanted = fills < 128 ? fills : 128, even = (rounds + wanted - 1) / wanted, per = even > least ? even : least;
+        const uint64_t fills = fill * resident / t.groups, wanted = fills < 128 ? fills : 128;
+        const uint64_t even = (rounds + wanted - 1) / wanted, per = even > least ? even : least;
         const uint64_t splits = (rounds + per - 1) / per, turns = (t.groups * splits + resident - 1) / resident;
         const uint64_t takes = turns * (2 * per + 3) + (few ? 4 : 8);
         if (splits > 1 && (takes < cost || (best > 1 && per >= 8 && 10 * takes <= 11 * cost))) best = splits, cost = takes;
@@ -1607,6 +1611,10 @@ hipError_t launch_attend(const Attend& a, hipStream_t stream) {
 
 namespace {
 
+// Queries of a sequence and K/V head up to which a wave that adds up weights has slots of its own: four tiles of 16, which
+// it reads beside its K rows.
+constexpr uint32_t kFewWeighed = 64;
+
 // How a step's weights are divided: by the most queries that a sequence may have.
 struct WeighTiling {
     bool few;
@@ -1616,7 +1624,7 @@ struct WeighTiling {
 
 WeighTiling weigh_tiling(const Cache& c, const Batch& b, uint32_t group) {
     WeighTiling t;
-    t.few = static_cast<uint64_t>(b.max_rows) * group <= kFewQueries;
+    t.few = static_cast<uint64_t>(b.max_rows) * group <= kFewWeighed;
     const uint32_t slots = kWeighWaves * (t.few ? kFewWeighSlots : 16 * (c.head_dim <= 128 ? kWeighTiles<128> : kWeighTiles<256>));
     t.blocks = static_cast<int>((b.max_length + slots - 1) / slots);
     t.groups = static_cast<uint64_t>(t.blocks) * c.n_head_kv * b.n_seq;
@@ -1645,7 +1653,7 @@ hipError_t weigh(const Weigh& a, hipStream_t stream) {
 uint32_t weigh_splits(const Cache& c, const Batch& b, uint32_t group) {
     const WeighTiling t = weigh_tiling(c, b, group);
     if (t.few || t.groups == 0) return 1;
-    // two work-groups per compute unit, of eight tiles of 32 queries at least
+    // two work-groups per compute unit, of four tiles of 64 queries at least
     const uint64_t wanted = (2 * kComputeUnits + t.groups - 1) / t.groups, most = static_cast<uint64_t>(b.max_rows) * group / 256;
     return static_cast<uint32_t>(wanted < most ? wanted : most > 0 ? most : 1);
 }
@@ -1664,7 +1672,9 @@ hipError_t launch_evict(const Evict& a, hipStream_t stream) {
     const int chunks = (a.width + kMoveSlots - 1) / kMoveSlots;
     if (pairs * static_cast<uint64_t>(chunks) > 0x7FFFFFFF) return hipErrorInvalidConfiguration;
     // the larger LDS takes a compute unit for one work-group
-    const hipError_t e = launch(a.batch.max_length <= kSelectFew ? k_evict_select<kSelectFew, 8> : k_evict_select<kSelectMany, 16>, dim3(static_cast<uint32_t>(pairs)), dim3(kSelectThreads), stream, a);
+    const bool few = a.batch.max_length <= kSelectFew;
+    const hipError_t e = launch(few ? k_evict_select<kSelectFew, 8> : k_evict_select<kSelectMany, 16>,
+                                dim3(static_cast<uint32_t>(pairs)), dim3(kSelectThreads), stream, a);
     if (e != hipSuccess) return e;
     return launch(k_evict_move, dim3(static_cast<uint32_t>(pairs) * chunks), dim3(kMoveThreads), stream, a, chunks);
 }

@@ -271,6 +271,30 @@ def test_attention_does_not_take_hidden_infinities(kind, rows):
     assert torch.isnan(lse[4:]).all() and torch.isfinite(lse[:4]).all()
 
 
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("rows,lens,dim", [([5, 6], [700, 7], 64), ([5, 8], [3000, 4100], 128), ([1, 5], [40, 3], 96), ([7, 0], [7, 1], 128)])
+def test_attention_with_room_for_long_sequences(rows, lens, dim, kind):
+    """Tables and bounds for many more positions than there are: 4 to 32 queries per K/V head, infinities of V that some
+    rows do not see."""
+    seq = Sequences(rows, lens, 4, dim, 16, TYPES[kind], seed=6).poison()
+    q = normal(seq.total, 16, dim, seed=7).to(seq.dtype)
+    want, want_lse, bound, lse_bound = seq.attend(q, 0.1)
+    at = seq.slot(0, lens[0] - rows[0] // 2 - 1)  # the last rows // 2 + 1 rows see it
+    seq.v[at[0], 2, at[1], 5] = float("inf")
+    kp, vp, _, _, table, lengths, starts = seq.to_gpu()
+    table = torch.cat([table, torch.full((2, 5000), -1, dtype=torch.int32, device="cuda")], 1)
+    batch = jf.PagedBatch(table, lengths, starts, max(rows), table.shape[1] * 16)
+    out, lse = jf.PagedCache(kp, vp).attend(batch, q.cuda(), 0.1)
+    out, lse = out.cpu(), lse.cpu()
+    struck = torch.zeros(out.shape, dtype=torch.bool)
+    struck[rows[0] - rows[0] // 2 - 1:rows[0], 8:12, 5] = True
+    assert (out[struck] == float("inf")).all()
+    within(out[~struck], want[~struck], bound[~struck])
+    some = want_lse > -float("inf")
+    assert torch.equal(lse[~some], want_lse[~some].float())
+    within(lse[some], want_lse[some], lse_bound[some])
+
+
 @pytest.mark.parametrize("dim", [64, 128, 256])
 @pytest.mark.parametrize("heads,rows,length", [(1, 200, 200), (1, 150, 333), (4, 130, 130)])
 def test_attention_takes_the_infinities_that_it_sees(heads, rows, length, dim):
