@@ -57,8 +57,16 @@ def _torch():
     return sys.modules["torch"]  # there once the caller has a tensor
 
 
+_current = None  # device -> address of torch's current stream
+
+
 def _stream(device: int) -> int:
-    return _torch().cuda.current_stream(device).cuda_stream
+    global _current
+    if _current is None:
+        # without the Stream object around it, which takes longer than the rest of a small call's checks
+        _current = getattr(_torch()._C, "_cuda_getCurrentRawStream", None) or (
+            lambda d: _torch().cuda.current_stream(d).cuda_stream)
+    return _current(device)
 
 
 class Rope:
