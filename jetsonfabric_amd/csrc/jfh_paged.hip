@@ -55,24 +55,30 @@ __device__ __forceinline__ void load(const void* data, int64_t at, uint32_t type
     }
 }
 
-// The one rounding to the output's type, to nearest.
-template <int N>
+template <bool PAST, typename V>
+__device__ __forceinline__ void put(V* to, V v) {
+    if constexpr (PAST) __builtin_nontemporal_store(v, to);
+    else *to = v;
+}
+
+// The one rounding to the output's type, to nearest. PAST: past the caches, for rows that they could not hold.
+template <int N, bool PAST = false>
 __device__ __forceinline__ void store(void* data, int64_t at, uint32_t type, const float (&x)[N]) {
     if constexpr (N == 8) {
         if (type == kF32) {
             float4v* p = reinterpret_cast<float4v*>(static_cast<float*>(data) + at);
-            p[0] = float4v{x[0], x[1], x[2], x[3]};
-            p[1] = float4v{x[4], x[5], x[6], x[7]};
+            put<PAST>(p, float4v{x[0], x[1], x[2], x[3]});
+            put<PAST>(p + 1, float4v{x[4], x[5], x[6], x[7]});
         } else if (type == kF16) {
             half8 v;
 #pragma unroll
             for (int i = 0; i < 8; ++i) v[i] = static_cast<_Float16>(x[i]);
-            *reinterpret_cast<half8*>(static_cast<_Float16*>(data) + at) = v;
+            put<PAST>(reinterpret_cast<half8*>(static_cast<_Float16*>(data) + at), v);
         } else {
             bhalf8 v;
 #pragma unroll
             for (int i = 0; i < 8; ++i) v[i] = static_cast<__bf16>(x[i]);
-            *reinterpret_cast<bhalf8*>(static_cast<__bf16*>(data) + at) = v;
+            put<PAST>(reinterpret_cast<bhalf8*>(static_cast<__bf16*>(data) + at), v);
         }
     } else {
         static_assert(N == 1);
@@ -101,7 +107,7 @@ __device__ __forceinline__ void row_angles(const Rotation& r, const int32_t* __r
 }
 
 // Unit u of a head: N pairs for u < pairs / N, then N values that stay.
-template <int N>
+template <int N, bool PAST>
 __device__ __forceinline__ void rotate_unit(const Rotation& r, const float2* cs, int u, const void* x, int64_t x_at,
                                             uint32_t x_type, void* y, int64_t y_at, uint32_t y_type) {
     const int half = static_cast<int>(r.n_rot / 2);
@@ -132,20 +138,20 @@ __device__ __forceinline__ void rotate_unit(const Rotation& r, const float2* cs,
                 b[i] = p * t[i].y + q * t[i].x;
             }
         }
-        store(y, y_at + lo, y_type, a);
-        store(y, y_at + hi, y_type, b);
+        store<N, PAST>(y, y_at + lo, y_type, a);
+        store<N, PAST>(y, y_at + hi, y_type, b);
     } else {
         const int d = static_cast<int>(r.n_rot) + (u * N - half);
         float a[N];
         load(x, x_at + d, x_type, a);
-        store(y, y_at + d, y_type, a);
+        store<N, PAST>(y, y_at + d, y_type, a);
     }
 }
 
 // Bound by the rows' bytes, one read and one write. A work-group computes the angles of its rows once for all heads;
-// a thread owns a unit, so rows may be rotated in place. 4096 rows of 48 heads of 128 bf16 values: 18 us, 5.6 TB/s; two
+// a thread owns a unit, so rows may be rotated in place. 4096 rows of 48 heads of 128 bf16 values: 17 us, 5.9 TB/s; two
 // rows: 3 us.
-template <int N>
+template <int N, bool PAST>
 __global__ __launch_bounds__(kRotateThreads) void k_rotate(Rotation r, Rows x, const int32_t* __restrict__ positions,
                                                            Rows y, int rows_per_group) {
     __shared__ float2 cs[kRotateRows][kMaxRotPairs];
@@ -159,7 +165,7 @@ __global__ __launch_bounds__(kRotateThreads) void k_rotate(Rotation r, Rows x, c
          t += static_cast<int>(gridDim.y) * kRotateThreads) {
         const int row = t / tasks, left = t - row * tasks;
         const int head = left / units, u = left - head * units;
-        rotate_unit<N>(r, cs[row], u, x.data, (row0 + row) * x.row_stride + head * x.head_stride, x.type, y.data,
+        rotate_unit<N, PAST>(r, cs[row], u, x.data, (row0 + row) * x.row_stride + head * x.head_stride, x.type, y.data,
                        (row0 + row) * y.row_stride + head * y.head_stride, y.type);
     }
 }
@@ -197,7 +203,7 @@ __global__ __launch_bounds__(kRotateThreads) void k_append(Rotation r, Cache c, 
         const int64_t at = slot_offset(c, page, slot);
         if (left < heads * ku) {
             const int head = left / ku;
-            rotate_unit<N>(r, cs[row], left - head * ku, k.data, (row0 + row) * k.row_stride + head * k.head_stride,
+            rotate_unit<N, false>(r, cs[row], left - head * ku, k.data, (row0 + row) * k.row_stride + head * k.head_stride,
                            k.type, c.k, at + head * c.head_stride, c.type);
         } else if ((left -= heads * ku) < heads * vu) {
             const int head = left / vu, d = (left - head * vu) * N;
@@ -1489,15 +1495,20 @@ bool by_eights(const Rows& x) {
            x.head_dim % 8 == 0;
 }
 
-// Long steps: four rows per work-group, so that 64 pairs' angles are one per thread. Short ones: one row, its units
-// over up to `tasks` / 256 work-groups, since the call's time is the time of one work-group.
+// Long steps: as many rows per work-group, four at most, as give every thread a unit (4096 rows of 48 heads: 17.1 us with
+// one row, 17.6 with four; 16384 rows 69 and 79). Short ones: one row, its units over up to `tasks` / 256 work-groups, since
+// the call's time is the time of one work-group.
 struct RowGrid {
     dim3 grid;
     int rows;
 };
 
 RowGrid row_grid(uint32_t rows, uint64_t tasks) {
-    if (rows >= kComputeUnits * kRotateRows) return {dim3((rows + kRotateRows - 1) / kRotateRows), kRotateRows};
+    if (rows >= kComputeUnits * kRotateRows) {
+        const uint64_t fit = (kRotateThreads + tasks - 1) / tasks;
+        const uint32_t per = static_cast<uint32_t>(fit < kRotateRows ? fit : kRotateRows);
+        return {dim3((rows + per - 1) / per), static_cast<int>(per)};
+    }
     const uint64_t parts = (tasks + kRotateThreads - 1) / kRotateThreads;
     return {dim3(rows, static_cast<uint32_t>(parts < 64 ? parts : 64)), 1};
 }
@@ -1508,7 +1519,10 @@ hipError_t launch_rotate(const Rotation& r, const Rows& x, const int32_t* positi
     const bool wide = by_eights(x) && by_eights(y) && r.n_rot % 16 == 0;
     const uint64_t units = (r.n_rot / 2 + (x.head_dim - r.n_rot)) / (wide ? 8 : 1);
     const RowGrid g = row_grid(x.rows, x.heads * units);
-    return launch(wide ? k_rotate<8> : k_rotate<1>, g.grid, dim3(kRotateThreads), stream, r, x, positions, y, g.rows);
+    // more than the 32 MB of the L2 caches is written past them: 4096 rows of 48 heads of bf16 values 17 us, 23 through them
+    const bool past = static_cast<uint64_t>(y.rows) * y.heads * y.head_dim * (y.type == kF32 ? 4 : 2) > (32U << 20);
+    return launch(wide ? past ? k_rotate<8, true> : k_rotate<8, false> : k_rotate<1, false>, g.grid, dim3(kRotateThreads),
+                  stream, r, x, positions, y, g.rows);
 }
 
 hipError_t launch_append(const Rotation* rotation, const Cache& c, const Batch& b, const Rows& k, const Rows& v,
