@@ -87,6 +87,23 @@ def test_rotation_in_place_and_of_strided_rows(dtype, layout):
         assert torch.equal(gpu.cpu()[rest], store[rest])
 
 
+@pytest.mark.parametrize("rows,heads,dim,n_rot,dtype", [(1027, 160, 128, 128, "bf16"), (66001, 2, 128, 64, "f16"),
+                                                        (1030, 65, 136, 128, "f32")])
+def test_rotation_of_more_rows_than_the_caches_hold(rows, heads, dim, n_rot, dtype):
+    """Out of place, in place behind it, and back to back with a reader of the result."""
+    t = TYPES[dtype]
+    x = normal(rows, heads, dim, seed=2).to(t)
+    p = torch.randint(0, 1 << 15, (rows,), generator=torch.Generator().manual_seed(2), dtype=torch.int32)
+    assert x.numel() * x.element_size() > 32 << 20
+    want, terms = rotate(x, p, n_rot)
+    bound = rotation_bound(want, terms, t)
+    rope, gx, gp = jf.Rope(n_rot), x.cuda(), p.cuda()
+    got = rope.rotate(gx, gp)
+    rope.rotate(gx, gp, out=gx)
+    assert torch.equal(got, gx)
+    within(got.cpu(), want, bound)
+
+
 def test_rotation_of_no_rows():
     x = torch.zeros(0, 4, 64, device="cuda")
     assert jf.Rope(64).rotate(x, torch.zeros(0, dtype=torch.int32, device="cuda")).shape == (0, 4, 64)
