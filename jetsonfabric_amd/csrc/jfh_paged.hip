@@ -339,7 +339,7 @@ __device__ __forceinline__ Query query_of(int m, int group, uint32_t kv_head) {
 // the product with P, and the pages of the one after it are looked up meanwhile.
 // Running maximum and sum are f32, base 2; P is rounded to the cache's type for the product (half a step per weight, as
 // the output), its sum is not. A row's maximum is raised only when a tile exceeds it by 2^8: P stays far below 65504.
-// Eight rows of 40 heads over 4087 to 32701 positions, bf16: 108 us and 5 for the join, 5.4 TB/s of K and V; one row over
+// Eight rows of 40 heads over 4087 to 32701 positions, bf16: 100 us and 5 for the join, 5.8 TB/s of K and V; one row over
 // 257: 11.7 us, the latency of its dependent loads.
 constexpr int kFewKeys = 32;  // keys of a wave's tile
 template <int HDP> constexpr int kFewWaves = HDP <= 128 ? 8 : 4;
@@ -409,14 +409,20 @@ __global__ __launch_bounds__(64 * kFewWaves<HDP>) void k_attend_few(Attend a, in
             }
         }
     };
-    const auto fetch_v = [&](const Keys& x) {
+    // V is read once, so where a load takes whole rows of 256 bytes it leaves nothing in the caches: eight sequences of
+    // 30000 positions 87 us, 95 through them; of 4000, which stay in the caches from call to call, 22.6 and 22.0. Loads of
+    // parts of rows (K's, and V's of other head dims) lose what the neighbouring loads find there (27.0 and 29.6 us).
+    typedef uint32_t Words __attribute__((ext_vector_type(kChunk)));
+    const auto fetch_v = [&](const Keys& keys) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
-            const T* row = v_head + __shfl(x.at[j / 4], 4 * g + j % 4);
+            const T* row = v_head + __shfl(keys.at[j / 4], 4 * g + j % 4);
 #pragma unroll
             for (int w = 0; w < VW; w += kChunk) {
                 const int d = VEC * i + 2 * w;
-                __builtin_memcpy(&v[j][w], __builtin_assume_aligned(row + (d < dim ? d : 0), 4 * kChunk), 4 * kChunk);
+                const Words* p = reinterpret_cast<const Words*>(row + (d < dim ? d : 0));
+                const Words x = VW == 4 ? __builtin_nontemporal_load(p) : *p;
+                __builtin_memcpy(&v[j][w], &x, sizeof x);
             }
         }
     };
@@ -1538,7 +1544,7 @@ namespace {
 
 // Queries (rows times the heads of a K/V head) of a sequence up to which the waves of a work-group divide its keys: 16,
 // one tile of scores, and 32 where there are so many positions that the bytes of K and V alone count (21 queries, 32 K/V
-// heads of sequences of 30000 positions: 102 us, 116 on tiles; of 4000: 29, 26 on tiles).
+// heads of sequences of 30000 positions: 95 us, 116 on tiles; of 4000: 29, 26 on tiles).
 uint32_t few_queries(const Cache& c, const Batch& b) {
     return c.head_dim <= 128 && static_cast<uint64_t>(c.n_head_kv) * b.n_seq * b.max_length >= (1U << 19) ? 32 : 16;
 }
@@ -1594,7 +1600,7 @@ uint32_t attend_splits(const Cache& c, const Batch& b, uint32_t group) {
     // the join four (of 256 keys; eight of a tile's 64). Work-groups that run at once: one per compute unit of the
     // few-query form, two of the tiles. No splits, or so many as fill the chip once, or, of long few-query calls, twice
     // where that costs little, and 128 at most, for the join: the second rounds even out sequences of different lengths
-    // (eight rows over up to 32701 positions 113 us, 140 in one round; 32 K/V heads of sequences of 4000, equal: 22 in
+    // (eight rows over up to 32701 positions 104 us, 133 in one round; 32 K/V heads of sequences of 4000, equal: 22 in
     // one, 29 in two short ones).
     const bool few = t.queries != kTileQueries;
     const uint64_t resident = few ? kComputeUnits : 2 * kComputeUnits, least = t.queries <= 16 ? 1 : 2;
