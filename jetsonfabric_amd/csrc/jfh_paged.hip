@@ -1598,12 +1598,13 @@ uint32_t attend_splits(const Cache& c, const Batch& b, uint32_t group) {
     if (t.groups == 0) return 1;
     // Rounds of keys in a row set the time, counted in halves: a work-group's beginning and end take about three halves,
     // the join four (of 256 keys; eight of a tile's 64). Work-groups that run at once: one per compute unit of the
-    // few-query form, two of the tiles. No splits, or so many as fill the chip once, or, of long few-query calls, twice
-    // where that costs little, and 128 at most, for the join: the second rounds even out sequences of different lengths
-    // (eight rows over up to 32701 positions 104 us, 133 in one round; 32 K/V heads of sequences of 4000, equal: 22 in
-    // one, 29 in two short ones).
+    // few-query form and of head dims above 128, two of the other tiles (two sequences of 18624 positions, 144 queries of
+    // 256: 43 us in 64 splits, 56 in the 117 of two rounds). No splits, or so many as fill the chip once, or, of long
+    // few-query calls, twice where that costs little, and 128 at most, for the join: the second rounds even out sequences
+    // of different lengths (eight rows over up to 32701 positions 104 us, 133 in one round; 32 K/V heads of sequences of
+    // 4000, equal: 22 in one, 29 in two short ones).
     const bool few = t.queries != kTileQueries;
-    const uint64_t resident = few ? kComputeUnits : 2 * kComputeUnits, least = t.queries <= 16 ? 1 : 2;
+    const uint64_t resident = (few || c.head_dim > 128 ? 1 : 2) * kComputeUnits, least = t.queries <= 16 ? 1 : 2;
     if (t.groups >= resident) return 1;
     const uint64_t rounds = (b.max_length + t.keys - 1) / t.keys;
     uint64_t best = 1, cost = 2 * rounds + 3;
