@@ -224,6 +224,7 @@ template <typename T> struct Values;
 template <> struct Values<_Float16> {
     using v8 = half8;
     static constexpr uint32_t kExponent = 0x7C00;
+    static constexpr float kRaised = 15.0F;  // base-2 logarithm of a row's largest weight
     static __device__ __forceinline__ float4v mfma(v8 a, v8 b, float4v c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
     }
@@ -234,6 +235,7 @@ template <> struct Values<_Float16> {
 template <> struct Values<__bf16> {
     using v8 = bhalf8;
     static constexpr uint32_t kExponent = 0x7F80;
+    static constexpr float kRaised = 0.0F;
     static __device__ __forceinline__ float4v mfma(v8 a, v8 b, float4v c) {
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
     }
@@ -308,7 +310,17 @@ __device__ __forceinline__ float split_share(float m, float l, float now) {
     return l == 0.0F ? 0.0F : m == -INFINITY ? 1.0F : exp2f(m - now);
 }
 
-constexpr float kRescale = 8.0F;  // a row's running maximum is raised when a tile exceeds it by this (base 2)
+// Weights are 2^(score - top), where `top` is a row's running maximum (base 2) less kRaised: the largest one is the power
+// of two 2^kRaised, which no type rounds, and f16 keeps full precision 29 octaves below it and numbers 40 below (from 1
+// on it would be 14 and 25, while long rows of small weights still count). Sums leave a kernel with the factor taken out.
+struct Sums {
+    float top, l, unit;  // maximum, sum of weights, what the sums of V are multiplied by
+};
+template <typename T>
+__device__ __forceinline__ Sums lowered(float top, float l) {
+    constexpr float unit = 1.0F / static_cast<float>(1U << static_cast<int>(Values<T>::kRaised));
+    return Sums{top + Values<T>::kRaised, l * unit, unit};
+}
 
 // Eight values of a row from column d, 0 from column dim on.
 template <typename T>
@@ -338,7 +350,7 @@ __device__ __forceinline__ Query query_of(int m, int group, uint32_t kv_head) {
 // exchange between lanes. No LDS on the way: the next tile's K is requested as soon as the scores are there, its V after
 // the product with P, and the pages of the one after it are looked up meanwhile.
 // Running maximum and sum are f32, base 2; P is rounded to the cache's type for the product (half a step per weight, as
-// the output), its sum is not. A row's maximum is raised only when a tile exceeds it by 2^8: P stays far below 65504.
+// the output), its sum is not.
 // Eight rows of 40 heads over 4087 to 32701 positions, bf16: 100 us and 5 for the join, 5.8 TB/s of K and V; one row over
 // 257: 11.7 us, the latency of its dependent loads.
 constexpr int kFewKeys = 32;  // keys of a wave's tile
@@ -509,8 +521,8 @@ __global__ __launch_bounds__(64 * kFewWaves<HDP>) void k_attend_few(Attend a, in
             most[mt] = sc[mt][0][0];
 #pragma unroll
             for (int j = 1; j < 8; ++j) most[mt] = fmaxf(most[mt], sc[mt][j / 4][j % 4]);
-            most[mt] = groups_max(most[mt]) * a.scale_log2;
-            rise |= most[mt] > top[mt] + kRescale;
+            most[mt] = groups_max(most[mt]) * a.scale_log2 - V::kRaised;
+            rise |= most[mt] > top[mt];
         }
         if (__ballot(rise)) {
 #pragma unroll
@@ -604,7 +616,8 @@ __global__ __launch_bounds__(64 * kFewWaves<HDP>) void k_attend_few(Attend a, in
         if (m0 + 16 * mt >= queries) break;
         __syncthreads();
         const float wave_l = groups_sum(sum[mt]);
-        if (g == 0) part_m[wave][i] = top[mt], part_l[wave][i] = wave_l;
+        const Sums all_seen = lowered<T>(top[mt], wave_l);
+        if (g == 0) part_m[wave][i] = all_seen.top, part_l[wave][i] = all_seen.l;
         // lane (i, g) holds columns VEC (4 g + r) + c of query i
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
@@ -629,7 +642,7 @@ __global__ __launch_bounds__(64 * kFewWaves<HDP>) void k_attend_few(Attend a, in
         }
         const Query q = query_of(m, group, h);
         const int64_t row = span.row0 + q.row, at = row * a.q.heads + q.head;
-        const float scale = !complete ? 1.0F : l == 0.0F ? 0.0F : 1.0F / l;
+        const float scale = all_seen.unit * (!complete ? 1.0F : l == 0.0F ? 0.0F : 1.0F / l);
         for (int d = threadIdx.x % kPer * 8; d < dim; d += 8 * kPer) {
             float x[8];
 #pragma unroll
@@ -861,8 +874,8 @@ __global__ __launch_bounds__(kTileThreads, HDP <= 128 ? 2 : 1) void k_attend_til
 #pragma unroll
             for (int r = 0; r < 16; ++r) most = fmaxf(most, sc[e][r]);
         }
-        most = halves_max(most) * a.scale_log2;
-        if (__ballot(most > top + kRescale)) {
+        most = halves_max(most) * a.scale_log2 - V::kRaised;
+        if (__ballot(most > top)) {
             const float now = fmaxf(top, most);
             const float shrink = now == -INFINITY ? 1.0F : exp2f(top - now);
             top = now;
@@ -914,15 +927,16 @@ __global__ __launch_bounds__(kTileThreads, HDP <= 128 ? 2 : 1) void k_attend_til
     }
 
     if (m >= queries) return;
-    const float l = halves_sum(sum);
+    const Sums seen = lowered<T>(top, halves_sum(sum));
+    const float l = seen.l;
     const int64_t at = row * a.q.heads + query.head, all = static_cast<int64_t>(a.q.rows) * a.q.heads;
     const bool whole = a.splits == 1;
     if (g == 0) {
-        if (!whole) *reinterpret_cast<float2*>(a.marks + 2 * (split * all + at)) = float2{top, l};
-        else if (a.lse) a.lse[at] = top * kLn2 + logf(l);
+        if (!whole) *reinterpret_cast<float2*>(a.marks + 2 * (split * all + at)) = float2{seen.top, l};
+        else if (a.lse) a.lse[at] = seen.top * kLn2 + logf(l);
     }
     if (!whole && l == 0.0F) return;  // nothing seen: the join does not read it
-    const float scale = whole ? (l == 0.0F ? 0.0F : 1.0F / l) : 1.0F;
+    const float scale = seen.unit * (whole ? (l == 0.0F ? 0.0F : 1.0F / l) : 1.0F);
     // rows 8 b + 4 g + r of the blocks: 4 HB consecutive columns, four at a time
 #pragma unroll
     for (int b = 0; b < 4; ++b) {

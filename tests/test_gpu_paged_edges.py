@@ -1,0 +1,98 @@
+"""The paged-cache operators on the GPU where single slots, weights or bounds decide: each result against its definition in
+64 bits (tests/paged_forms.py), with bounds relative to the output."""
+from __future__ import annotations
+
+import math
+
+import pytest
+import torch
+
+import jetsonfabric_amd as jf
+from tests.paged_forms import TYPES, Sequences, half_step
+
+pytestmark = pytest.mark.gpu
+
+
+def normal(*size, seed=0, std=1.0):
+    return torch.randn(*size, generator=torch.Generator().manual_seed(seed)) * std
+
+
+def put(seq, s, t, k=None, v=None, at=slice(None)):
+    """Sets K or V of a sequence's slot (every K/V head, columns `at`)."""
+    page, i = seq.slot(s, t)
+    if k is not None:
+        seq.k[page, :, i, at] = torch.as_tensor(k, dtype=seq.dtype)
+    if v is not None:
+        seq.v[page, :, i, at] = torch.as_tensor(v, dtype=seq.dtype)
+
+
+def attend(seq, q, scale, causal=True, max_length=0):
+    kp, vp, _, _, table, lengths, starts = seq.to_gpu()
+    batch = jf.PagedBatch(table, lengths, starts, seq.max_rows, max_length or seq.max_length)
+    out, lse = jf.PagedCache(kp, vp).attend(batch, q.cuda(), scale, causal)
+    return out.cpu(), lse.cpu()
+
+
+# rows, heads of the one K/V head, slots: few queries in one part and in many, tiles in one part and in many
+FORMS = [(1, 2, 700), (2, 4, 6000), (1, 1, 40000), (40, 2, 700), (40, 2, 6000), (300, 1, 3000)]
+
+
+@pytest.mark.parametrize("rows,heads,length", FORMS)
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("bits", [20, 24, 28])
+def test_a_heavy_slot_does_not_take_the_others_weight(rows, heads, length, kind, bits):
+    """One early slot with V = 0 and 2^bits times the weight of each other: the output is the others' alone."""
+    seq = Sequences([rows], [length], 1, 64, 16, TYPES[kind], seed=bits)
+    seq.k.zero_()
+    seq.v = (torch.rand(seq.v.shape, generator=torch.Generator().manual_seed(1)) * 64 + 32).to(seq.dtype)
+    less = bits + torch.rand(seq.k.shape[:3], generator=torch.Generator().manual_seed(2))
+    seq.k[..., 0] = (4.0 - less / 4.0).to(seq.dtype)
+    put(seq, 0, 3, k=4.0, v=0.0)
+    put(seq, 0, 3, k=0.0, at=slice(1, 64))
+    q = torch.zeros(rows, heads, 64, dtype=seq.dtype)
+    q[..., 0] = 4.0
+    scale = math.log(2.0)
+    want, want_lse, _, _ = seq.attend(q, scale)
+    out, lse = attend(seq, q, scale)
+    # All terms are positive. Weights are 29 octaves below the largest at most, where either type has its full precision: a
+    # half step each, and one of the output; scores of up to 33 in base 2 (2^-24 of it each for product, scale and
+    # difference, 7e-6 of the weight), and f32 sums of 40000 / 256 terms a lane and fewer than 2^8 parts (2^-24 each, 3e-5).
+    off = ((out.double() - want) / want).abs().max().item()
+    assert off <= 2 * half_step(seq.dtype) + 5e-5, off
+    assert (lse.double() - want_lse).abs().max() <= 1e-5
+
+
+@pytest.mark.parametrize("rows,heads,length", FORMS)
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+def test_a_slot_that_takes_all_weight_gives_its_value(rows, heads, length, kind):
+    """The other slots' weights are below 2^-60 together: the output is V of the one, to the bit."""
+    for slot in (0, length - rows, (length - rows) // 2 + 1):
+        seq = Sequences([rows], [length], 1, 64, 16, TYPES[kind], seed=slot)
+        seq.k *= 0.01
+        put(seq, 0, slot, k=normal(64, seed=slot + 1, std=3.0))
+        page, i = seq.slot(0, slot)
+        q = (seq.k[page, 0, i].float() + normal(rows, heads, 64, seed=2, std=0.3)).to(seq.dtype)
+        out, _ = attend(seq, q, 0.25)
+        assert torch.equal(out, seq.v[page, 0, i].expand_as(out))
+
+
+@pytest.mark.parametrize("rows,heads,length", FORMS)
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("bits", [0.3, 3.4, 7.6])
+def test_the_heaviest_weight_is_not_rounded(rows, heads, length, kind, bits):
+    """Behind many slots with V = 0 comes one of 2^bits times their weight: its value over the sum of weights, rounded once."""
+    seq = Sequences([rows], [length], 1, 64, 16, TYPES[kind], seed=5)
+    heavy = length - rows
+    seq.k.zero_()
+    seq.v.zero_()
+    seq.k[..., 0] = 4.0 - bits / 8.0
+    put(seq, 0, heavy, k=4.0, v=normal(64, seed=3))
+    put(seq, 0, heavy, k=0.0, at=slice(1, 64))
+    q = torch.zeros(rows, heads, 64, dtype=seq.dtype)
+    q[..., 0] = 8.0
+    want, _, _, _ = seq.attend(q, math.log(2.0))
+    out, _ = attend(seq, q, math.log(2.0))
+    # one rounding, scores of up to 32 (2^-24 of it each for product, scale and difference), f32 sums as above
+    off = (out.double() - want).abs()
+    bound = (half_step(seq.dtype) + 5e-5) * want.abs() + torch.finfo(seq.dtype).tiny * torch.finfo(seq.dtype).eps
+    assert (off <= bound).all(), (off / want.abs()).nan_to_num().max().item()
