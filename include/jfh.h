@@ -509,8 +509,10 @@ jfh_status jfh_paged_append(const jfh_paged_cache * cache, const jfh_paged_batch
  * be q itself, and overlaps it in no other way. A row
  * that sees nothing gives 0 and -inf; what a row does not see does not reach
  * it, infinities and NaN included; rows of no sequence are left as they were.
- * Sums are f32, the weights are rounded to the cache's type for their product
- * with V. workspace: workspace_bytes of device memory, 16-byte aligned, at
+ * Sums are f32. For up to 16 queries per K/V head (rows of a sequence times
+ * heads of a K/V head, by max_rows; up to 32 of long caches) the weights keep
+ * twice the bits of the cache's type in their product with V, for more they are
+ * rounded to the cache's type. workspace: workspace_bytes of device memory, 16-byte aligned, at
  * least what jfh_paged_attention_workspace says for the same batch and q (0
  * where the step needs none); a call in flight, or a captured one, needs its
  * own. */

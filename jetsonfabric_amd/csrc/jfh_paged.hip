@@ -349,8 +349,10 @@ __device__ __forceinline__ Query query_of(int m, int group, uint32_t kv_head) {
 // c-th of columns VEC i + c. The keys of lane group g are those whose scores the group holds after S^T, so P needs no
 // exchange between lanes. No LDS on the way: the next tile's K is requested as soon as the scores are there, its V after
 // the product with P, and the pages of the one after it are looked up meanwhile.
-// Running maximum and sum are f32, base 2; P is rounded to the cache's type for the product (half a step per weight, as
-// the output), its sum is not.
+// Running maximum and sum are f32, base 2. P goes to its product as two values of the cache's type, the second what the
+// rounding of the first left, so that the one rounding that counts is the output's: the bytes bound the call, and the
+// second product costs it 0 to 2 % (eight rows over up to 32701 positions, bf16: 104 us, error against 64 bits 1.66e-3,
+// with P rounded once 104 us and 1.77e-3; head dim 64, f16, 30000: 37.3 us and 2.03e-4, 36.6 and 2.18e-4).
 // Eight rows of 40 heads over 4087 to 32701 positions, bf16: 100 us and 5 for the join, 5.8 TB/s of K and V; one row over
 // 257: 11.7 us, the latency of its dependent loads.
 constexpr int kFewKeys = 32;  // keys of a wave's tile
@@ -535,7 +537,7 @@ __global__ __launch_bounds__(64 * kFewWaves<HDP>) void k_attend_few(Attend a, in
                 for (int c = 0; c < VEC; ++c) o[mt][c] *= shrink;
             }
         }
-        v8 p[MT];
+        v8 p[MT], rest[MT];  // weights, what their rounding left
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) {
             const float ref = top[mt] == -INFINITY ? 0.0F : top[mt];
@@ -544,6 +546,7 @@ __global__ __launch_bounds__(64 * kFewWaves<HDP>) void k_attend_few(Attend a, in
                 const float w = __builtin_amdgcn_exp2f(fmaf(sc[mt][j / 4][j % 4], a.scale_log2, -ref));
                 sum[mt] += w;
                 p[mt][j] = static_cast<T>(w);
+                rest[mt][j] = static_cast<T>(w - static_cast<float>(p[mt][j]));
             }
         }
         if (!whole || dim < HDP) {  // what is not there must be a number: its weight is 0
@@ -580,7 +583,7 @@ __global__ __launch_bounds__(64 * kFewWaves<HDP>) void k_attend_few(Attend a, in
         for (int c = 0; c < VEC; ++c) {
             const v8 x = __builtin_bit_cast(v8, column<VW>(v, c));
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt) o[mt][c] = V::mfma(x, p[mt], o[mt][c]);
+            for (int mt = 0; mt < MT; ++mt) o[mt][c] = V::mfma(x, rest[mt], V::mfma(x, p[mt], o[mt][c]));
         }
         if (any_odd) {
             asm volatile("" ::: "memory");
@@ -675,7 +678,10 @@ __global__ __launch_bounds__(64 * kFewWaves<HDP>) void k_attend_few(Attend a, in
 // over the banks, and every read of a tile has one address register and an immediate. Block e of O^T has columns HB n + e
 // (HB blocks), whose rows in LDS follow one another. 32 queries per wave need a byte of LDS for 16 operations, which the
 // LDS gives at the matrix cores' rate; 64 would need half, and twice the registers.
-// Statistics and rounding as in k_attend_few. 2048 rows of 28 heads over 8192 positions of 4 K/V heads of 128 values, f16:
+// Statistics as in k_attend_few. P is rounded to the cache's type once, half a step per weight: the products bound this
+// form, and a second one for what the rounding leaves takes 2048 rows over 8192 positions of 7B heads from 280 to 368 us
+// (f16: error against 64 bits 2.5e-4, with the second product 2.1e-4, of which the output's own rounding is nearly all).
+// 2048 rows of 28 heads over 8192 positions of 4 K/V heads of 128 values, f16:
 // 270 us, 780 TFLOP/s; products and the softmax's instructions share the time, 36 % and 45 % of a SIMD's cycles.
 constexpr int kTileThreads = 256;
 constexpr int kTileWaves = kTileThreads / 64;

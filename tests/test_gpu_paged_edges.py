@@ -26,9 +26,11 @@ def put(seq, s, t, k=None, v=None, at=slice(None)):
         seq.v[page, :, i, at] = torch.as_tensor(v, dtype=seq.dtype)
 
 
-def attend(seq, q, scale, causal=True, max_length=0):
+def attend(seq, q, scale, causal=True, room=0):
+    """room: pages that the table has beyond the sequences', all absent."""
     kp, vp, _, _, table, lengths, starts = seq.to_gpu()
-    batch = jf.PagedBatch(table, lengths, starts, seq.max_rows, max_length or seq.max_length)
+    table = torch.cat([table, torch.full((len(table), room), -1, dtype=torch.int32, device="cuda")], 1)
+    batch = jf.PagedBatch(table, lengths, starts, seq.max_rows, table.shape[1] * seq.page if room else seq.max_length)
     out, lse = jf.PagedCache(kp, vp).attend(batch, q.cuda(), scale, causal)
     return out.cpu(), lse.cpu()
 
@@ -96,3 +98,29 @@ def test_the_heaviest_weight_is_not_rounded(rows, heads, length, kind, bits):
     off = (out.double() - want).abs()
     bound = (half_step(seq.dtype) + 5e-5) * want.abs() + torch.finfo(seq.dtype).tiny * torch.finfo(seq.dtype).eps
     assert (off <= bound).all(), (off / want.abs()).nan_to_num().max().item()
+
+
+@pytest.mark.parametrize("rows,lens,heads,kv,dim,room", [
+    ([1], [1], 1, 1, 64, 0), ([1, 2], [40, 17], 8, 2, 128, 0), ([3], [300], 5, 1, 256, 0), ([2, 1], [90, 33], 6, 2, 200, 0),
+    ([1], [2000], 28, 4, 128, 0), ([4], [9000], 4, 1, 72, 0), ([8, 5], [60, 500], 16, 4, 128, 1 << 13),
+    ([9], [70], 3, 1, 48, 1 << 15)])
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+def test_attention_of_few_queries_rounds_once(rows, lens, heads, kv, dim, room, kind):
+    """Queries and keys whose scores are exact in f32: what is left is the output's rounding."""
+    seq = Sequences(rows, lens, kv, dim, 16, TYPES[kind], seed=3)
+    g = torch.Generator().manual_seed(7)
+    seq.k = (torch.randint(-8, 9, seq.k.shape, generator=g) / 8).to(seq.dtype)
+    q = (torch.randint(-8, 9, (seq.total, heads, dim), generator=g) / 8).to(seq.dtype)
+    scale = dim ** -0.5
+    want, _, _, _ = seq.attend(q, scale)
+    out, _ = attend(seq, q, scale, room=room)
+    values = seq.v
+    seq.v = values.abs()
+    size = seq.attend(q, scale)[0]
+    # Products of eighths add up exactly, to scores of 6 at most after the scale (2^-24 of it for product, scale and
+    # difference each, 1.1e-6), exp2 2^-23; a weight's two values leave half a step of half a step; f32 sums of 9000 / 64
+    # products of 32 a wave, 8 waves and 40 parts, 1.2e-5.
+    step = half_step(seq.dtype)
+    bound = size * (step * step + 1.4e-5) + step * (want.abs() + size * 2e-5) + torch.finfo(seq.dtype).tiny * torch.finfo(seq.dtype).eps
+    off = (out.double() - want).abs()
+    assert (off <= bound).all(), ((off - bound) / size).max().item()
