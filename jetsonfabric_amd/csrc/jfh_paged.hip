@@ -304,10 +304,14 @@ __device__ __forceinline__ uint4 column(const uint32_t (&v)[8][VW], int c) {
                  __builtin_amdgcn_perm(v[5][c / 2], v[4][c / 2], pick), __builtin_amdgcn_perm(v[7][c / 2], v[6][c / 2], pick)};
 }
 
+// 2^x for the sums of slots whose maximum lies x below the row's: never 0, or an infinite sum would become NaN. (2^-149 of
+// a sum of finite values is nothing beside any that count.)
+__device__ __forceinline__ float share_of(float x) { return fmaxf(exp2f(x), 1.4e-45F); }
+
 // Weight of sums with maximum m among others with maximum `now`. A part that has seen nothing (l = 0) weighs nothing; one
 // whose scores are NaN (m = -inf, l NaN) goes on as such.
 __device__ __forceinline__ float split_share(float m, float l, float now) {
-    return l == 0.0F ? 0.0F : m == -INFINITY ? 1.0F : exp2f(m - now);
+    return l == 0.0F ? 0.0F : m == -INFINITY ? 1.0F : share_of(m - now);
 }
 
 // Weights are 2^(score - top), where `top` is a row's running maximum (base 2) less kRaised: the largest one is the power
@@ -441,13 +445,12 @@ __global__ __launch_bounds__(64 * kFewWaves<HDP>) void k_attend_few(Attend a, in
         }
     };
 
-    int t = t0 + wave;
     Keys now{}, next{};
-    if (t < t1) {
-        now = look_up(t);
+    if (t0 + wave < t1) {
+        now = look_up(t0 + wave);
         fetch_k(now);
         fetch_v(now);
-        if (t + kWaves < t1) next = look_up(t + kWaves);
+        if (t0 + wave + kWaves < t1) next = look_up(t0 + wave + kWaves);
     }
 
     // queries to LDS in operand order, zeros behind the last one and beyond head_dim
@@ -469,147 +472,166 @@ __global__ __launch_bounds__(64 * kFewWaves<HDP>) void k_attend_few(Attend a, in
     for (int mt = 0; mt < MT; ++mt) limit[mt] = sees(min(m0 + 16 * mt + i, queries - 1));
     float4v o[MT][VEC];
     float top[MT], sum[MT];
+    const auto walk = [&](auto again) __attribute__((always_inline)) {
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-        top[mt] = -INFINITY;
-        sum[mt] = 0.0F;
+        for (int mt = 0; mt < MT; ++mt) {
+            top[mt] = -INFINITY;
+            sum[mt] = 0.0F;
 #pragma unroll
-        for (int c = 0; c < VEC; ++c) o[mt][c] = float4v{0.0F, 0.0F, 0.0F, 0.0F};
-    }
+            for (int c = 0; c < VEC; ++c) o[mt][c] = float4v{0.0F, 0.0F, 0.0F, 0.0F};
+        }
 
-    for (; t < t1; t += kWaves) {
-        const int base = t * kFewKeys;
-        const bool whole = now.present == 0xFFFFFFFFU;
-        const bool hidden = base + kFewKeys > least;  // some query here does not see some of the tile
-        if (dim < HDP) {  // beyond head_dim Q is 0, and what it meets must be a number
+        for (int t = t0 + wave; t < t1; t += kWaves) {
+            if constexpr (again) {
+                now = look_up(t);
+                fetch_k(now);
+                fetch_v(now);
+            }
+            const int base = t * kFewKeys;
+            const bool whole = now.present == 0xFFFFFFFFU;
+            const bool hidden = base + kFewKeys > least;  // some query here does not see some of the tile
+            if (dim < HDP) {  // beyond head_dim Q is 0, and what it meets must be a number
+#pragma unroll
+                for (int c = 0; c < KC; ++c) {
+                    if (32 * c + 8 * g >= dim) k[0][c] = k[1][c] = __builtin_bit_cast(v8, uint4{0, 0, 0, 0});
+                }
+            }
+            float4v sc[MT][2];
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) sc[mt][0] = sc[mt][1] = float4v{0.0F, 0.0F, 0.0F, 0.0F};
 #pragma unroll
             for (int c = 0; c < KC; ++c) {
-                if (32 * c + 8 * g >= dim) k[0][c] = k[1][c] = __builtin_bit_cast(v8, uint4{0, 0, 0, 0});
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) {
+                    const v8 q = __builtin_bit_cast(v8, q_lds[mt][c][lane]);
+                    sc[mt][0] = V::mfma(k[0][c], q, sc[mt][0]);
+                    sc[mt][1] = V::mfma(k[1][c], q, sc[mt][1]);
+                }
             }
-        }
-        float4v sc[MT][2];
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) sc[mt][0] = sc[mt][1] = float4v{0.0F, 0.0F, 0.0F, 0.0F};
-#pragma unroll
-        for (int c = 0; c < KC; ++c) {
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
-                const v8 q = __builtin_bit_cast(v8, q_lds[mt][c][lane]);
-                sc[mt][0] = V::mfma(k[0][c], q, sc[mt][0]);
-                sc[mt][1] = V::mfma(k[1][c], q, sc[mt][1]);
-            }
-        }
-        if (t + kWaves < t1) fetch_k(next);
+            if (!again && t + kWaves < t1) fetch_k(next);
 
-        // scores of keys base + 16 u + 4 g + r, query i
-        uint32_t seen[MT];
-        if (!whole || hidden) {
+            // scores of keys base + 16 u + 4 g + r, query i
+            uint32_t seen[MT];
+            if (again || !whole || hidden) {
 #pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
-                seen[mt] = 0;
+                for (int mt = 0; mt < MT; ++mt) {
+                    seen[mt] = 0;
 #pragma unroll
-                for (int j = 0; j < 8; ++j) {
-                    const int e = 16 * (j / 4) + 4 * g + j % 4;
-                    const bool see = (now.present >> e & 1U) && base + e < limit[mt];
-                    seen[mt] |= static_cast<uint32_t>(see) << j;
-                    if (!see) sc[mt][j / 4][j % 4] = -INFINITY;
-                }
-            }
-        }
-        float most[MT];
-        bool rise = false;
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-            most[mt] = sc[mt][0][0];
-#pragma unroll
-            for (int j = 1; j < 8; ++j) most[mt] = fmaxf(most[mt], sc[mt][j / 4][j % 4]);
-            most[mt] = groups_max(most[mt]) * a.scale_log2 - V::kRaised;
-            rise |= most[mt] > top[mt];
-        }
-        if (__ballot(rise)) {
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
-                const float to = fmaxf(top[mt], most[mt]);
-                const float shrink = to == -INFINITY ? 1.0F : exp2f(top[mt] - to);
-                top[mt] = to;
-                sum[mt] *= shrink;
-#pragma unroll
-                for (int c = 0; c < VEC; ++c) o[mt][c] *= shrink;
-            }
-        }
-        v8 p[MT], rest[MT];  // weights, what their rounding left
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) {
-            const float ref = top[mt] == -INFINITY ? 0.0F : top[mt];
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float w = __builtin_amdgcn_exp2f(fmaf(sc[mt][j / 4][j % 4], a.scale_log2, -ref));
-                sum[mt] += w;
-                p[mt][j] = static_cast<T>(w);
-                rest[mt][j] = static_cast<T>(w - static_cast<float>(p[mt][j]));
-            }
-        }
-        if (!whole || dim < HDP) {  // what is not there must be a number: its weight is 0
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-#pragma unroll
-                for (int w = 0; w < VW; ++w) {
-                    if (!(now.present >> (16 * (j / 4) + 4 * g + j % 4) & 1U) || VEC * i + 2 * w >= dim) v[j][w] = 0;
-                }
-            }
-        }
-        bool odd = false;
-        if (hidden) {
-#pragma unroll
-            for (int j = 0; j < 8; ++j) {
-#pragma unroll
-                for (int w = 0; w < VW; ++w) odd |= nonfinite<T>(v[j][w]);
-            }
-        }
-        // rare: marks of the infinities and NaN of V, taken out for the product, go to LDS by column, a byte per lane group
-        uint32_t* marks = reinterpret_cast<uint32_t*>(part_o[wave]);  // [3][HDP], the wave's own until the loop ends
-        const bool any_odd = __ballot(odd) != 0;
-        if (any_odd) {
-#pragma unroll
-            for (int c = 0; c < VEC; ++c) {
-                uint32_t mark[3] = {0, 0, 0};
-#pragma unroll
-                for (int j = 0; j < 8; ++j) take_nonfinite<T>(v[j][c / 2], c % 2, j, mark);
-#pragma unroll
-                for (int n = 0; n < 3; ++n) reinterpret_cast<uint8_t*>(marks + n * HDP + VEC * i + c)[g] = static_cast<uint8_t>(mark[n]);
-            }
-        }
-#pragma unroll
-        for (int c = 0; c < VEC; ++c) {
-            const v8 x = __builtin_bit_cast(v8, column<VW>(v, c));
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt) o[mt][c] = V::mfma(x, rest[mt], V::mfma(x, p[mt], o[mt][c]));
-        }
-        if (any_odd) {
-            asm volatile("" ::: "memory");
-#pragma unroll
-            for (int mt = 0; mt < MT; ++mt) {
-                // the query's keys: bit 8 g + j
-                uint32_t see = seen[mt] << (8 * g);
-                see |= __shfl_xor(see, 16);
-                see |= __shfl_xor(see, 32);
-#pragma unroll
-                for (int c = 0; c < VEC; ++c) {
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const int d = VEC * (4 * g + r) + c;
-                        o[mt][c][r] = with_nonfinite(o[mt][c][r], marks[d] & see, marks[HDP + d] & see, marks[2 * HDP + d] & see);
-                        asm volatile("" ::: "memory");  // one column's marks at a time: the sums leave few registers
+                    for (int j = 0; j < 8; ++j) {
+                        const int e = 16 * (j / 4) + 4 * g + j % 4;
+                        const bool see = (now.present >> e & 1U) && base + e < limit[mt];
+                        seen[mt] |= static_cast<uint32_t>(see) << j;
+                        if (!see) sc[mt][j / 4][j % 4] = -INFINITY;
                     }
                 }
             }
+            float most[MT];
+            bool rise = false;
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+                most[mt] = sc[mt][0][0];
+#pragma unroll
+                for (int j = 1; j < 8; ++j) most[mt] = fmaxf(most[mt], sc[mt][j / 4][j % 4]);
+                most[mt] = groups_max(most[mt]) * a.scale_log2 - V::kRaised;
+                rise |= most[mt] > top[mt];
+            }
+            if (__ballot(rise)) {
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) {
+                    const float to = fmaxf(top[mt], most[mt]);
+                    const float shrink = to == -INFINITY ? 1.0F : share_of(top[mt] - to);
+                    top[mt] = to;
+                    sum[mt] *= shrink;
+#pragma unroll
+                    for (int c = 0; c < VEC; ++c) o[mt][c] *= shrink;
+                }
+            }
+            v8 p[MT], rest[MT];  // weights, what their rounding left
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+                const float ref = top[mt] == -INFINITY ? 0.0F : top[mt];
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const float w = __builtin_amdgcn_exp2f(fmaf(sc[mt][j / 4][j % 4], a.scale_log2, -ref));
+                    sum[mt] += w;
+                    p[mt][j] = static_cast<T>(w);
+                    rest[mt][j] = static_cast<T>(w - static_cast<float>(p[mt][j]));
+                }
+            }
+            if (!whole) {  // what is not there must be a number: its weight is 0 (columns beyond head_dim go nowhere)
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    if (now.present >> (16 * (j / 4) + 4 * g + j % 4) & 1U) continue;
+#pragma unroll
+                    for (int w = 0; w < VW; ++w) v[j][w] = 0;
+                }
+            }
+            bool odd = false;
+            if constexpr (again) {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+#pragma unroll
+                    for (int w = 0; w < VW; ++w) odd |= nonfinite<T>(v[j][w]);
+                }
+            }
+            // marks of the infinities and NaN of V, taken out for the product, go to LDS by column, a byte per lane group
+            uint32_t* marks = reinterpret_cast<uint32_t*>(part_o[wave]);  // [3][HDP], the wave's own until the loop ends
+            const bool any_odd = __ballot(odd) != 0;
+            if (any_odd) {
+#pragma unroll
+                for (int c = 0; c < VEC; ++c) {
+                    uint32_t mark[3] = {0, 0, 0};
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) take_nonfinite<T>(v[j][c / 2], c % 2, j, mark);
+#pragma unroll
+                    for (int n = 0; n < 3; ++n) reinterpret_cast<uint8_t*>(marks + n * HDP + VEC * i + c)[g] = static_cast<uint8_t>(mark[n]);
+                }
+            }
+#pragma unroll
+            for (int c = 0; c < VEC; ++c) {
+                const v8 x = __builtin_bit_cast(v8, column<VW>(v, c));
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) o[mt][c] = V::mfma(x, rest[mt], V::mfma(x, p[mt], o[mt][c]));
+            }
+            if (any_odd) {
+                asm volatile("" ::: "memory");
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) {
+                    // the query's keys: bit 8 g + j
+                    uint32_t see = seen[mt] << (8 * g);
+                    see |= __shfl_xor(see, 16);
+                    see |= __shfl_xor(see, 32);
+#pragma unroll
+                    for (int c = 0; c < VEC; ++c) {
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            const int d = VEC * (4 * g + r) + c;
+                            o[mt][c][r] = with_nonfinite(o[mt][c][r], marks[d] & see, marks[HDP + d] & see, marks[2 * HDP + d] & see);
+                            asm volatile("" ::: "memory");  // one column's marks at a time: the sums leave few registers
+                        }
+                    }
+                }
+            }
+            if (!again && t + kWaves < t1) {
+                fetch_v(next);
+                now = next;
+                if (t + 2 * kWaves < t1) next = look_up(t + 2 * kWaves);
+            }
         }
-        if (t + kWaves < t1) {
-            fetch_v(next);
-            now = next;
-            if (t + 2 * kWaves < t1) next = look_up(t + 2 * kWaves);
+        float odd = 0.0F;
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) {
+#pragma unroll
+            for (int c = 0; c < VEC; ++c) {
+#pragma unroll
+                for (int r = 0; r < 4; ++r) odd = fmaf(o[mt][c][r], 0.0F, odd);
+            }
         }
-    }
+        return __ballot(odd != odd) != 0;
+    };
+    // A sum that is not finite at the end has met infinities or NaN of V, whose weight may be 0 (hidden, or rounded to 0): the
+    // wave walks its tiles again and takes them out of V.
+    if (walk(std::false_type{})) walk(std::true_type{});
 
     // the waves' sums, 16 queries at a time
     const int64_t all = static_cast<int64_t>(a.q.rows) * a.q.heads;
@@ -709,7 +731,7 @@ __global__ __launch_bounds__(kTileThreads, HDP <= 128 ? 2 : 1) void k_attend_til
     __shared__ uint4 v_lds[2][HDP * VS];
     __shared__ int64_t offsets[3][KT];
     __shared__ unsigned long long there[3];
-    // of tiles that some query does not see whole: the keys (bits) whose V is +inf, -inf, NaN, by column and piece
+    // the keys (bits) whose V is +inf, -inf, NaN, by column and piece
     __shared__ alignas(8) uint8_t marks[2][3][HDP][8];
     __shared__ bool odd[2][kTileWaves];
 
@@ -743,7 +765,7 @@ __global__ __launch_bounds__(kTileThreads, HDP <= 128 ? 2 : 1) void k_attend_til
     const auto sees = [&](int query_index) {  // slots that a query sees
         return a.causal ? max(0, first + min(query_index, queries - 1) / group + 1) : span.len;
     };
-    const int limit = sees(m), least = sees(wm), group_least = sees(m0), end = sees(m0 + kTileQueries - 1);
+    const int limit = sees(m), least = sees(wm), end = sees(m0 + kTileQueries - 1);
 
     const int tiles = (span.len + KT - 1) / KT;
     const int per = (tiles + static_cast<int>(a.splits) - 1) / static_cast<int>(a.splits);
@@ -780,7 +802,7 @@ __global__ __launch_bounds__(kTileThreads, HDP <= 128 ? 2 : 1) void k_attend_til
             }
         }
     };
-    const auto stage = [&](int t) {
+    const auto stage = [&](int t, auto again) __attribute__((always_inline)) {
         const int b = t % 2;
 #pragma unroll
         for (int p = 0; p < KP; ++p) {
@@ -797,7 +819,7 @@ __global__ __launch_bounds__(kTileThreads, HDP <= 128 ? 2 : 1) void k_attend_til
                     if (!(present >> key & 1ULL) || v_at >= dim) vr[j] = uint2{0, 0};
                 }
             }
-            if ((t + 1) * KT > group_least) {
+            if constexpr (again) {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) any |= nonfinite<T>(vr[j].x) || nonfinite<T>(vr[j].y);
 #pragma unroll
@@ -820,116 +842,138 @@ __global__ __launch_bounds__(kTileThreads, HDP <= 128 ? 2 : 1) void k_attend_til
                 v_lds[b][((v_at + e) % HB * 32 + (v_at + e) / HB) * VS + v_piece] = uint4{two(0), two(2), two(4), two(6)};
             }
         }
-        any = __ballot(any) != 0;
-        if (lane == 0) odd[b][wave] = any;
+        if constexpr (again) {
+            any = __ballot(any) != 0;
+            if (lane == 0) odd[b][wave] = any;
+        }
     };
 
     float16v o[HB];
+    float top, sum;
+    const auto walk = [&](auto again) __attribute__((always_inline)) {
 #pragma unroll
-    for (int e = 0; e < HB; ++e) {
+        for (int e = 0; e < HB; ++e) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) o[e][r] = 0.0F;
-    }
-    float top = -INFINITY, sum = 0.0F;
-
-    if (t0 < t1) {
-        look_up(t0);
-        look_up(t0 + 1);
-        __syncthreads();
-        fetch(t0);
-        stage(t0);
-        __syncthreads();
-    }
-    for (int t = t0; t < t1; ++t) {
-        const int b = t % 2, base = t * KT;
-        if (t + 1 < t1) fetch(t + 1);
-        if (t + 2 < t1) look_up(t + 2);
-
-        float16v sc[KB];
-#pragma unroll
-        for (int e = 0; e < KB; ++e) {
-#pragma unroll
-            for (int r = 0; r < 16; ++r) sc[e][r] = 0.0F;
+            for (int r = 0; r < 16; ++r) o[e][r] = 0.0F;
         }
-#pragma unroll
-        for (int c = 0; c < KC; ++c) {
+        top = -INFINITY;
+        sum = 0.0F;
+
+        if (t0 < t1) {
+            look_up(t0);
+            look_up(t0 + 1);
+            __syncthreads();
+            fetch(t0);
+            stage(t0, again);
+            __syncthreads();
+        }
+        for (int t = t0; t < t1; ++t) {
+            const int b = t % 2, base = t * KT;
+            if (t + 1 < t1) fetch(t + 1);
+            if (t + 2 < t1) look_up(t + 2);
+
+            float16v sc[KB];
 #pragma unroll
             for (int e = 0; e < KB; ++e) {
-                const uint4 k = k_lds[b][(32 * e + n) * KS + 2 * c + g];
-                sc[e] = V::mfma(__builtin_bit_cast(v8, k), q[c], sc[e]);
+#pragma unroll
+                for (int r = 0; r < 16; ++r) sc[e][r] = 0.0F;
             }
-        }
-        const unsigned long long present = there[t % 3];
-        const bool hidden = base + KT > least;
-        if (hidden || present != kAllKeys) {
+#pragma unroll
+            for (int c = 0; c < KC; ++c) {
+#pragma unroll
+                for (int e = 0; e < KB; ++e) {
+                    const uint4 k = k_lds[b][(32 * e + n) * KS + 2 * c + g];
+                    sc[e] = V::mfma(__builtin_bit_cast(v8, k), q[c], sc[e]);
+                }
+            }
+            const unsigned long long present = there[t % 3];
+            const bool hidden = base + KT > least;
+            if (hidden || present != kAllKeys) {
+#pragma unroll
+                for (int e = 0; e < KB; ++e) {
+                    // keys 32 e + 4 g + 8 (r / 4) + r % 4
+                    const uint32_t here = static_cast<uint32_t>(present >> (32 * e + 4 * g));
+                    const int left = limit - base - 32 * e - 4 * g;
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const int key = 8 * (r / 4) + r % 4;
+                        if (key >= left || !(here >> key & 1U)) sc[e][r] = -INFINITY;
+                    }
+                }
+            }
+            float most = sc[0][0];
 #pragma unroll
             for (int e = 0; e < KB; ++e) {
-                // keys 32 e + 4 g + 8 (r / 4) + r % 4
-                const uint32_t here = static_cast<uint32_t>(present >> (32 * e + 4 * g));
-                const int left = limit - base - 32 * e - 4 * g;
+#pragma unroll
+                for (int r = 0; r < 16; ++r) most = fmaxf(most, sc[e][r]);
+            }
+            most = halves_max(most) * a.scale_log2 - V::kRaised;
+            if (__ballot(most > top)) {
+                const float now = fmaxf(top, most);
+                const float shrink = now == -INFINITY ? 1.0F : share_of(top - now);
+                top = now;
+                sum *= shrink;
+#pragma unroll
+                for (int e = 0; e < HB; ++e) o[e] *= shrink;
+            }
+            const float ref = top == -INFINITY ? 0.0F : top;
+            v8 p[KB][2];
+#pragma unroll
+            for (int e = 0; e < KB; ++e) {
 #pragma unroll
                 for (int r = 0; r < 16; ++r) {
-                    const int key = 8 * (r / 4) + r % 4;
-                    if (key >= left || !(here >> key & 1U)) sc[e][r] = -INFINITY;
+                    const float w = __builtin_amdgcn_exp2f(fmaf(sc[e][r], a.scale_log2, -ref));
+                    sum += w;
+                    p[e][r / 8][r % 8] = static_cast<T>(w);
                 }
             }
-        }
-        float most = sc[0][0];
 #pragma unroll
-        for (int e = 0; e < KB; ++e) {
+            for (int c = 0; c < 2 * KB; ++c) {
 #pragma unroll
-            for (int r = 0; r < 16; ++r) most = fmaxf(most, sc[e][r]);
-        }
-        most = halves_max(most) * a.scale_log2 - V::kRaised;
-        if (__ballot(most > top)) {
-            const float now = fmaxf(top, most);
-            const float shrink = now == -INFINITY ? 1.0F : exp2f(top - now);
-            top = now;
-            sum *= shrink;
-#pragma unroll
-            for (int e = 0; e < HB; ++e) o[e] *= shrink;
-        }
-        const float ref = top == -INFINITY ? 0.0F : top;
-        v8 p[KB][2];
-#pragma unroll
-        for (int e = 0; e < KB; ++e) {
-#pragma unroll
-            for (int r = 0; r < 16; ++r) {
-                const float w = __builtin_amdgcn_exp2f(fmaf(sc[e][r], a.scale_log2, -ref));
-                sum += w;
-                p[e][r / 8][r % 8] = static_cast<T>(w);
-            }
-        }
-#pragma unroll
-        for (int c = 0; c < 2 * KB; ++c) {
-#pragma unroll
-            for (int e = 0; e < HB; ++e) {
-                const uint4 v = v_lds[b][(32 * e + n) * VS + 2 * c + g];
-                o[e] = V::mfma(__builtin_bit_cast(v8, v), p[c / 2][c % 2], o[e]);
-            }
-        }
-        if (base + KT > group_least && (odd[b][0] || odd[b][1] || odd[b][2] || odd[b][3])) {
-            // what the tile's V has of infinities and NaN, staged as 0 for all waves, for the queries that see them
-            unsigned long long seen = 0;
-            for (int k = 0; k < KT; ++k) {
-                const int key = 16 * (k / 16) + 8 * (k % 8 / 4) + 4 * (k / 8 % 2) + k % 4;
-                seen |= static_cast<unsigned long long>(base + key < limit && (present >> key & 1ULL)) << k;
-            }
-#pragma unroll
-            for (int e = 0; e < HB; ++e) {
-#pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int d = HB * (8 * (r / 4) + 4 * g + r % 4) + e;
-                    const auto any = [&](int k) {
-                        return (*reinterpret_cast<const unsigned long long*>(marks[b][k][d]) & seen) != 0;
-                    };
-                    o[e][r] = with_nonfinite(o[e][r], any(0), any(1), any(2));
-                    asm volatile("" ::: "memory");  // one column's marks at a time: the sums leave few registers
+                for (int e = 0; e < HB; ++e) {
+                    const uint4 v = v_lds[b][(32 * e + n) * VS + 2 * c + g];
+                    o[e] = V::mfma(__builtin_bit_cast(v8, v), p[c / 2][c % 2], o[e]);
                 }
             }
+            if (again && (odd[b][0] || odd[b][1] || odd[b][2] || odd[b][3])) {
+                // what the tile's V has of infinities and NaN, staged as 0 for all waves, for the queries that see them
+                unsigned long long seen = 0;
+                for (int k = 0; k < KT; ++k) {
+                    const int key = 16 * (k / 16) + 8 * (k % 8 / 4) + 4 * (k / 8 % 2) + k % 4;
+                    seen |= static_cast<unsigned long long>(base + key < limit && (present >> key & 1ULL)) << k;
+                }
+#pragma unroll
+                for (int e = 0; e < HB; ++e) {
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) {
+                        const int d = HB * (8 * (r / 4) + 4 * g + r % 4) + e;
+                        const auto any = [&](int k) {
+                            return (*reinterpret_cast<const unsigned long long*>(marks[b][k][d]) & seen) != 0;
+                        };
+                        o[e][r] = with_nonfinite(o[e][r], any(0), any(1), any(2));
+                        asm volatile("" ::: "memory");  // one column's marks at a time: the sums leave few registers
+                    }
+                }
+            }
+            if (t + 1 < t1) stage(t + 1, again);
+            __syncthreads();
         }
-        if (t + 1 < t1) stage(t + 1);
+        if (again || t0 >= t1) return false;
+        float not_finite = 0.0F;
+#pragma unroll
+        for (int e = 0; e < HB; ++e) {
+#pragma unroll
+            for (int r = 0; r < 16; ++r) not_finite = fmaf(o[e][r], 0.0F, not_finite);
+        }
+        const bool any = __ballot(not_finite != not_finite) != 0;
+        if (lane == 0) odd[0][wave] = any;
         __syncthreads();
+        return odd[0][0] || odd[0][1] || odd[0][2] || odd[0][3];
+    };
+    // as in k_attend_few: where some sum is not finite at the end, the work-group walks its tiles again
+    if (walk(std::false_type{})) {
+        __syncthreads();
+        walk(std::true_type{});
     }
 
     if (m >= queries) return;

@@ -124,3 +124,46 @@ def test_attention_of_few_queries_rounds_once(rows, lens, heads, kv, dim, room, 
     bound = size * (step * step + 1.4e-5) + step * (want.abs() + size * 2e-5) + torch.finfo(seq.dtype).tiny * torch.finfo(seq.dtype).eps
     off = (out.double() - want).abs()
     assert (off <= bound).all(), ((off - bound) / size).max().item()
+
+
+@pytest.mark.parametrize("rows,heads,length", FORMS)
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+@pytest.mark.parametrize("bits", [1, 60, 140, 240])
+def test_infinities_reach_every_row_that_sees_them(rows, heads, length, kind, bits):
+    """Infinite and NaN V of slots with 2^-bits of the other slots' weight: early ones that all rows see, at places of a tile
+    that they see whole, and one among the new rows. Whatever the weight rounds to, rows that see them have them."""
+    seq = Sequences([rows], [length], 1, 64, 16, TYPES[kind], seed=bits)
+    seq.k.zero_()
+    seq.k[..., 0] = 4.0
+    first = length - rows
+    odd = {2: (0, math.inf), 5: (first // 2, -math.inf), 7: (100, math.nan), 11: (first - 1, math.inf), 13: (first + rows // 2, math.inf)}
+    for t, _ in odd.values():
+        put(seq, 0, t, k=4.0 - bits / 16.0, at=0)
+    q = torch.zeros(rows, heads, 64, dtype=seq.dtype)
+    q[..., 0] = 16.0
+    want, _, bound, _ = seq.attend(q, math.log(2.0))
+    for column, (t, x) in odd.items():
+        put(seq, 0, t, v=x, at=column)
+    out, lse = attend(seq, q, math.log(2.0))
+    assert torch.isfinite(lse).all()
+    for column, (t, x) in odd.items():
+        sees = max(0, t - first)  # the first row that sees it
+        off = (out[:sees, :, column].double() - want[:sees, :, column]).abs()
+        assert (off <= bound[:sees, :, column]).all()
+        got = out[sees:, :, column]
+        assert torch.isnan(got).all() if x != x else (got == x).all(), (column, t, x)
+    plain = [c for c in range(64) if c not in odd]
+    assert ((out.double() - want).abs() <= bound)[..., plain].all()
+
+
+@pytest.mark.parametrize("rows,heads,length", FORMS)
+@pytest.mark.parametrize("dim", [40, 96, 128, 200])
+def test_infinities_of_both_signs_make_nan(rows, heads, length, dim):
+    seq = Sequences([rows], [length], 2, dim, 16, torch.float16, seed=3)
+    want, _, bound, _ = seq.attend(q := normal(rows, 2 * heads, dim, seed=4).half(), 0.125)
+    put(seq, 0, 0, v=math.inf, at=9)
+    put(seq, 0, length - rows - 1, v=-math.inf, at=9)
+    out, _ = attend(seq, q, 0.125)
+    assert torch.isnan(out[..., 9]).all()
+    plain = torch.arange(dim) != 9
+    assert ((out.double() - want).abs() <= bound)[..., plain].all()
