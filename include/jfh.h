@@ -479,8 +479,10 @@ typedef struct jfh_paged_cache {
  * none. An entry of the table that is no page (negative, or n_pages and more)
  * is an absent page: nothing is written there, and nobody sees its positions.
  * The arrays are in device memory; max_rows and max_length bound what they
- * hold (rows and slots beyond them are left out) and fix the launches, so a
- * captured call may be replayed with other contents. */
+ * hold and fix the launches, so a captured call may be replayed with other
+ * contents. Rows from max_rows on and slots from max_length on are left out,
+ * neither written nor seen; the others stand where they would without the
+ * bounds: row i of a sequence's n at slot lengths - n + i. */
 typedef struct jfh_paged_batch {
     const int32_t * table;      /* [n_seq][table_stride] */
     int32_t * lengths;          /* [n_seq] */

@@ -185,8 +185,8 @@ __global__ __launch_bounds__(kRotateThreads) void k_append(Rotation r, Cache c, 
         const int row = row0 + threadIdx.x;
         Span span;
         const int s = sequence_of(b, k.rows, row, &span);
-        const int slot = span.len - span.rows + (row - span.row0);
-        pages[threadIdx.x] = s >= 0 && slot >= 0 ? page_of(c, b, s, slot) : -1;
+        const int slot = s >= 0 ? span.first + (row - span.row0) : -1;
+        pages[threadIdx.x] = slot >= 0 && slot < span.len ? page_of(c, b, s, slot) : -1;
         slots[threadIdx.x] = slot;
     }
     if (r.n_rot) row_angles(r, positions, row0, rows, cs);
@@ -386,8 +386,7 @@ __global__ __launch_bounds__(64 * kFewWaves<HDP>) void k_attend_few(Attend a, in
     const int queries = span.rows * group;
     if (m0 >= queries) return;
     const int dim = static_cast<int>(a.cache.head_dim);
-    const int first = span.len - span.rows;  // slot of row 0
-    const auto sees = [&](int m) { return a.causal ? max(0, first + m / group + 1) : span.len; };  // slots of query m
+    const auto sees = [&](int m) { return a.causal ? slots_seen(span, m / group) : span.len; };  // slots of query m
     const int least = sees(m0), end = sees(min(queries, m0 + 16 * MT) - 1);  // seen by all queries here, by any
 
     // the split's tiles: equal parts of the sequence's, whole rounds of the waves
@@ -746,7 +745,6 @@ __global__ __launch_bounds__(kTileThreads, HDP <= 128 ? 2 : 1) void k_attend_til
     const int m0 = ((queries + kTileQueries - 1) / kTileQueries - 1 - static_cast<int>(blockIdx.x / pairs / a.splits)) * kTileQueries;
     if (m0 < 0) return;
     const int dim = static_cast<int>(a.cache.head_dim);
-    const int first = span.len - span.rows;
 
     const int wm = m0 + 32 * wave, m = wm + n;
     const Query query = query_of(min(m, queries - 1), group, h);
@@ -763,7 +761,7 @@ __global__ __launch_bounds__(kTileThreads, HDP <= 128 ? 2 : 1) void k_attend_til
         }
     }
     const auto sees = [&](int query_index) {  // slots that a query sees
-        return a.causal ? max(0, first + min(query_index, queries - 1) / group + 1) : span.len;
+        return a.causal ? slots_seen(span, min(query_index, queries - 1) / group) : span.len;
     };
     const int limit = sees(m), least = sees(wm), end = sees(m0 + kTileQueries - 1);
 
@@ -1141,7 +1139,6 @@ __global__ __launch_bounds__(kWeighThreads) void k_weigh_few(Weigh a, int group,
     const int base = (static_cast<int>(blockIdx.x % blocks) * kWeighWaves + wave) * kFewWeighSlots;
     const int queries = span.rows * group;
     if (base >= span.len || queries == 0) return;
-    const int first = span.len - span.rows;
 
     int64_t index[U];
     v8 k[U][KC];
@@ -1150,7 +1147,7 @@ __global__ __launch_bounds__(kWeighThreads) void k_weigh_few(Weigh a, int group,
 #pragma unroll
     for (int u = 0; u < U; ++u) sum[u] = float4v{0.0F, 0.0F, 0.0F, 0.0F};
     // from the first row that sees slot `base`
-    for (int m0 = a.causal ? max(0, base - first) * group / 16 * 16 : 0; m0 < queries; m0 += 16) {
+    for (int m0 = a.causal ? rows_before(span, base) * group / 16 * 16 : 0; m0 < queries; m0 += 16) {
         const Query query = query_of(min(m0 + i, queries - 1), group, h);
         const int64_t row = span.row0 + query.row;
         const T* x = static_cast<const T*>(a.q.data) + row * a.q.row_stride + query.head * a.q.head_stride;
@@ -1159,7 +1156,7 @@ __global__ __launch_bounds__(kWeighThreads) void k_weigh_few(Weigh a, int group,
         for (int c = 0; c < KC; ++c) q[c] = row_piece<T>(x, 32 * c + 8 * g, static_cast<int>(a.cache.head_dim));
         const float lse = a.lse[row * a.q.heads + query.head];
         // a row that saw nothing adds nothing
-        const int limit = m0 + i >= queries || lse == -INFINITY ? 0 : a.causal ? first + query.row + 1 : span.len;
+        const int limit = m0 + i >= queries || lse == -INFINITY ? 0 : a.causal ? slots_seen(span, query.row) : span.len;
         weigh_queries<T, false>(a, base, k, q, lse * kLog2e, limit, sum);
     }
 #pragma unroll
@@ -1196,14 +1193,14 @@ __global__ __launch_bounds__(kWeighThreads, 2) void k_weigh_many(Weigh a, int gr
     const int group_base = static_cast<int>(blockIdx.x % blocks) * kWeighWaves * 16 * U, base = group_base + wave * 16 * U;
     const int queries = span.rows * group;
     if (group_base >= span.len) return;
-    const int first = span.len - span.rows, dim = static_cast<int>(a.cache.head_dim);
+    const int dim = static_cast<int>(a.cache.head_dim);
 
     int64_t index[U];
     v8 k[U][KC];
     weighed_rows<T>(a, s, h, span.len, base, k, index);
 
     // the split's queries, in whole tiles, from the first row that sees the work-group's first slot
-    const int from = a.causal ? max(0, group_base - first) * group / QT : 0;
+    const int from = a.causal ? rows_before(span, group_base) * group / QT : 0;
     const int tiles = (queries + QT - 1) / QT - from, per = (tiles + static_cast<int>(a.splits) - 1) / static_cast<int>(a.splits);
     const int t0 = from + min(static_cast<int>(split) * per, tiles), t1 = from + min(static_cast<int>(split + 1) * per, tiles);
 
@@ -1238,7 +1235,7 @@ __global__ __launch_bounds__(kWeighThreads, 2) void k_weigh_many(Weigh a, int gr
             const Query query = query_of(min(m, queries - 1), group, h);
             const float lse = a.lse[(span.row0 + query.row) * static_cast<int64_t>(a.q.heads) + query.head];
             // a row that saw nothing adds nothing
-            limits[b][tid] = m >= queries || lse == -INFINITY ? 0 : a.causal ? first + query.row + 1 : span.len;
+            limits[b][tid] = m >= queries || lse == -INFINITY ? 0 : a.causal ? slots_seen(span, query.row) : span.len;
             refs[b][tid] = lse * kLog2e;
         }
     };

@@ -46,10 +46,11 @@ struct Batch {
     uint32_t n_seq, table_stride, max_rows, max_length;
 };
 
-// Rows [row0, row0 + rows) of the step are sequence s's and stand at its slots len - rows .. len - 1. Whatever the
-// device arrays hold, the rows lie inside the step's n_rows and the slots inside the table.
+// Rows [row0, row0 + rows) of the step are sequence s's; row row0 + r stands at slot first + r, of which those in
+// [0, len) exist: the bounds leave out rows from max_rows and slots from max_length on, and move nothing. Whatever the
+// device arrays hold, the rows lie inside the step's n_rows, [0, len) inside the table, and first + rows in 32 bits.
 struct Span {
-    int32_t row0, rows, len;
+    int32_t row0, rows, len, first;
 };
 
 JFH_HOST_DEVICE int32_t clamped(int32_t v, int32_t lo, int32_t hi) { return v < lo ? lo : v > hi ? hi : v; }
@@ -59,10 +60,21 @@ JFH_HOST_DEVICE int32_t span_length(const Batch& b, uint32_t s) {
 }
 
 JFH_HOST_DEVICE Span sequence_span(const Batch& b, uint32_t n_rows, uint32_t s) {
-    const int32_t r0 = clamped(b.row_starts[s], 0, static_cast<int32_t>(n_rows));
-    const int32_t r1 = clamped(b.row_starts[s + 1], r0, static_cast<int32_t>(n_rows));
+    const int32_t r0 = clamped(b.row_starts[s], 0, static_cast<int32_t>(n_rows)), end = b.row_starts[s + 1];
+    const int32_t r1 = clamped(end, r0, static_cast<int32_t>(n_rows));
     const int32_t n = clamped(r1 - r0, 0, static_cast<int32_t>(b.max_rows));
-    return Span{r0, n, span_length(b, s)};
+    // row end - 1 stands at the last slot
+    const int64_t first = static_cast<int64_t>(b.lengths[s] > 0 ? b.lengths[s] : 0) - end + r0;
+    return Span{r0, n, span_length(b, s), static_cast<int32_t>(first < b.max_length ? first : b.max_length)};
+}
+
+// Slots that row row0 + r sees when it sees what is before it and itself.
+JFH_HOST_DEVICE int32_t slots_seen(const Span& x, int32_t r) { return clamped(x.first + r + 1, 0, x.len); }
+
+// Rows of a sequence before the first that sees a slot.
+JFH_HOST_DEVICE int32_t rows_before(const Span& x, int32_t slot) {
+    const int64_t n = static_cast<int64_t>(slot) - x.first;
+    return n < 0 ? 0 : n < x.rows ? static_cast<int32_t>(n) : x.rows;
 }
 
 // The sequence of a row (row_starts ascending), or -1 for a row of none.

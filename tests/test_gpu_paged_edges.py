@@ -167,3 +167,60 @@ def test_infinities_of_both_signs_make_nan(rows, heads, length, dim):
     assert torch.isnan(out[..., 9]).all()
     plain = torch.arange(dim) != 9
     assert ((out.double() - want).abs() <= bound)[..., plain].all()
+
+
+# ---------------------------------------------------------------- rows and lengths beyond a batch's bounds
+
+BOUNDS = [([3, 2, 1], [20, 33, 100], 2, 30), ([1, 1, 1], [30, 31, 29], 1, 30), ([40, 30, 3], [60, 300, 700], 35, 290),
+          ([70, 5, 2], [20, 5, 500], 60, 400)]
+
+
+def step(seq, heads, rows, length):
+    """A cache on the GPU, a batch of max_rows and max_length, and random queries."""
+    kp, vp, w, pos, table, lengths, starts = seq.to_gpu()
+    return jf.PagedCache(kp, vp, w, pos), jf.PagedBatch(table, lengths, starts, rows, length), normal(seq.total, heads, seq.dim, seed=9).half()
+
+
+@pytest.mark.parametrize("rows,lens,max_rows,max_length", BOUNDS)
+def test_appended_rows_beyond_the_bounds_are_not_written(rows, lens, max_rows, max_length):
+    """Those within them go to the slots where they would go without: a longer sequence loses nothing that it has."""
+    seq = Sequences(rows, lens, 2, 64, 16, torch.float16, seed=4)
+    cache, batch, x = step(seq, 4, max_rows, max_length)
+    positions = torch.arange(1, seq.total + 1, dtype=torch.int32)
+    cache.append(batch, x[:, :2].cuda(), x[:, 2:].cuda(), positions.cuda())
+    for s in range(len(rows)):
+        for i in range(min(rows[s], max_rows)):
+            t = lens[s] - rows[s] + i
+            if 0 <= t < max_length:
+                page, place = seq.slot(s, t)
+                row = seq.starts[s] + i
+                seq.k[page, :, place], seq.v[page, :, place] = x[row, :2], x[row, 2:]
+                seq.weights[page, :, place], seq.positions[page, :, place] = 0.0, positions[row]
+    assert torch.equal(cache.k.cpu(), seq.k) and torch.equal(cache.v.cpu(), seq.v)
+    assert torch.equal(cache.weights.cpu(), seq.weights) and torch.equal(cache.positions.cpu(), seq.positions)
+
+
+@pytest.mark.parametrize("rows,lens,max_rows,max_length", BOUNDS)
+@pytest.mark.parametrize("causal", [True, False])
+def test_attention_and_weights_within_bounds(rows, lens, max_rows, max_length, causal):
+    """Rows beyond max_rows are left out; the others see what they see without bounds, of the first max_length slots."""
+    seq = Sequences(rows, lens, 2, 64, 16, torch.float16, seed=5)
+    cache, batch, q = step(seq, 8, max_rows, max_length)
+    whole = seq.sees
+    seq.sees = lambda s, causal, there: (whole(s, causal, there) & (torch.arange(seq.lens[s]) < max_length)
+                                         & (torch.arange(seq.rows[s]) < max_rows)[:, None])
+    want, want_lse, bound, lse_bound = seq.attend(q, 0.125, causal)
+    out, lse = torch.full(q.shape, 7.0, dtype=torch.float16, device="cuda"), torch.full(q.shape[:2], 5.0, device="cuda")
+    cache.attend(batch, q.cuda(), 0.125, causal, out=out, lse=lse)
+    out, lse = out.cpu(), lse.cpu()
+    for s in range(len(rows)):
+        r0, r1, r2 = seq.starts[s], seq.starts[s] + min(rows[s], max_rows), seq.starts[s + 1]
+        assert ((out[r0:r1].double() - want[r0:r1]).abs() <= bound[r0:r1]).all()
+        some = want_lse[r0:r1] > -math.inf
+        assert (lse[r0:r1][~some] == -math.inf).all()
+        assert ((lse[r0:r1].double() - want_lse[r0:r1]).abs()[some] <= lse_bound[r0:r1][some]).all()
+        assert (out[r1:r2] == 7).all() and (lse[r1:r2] == 5).all()
+    given = want_lse.float()
+    cache.weigh(batch, q.cuda(), given.cuda(), 0.125, causal)
+    want, bound = seq.weigh(q, given, 0.125, causal)
+    assert ((cache.weights.cpu().double() - want).abs() <= bound).all()
