@@ -490,7 +490,7 @@ typedef struct jfh_paged_batch {
     uint32_t n_seq;
     uint32_t table_stride;
     uint32_t max_rows;
-    uint32_t max_length; /* at most table_stride * page_size */
+    uint32_t max_length; /* at most table_stride * page_size, and 2^31 - 65537 */
 } jfh_paged_batch;
 
 /* Writes a step's K and V rows (any type and strides, the cache's K/V heads

@@ -94,7 +94,8 @@ paged::Batch batch_of(const jfh_paged_batch* b, const jfh_paged_cache& c, bool r
             "a batch needs its table, lengths and row starts");
     const uint64_t slots = static_cast<uint64_t>(b->table_stride) * c.page_size;
     require(b->max_length <= slots, "the batch's max_length exceeds its table");
-    require(b->max_length <= kMaxIndex - 1024 && b->max_rows <= kMaxIndex, "the batch's bounds exceed 2^31");
+    require(b->max_length <= paged::kMaxLength, "the batch's max_length exceeds 2^31 - 65537");
+    require(b->max_rows <= kMaxIndex, "the batch's max_rows exceeds 2^31 - 1");
     return paged::Batch{b->table, b->lengths, b->row_starts, b->n_seq, b->table_stride,
                         std::min(b->max_rows, n_rows), b->max_length};
 }

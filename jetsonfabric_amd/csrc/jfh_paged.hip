@@ -1304,6 +1304,8 @@ __global__ __launch_bounds__(kWeighThreads) void k_weigh_join(Weigh a, int block
 // read caches of up to 8192 slots once. 16 K/V heads of 16384 slots 23 us, 32 of 4097 12.3 us, of which the counts are half.
 constexpr int kSelectThreads = 1024;
 constexpr int kSelectBins = 2048;
+constexpr int kSelectRun = 63;  // most slots of a thread's run, bits of a word
+static_assert(kSelectRun * kSelectThreads <= static_cast<int>(kSlotStep));
 constexpr int kSelectFew = 8192, kSelectMany = 36864;  // keys in LDS; later slots' are computed again where they are used
 
 // Order of weights as unsigned integers, 1 for NaN (nothing is lighter), 0 free.
@@ -1345,6 +1347,7 @@ __device__ __forceinline__ int2 exclusive_sum(int2 v, int2* waves, int2* all) {
 
 template <int CAP, int BATCH>
 __global__ __launch_bounds__(kSelectThreads) void k_evict_select(Evict a) {
+    static_assert(2 * BATCH * kSelectThreads <= static_cast<int>(kSlotStep));
     constexpr bool kStay = CAP <= BATCH * kSelectThreads;  // the first batch, in registers from pass to pass
     __shared__ uint32_t keys[CAP];
     __shared__ uint32_t bins[kSelectBins];
@@ -1488,8 +1491,8 @@ __global__ __launch_bounds__(kSelectThreads) void k_evict_select(Evict a) {
     // banks) as bits of two words; sequences beyond 63 slots per thread take several rounds.
     int equals = 0;      // of earlier rounds
     int2 moves{0, 0};
-    for (int round = 0; round < len; round += 63 * kSelectThreads) {
-        const int upto = min(len - round, 63 * kSelectThreads);
+    for (int round = 0; round < len; round += kSelectRun * kSelectThreads) {
+        const int upto = min(len - round, kSelectRun * kSelectThreads);
         const int run = ((upto + kSelectThreads - 1) / kSelectThreads) | 1;
         const int t0 = round + min(tid * run, upto), count = min(run, round + upto - t0);
         unsigned long long larger = 0, equal = 0;

@@ -20,6 +20,8 @@ constexpr uint32_t kMaxHeadDim = 256;
 constexpr uint32_t kMaxRotPairs = 128;
 constexpr uint32_t kMaxPageSize = 65536;
 constexpr uint32_t kComputeUnits = 256;  // of an MI355X
+constexpr uint32_t kSlotStep = 65536;    // no kernel's loop over slots steps further, so that slots stay in 32 bits
+constexpr uint32_t kMaxLength = 0x7FFFFFFF - kSlotStep;
 
 // Value d of head h of row r lies at data[r * row_stride + h * head_stride + d] (strides in values).
 struct Rows {

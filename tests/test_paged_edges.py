@@ -1,8 +1,16 @@
 """The paged-cache operators without a GPU, where bounds and handles decide."""
 from __future__ import annotations
 
+import ctypes
 import os
 import subprocess
+
+import pytest
+
+import jetsonfabric_amd as jf
+from jetsonfabric_amd import _capi
+from jetsonfabric_amd._capi import check
+from tests.test_paged import AT, _append, _attend, _evict, _weigh, batch, cache, refused, rows
 
 ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 
@@ -13,3 +21,21 @@ def test_bounds_cpp_tests():
     r = subprocess.run([exe], capture_output=True, text=True, timeout=60)
     assert r.returncode == 0, r.stdout + r.stderr
     assert "paged bounds tests passed" in r.stdout
+
+
+LONGEST = (1 << 31) - 65537  # kernels' loops step by up to 65536 slots in 32 bits
+
+
+@pytest.mark.parametrize("length", [LONGEST + 1, (1 << 31) - 1025, (1 << 31) - 1])
+@pytest.mark.parametrize("call", [_append, _attend, _weigh, _evict])
+def test_lengths_that_a_loop_could_step_out_of_are_refused(call, length):
+    refused(lambda: call(b=batch(table_stride=1 << 28, max_length=length)), "max_length exceeds 2\\^31 - 65537")
+
+
+def test_the_longest_sequences_have_workspaces():
+    lib, need = jf.library(), ctypes.c_size_t()
+    long = batch(n_seq=1, table_stride=1 << 28, max_length=LONGEST)
+    check(lib.jfh_paged_attention_workspace(ctypes.byref(cache()), ctypes.byref(long), ctypes.byref(rows()), ctypes.byref(need)))
+    check(lib.jfh_paged_weigh_workspace(ctypes.byref(cache()), ctypes.byref(long), ctypes.byref(rows()), ctypes.byref(need)))
+    check(lib.jfh_paged_evict_workspace(ctypes.byref(cache()), ctypes.byref(long), 8, ctypes.byref(need)))
+    assert need.value == 4 * (1 + 2 * 8) * 4
