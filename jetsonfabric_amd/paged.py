@@ -100,6 +100,8 @@ class Rope:
 
     @property
     def handle(self) -> ctypes.c_void_p:
+        if not self._h:  # a null handle would be a call without rotation
+            raise _capi.InvalidArgument(1, "the rotation is closed")
         return self._h
 
     def rotate(self, x, positions, out=None):

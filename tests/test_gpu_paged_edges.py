@@ -224,3 +224,17 @@ def test_attention_and_weights_within_bounds(rows, lens, max_rows, max_length, c
     cache.weigh(batch, q.cuda(), given.cuda(), 0.125, causal)
     want, bound = seq.weigh(q, given, 0.125, causal)
     assert ((cache.weights.cpu().double() - want).abs() <= bound).all()
+
+
+# ---------------------------------------------------------------- handles and tensors
+
+def test_a_closed_rotation_appends_nothing():
+    seq = Sequences([3], [20], 2, 64, 16, torch.float16, seed=1)
+    cache, batch, x = step(seq, 4, 3, 20)
+    x, positions, rope = x.cuda(), torch.arange(3, dtype=torch.int32, device="cuda"), jf.Rope(64)
+    rope.close()
+    with pytest.raises(jf.InvalidArgument, match="closed"):
+        cache.append(batch, x[:, :2], x[:, 2:], positions, rope)
+    with pytest.raises(jf.InvalidArgument, match="rotation is required"):
+        rope.rotate(x, positions)
+    assert torch.equal(cache.k.cpu(), seq.k) and torch.equal(cache.v.cpu(), seq.v)

@@ -39,3 +39,15 @@ def test_the_longest_sequences_have_workspaces():
     check(lib.jfh_paged_weigh_workspace(ctypes.byref(cache()), ctypes.byref(long), ctypes.byref(rows()), ctypes.byref(need)))
     check(lib.jfh_paged_evict_workspace(ctypes.byref(cache()), ctypes.byref(long), 8, ctypes.byref(need)))
     assert need.value == 4 * (1 + 2 * 8) * 4
+
+
+def test_a_closed_rotation_has_no_handle():
+    rope = jf.Rope(64)
+    assert rope.handle
+    rope.close()
+    rope.close()
+    with pytest.raises(jf.InvalidArgument, match="closed"):
+        rope.handle
+    x = rows()
+    with pytest.raises(jf.InvalidArgument, match="a rotation is required"):
+        check(jf.library().jfh_rope_rotate(rope._h, ctypes.byref(x), AT, ctypes.byref(x), 0, None))
