@@ -69,6 +69,11 @@ def _stream(device: int) -> int:
     return _current(device)
 
 
+def _kept(i: int, doc: str) -> property:
+    """A tensor whose address a handle has passed on: read-only, since another one would leave the address behind."""
+    return property(lambda self: self._tensors[i], doc=doc)
+
+
 class Rope:
     """Rotary positions (jfh_rope_params): the leading n_rot values of a head turn in pairs,
     (i, i + n_rot / 2) in the "half" layout, (2 i, 2 i + 1) in the "interleaved" one, by position *
@@ -119,15 +124,21 @@ class Rope:
 class PagedBatch:
     """The sequences of a step (jfh_paged_batch), int32 tensors on the cache's GPU: table [sequences,
     pages], lengths [sequences] (slots in use, the new rows included) and row_starts [sequences + 1].
-    max_rows and max_length bound the rows of a sequence and its length."""
+    max_rows and max_length bound the rows of a sequence and its length. The tensors' contents may change
+    between calls, the tensors and their storage may not."""
+
+    table = _kept(0, "int32 [sequences, pages]")
+    lengths = _kept(1, "int32 [sequences]")
+    row_starts = _kept(2, "int32 [sequences + 1]")
+    device = property(lambda self: self._device, doc="ordinal of the GPU")
 
     def __init__(self, table, lengths, row_starts, max_rows: int, max_length: int):
         device = table.get_device()
         if table.dim() != 2:
             raise ValueError("table must be [sequences, pages]")
         n = table.shape[0]
-        self.table, self.lengths, self.row_starts = table, lengths, row_starts
-        self.device = device
+        self._tensors = (table, lengths, row_starts)
+        self._device = device
         self.c = _capi.PagedBatch(_array(table, "table", "int32", device),
                                   _array(lengths, "lengths", "int32", device, (n,)),
                                   _array(row_starts, "row_starts", "int32", device, (n + 1,)), n, table.shape[1],
@@ -139,7 +150,14 @@ class PagedBatch:
 class PagedCache:
     """One layer's K/V cache in pages (jfh_paged_cache): k and v [pages, K/V heads, page size, head
     dim], float16 or bfloat16, of equal strides (a permuted view of another order will do); weights
-    (float32) and positions (int32) [pages, K/V heads, page size], which only a cache that is cut needs."""
+    (float32) and positions (int32) [pages, K/V heads, page size], which only a cache that is cut needs. The
+    tensors' contents may change between calls, the tensors and their storage may not."""
+
+    k = _kept(0, "[pages, K/V heads, page size, head dim]")
+    v = _kept(1, "like k")
+    weights = _kept(2, "float32 [pages, K/V heads, page size] or None")
+    positions = _kept(3, "int32 [pages, K/V heads, page size] or None")
+    device = property(lambda self: self._device, doc="ordinal of the GPU")
 
     def __init__(self, k, v, weights=None, positions=None):
         device = k.get_device()
@@ -151,8 +169,8 @@ class PagedCache:
             raise ValueError("the values of a head must be contiguous")
         pages, heads, page_size, dim = k.shape
         meta = (pages, heads, page_size)
-        self.k, self.v, self.weights, self.positions = k, v, weights, positions
-        self.device = device
+        self._tensors = (k, v, weights, positions)
+        self._device = device
         self.c = _capi.PagedCache(
             k.data_ptr(), v.data_ptr(),
             None if weights is None else _array(weights, "weights", "float32", device, meta),
@@ -162,8 +180,8 @@ class PagedCache:
         self.shape = (heads, dim, page_size)
 
     def _of(self, batch: PagedBatch):
-        if batch.device != self.device:
-            raise ValueError(f"the batch is on GPU {batch.device}, the cache on GPU {self.device}")
+        if batch._device != self._device:
+            raise ValueError(f"the batch is on GPU {batch._device}, the cache on GPU {self._device}")
         return batch.ref
 
     def _workspace(self, batch: PagedBatch, call: str, *args):
@@ -178,16 +196,16 @@ class PagedCache:
             size = batch.workspaces[key] = need.value
         if size == 0:
             return None, 0, None
-        space = _torch().empty(size, dtype=_torch().uint8, device=self.k.device)
+        space = _torch().empty(size, dtype=_torch().uint8, device=self._tensors[0].device)
         return space.data_ptr(), size, space
 
     def append(self, batch: PagedBatch, k, v, positions=None, rope: Rope | None = None) -> None:
         """Writes a step's rows k and v [rows, K/V heads, head dim] at its sequences' last slots, k
         rotated by rope; positions int32 [rows]."""
-        a, b = _rows(k, "k", self.device), _rows(v, "v", self.device)
-        at = None if positions is None else _array(positions, "positions", "int32", self.device, (k.shape[0],))
+        a, b = _rows(k, "k", self._device), _rows(v, "v", self._device)
+        at = None if positions is None else _array(positions, "positions", "int32", self._device, (k.shape[0],))
         check(library().jfh_paged_append(self.ref, self._of(batch), ctypes.byref(a), ctypes.byref(b),
-                                         None if rope is None else rope.handle, at, _stream(self.device)))
+                                         None if rope is None else rope.handle, at, _stream(self._device)))
 
     def attend(self, batch: PagedBatch, q, scale: float | None = None, causal: bool = True, out=None, lse=None):
         """softmax(scale q K^T) V of a step's rows q [rows, heads, head dim] over their sequences' slots
@@ -198,27 +216,27 @@ class PagedCache:
             out = torch.empty_like(q)
         if lse is None:
             lse = torch.empty(q.shape[:2], dtype=torch.float32, device=q.device)
-        a, b = _rows(q, "q", self.device), _rows(out, "out", self.device)
-        at = _array(lse, "lse", "float32", self.device, q.shape[:2])
+        a, b = _rows(q, "q", self._device), _rows(out, "out", self._device)
+        at = _array(lse, "lse", "float32", self._device, q.shape[:2])
         ref = self._of(batch)
         space, size, _held = self._workspace(batch, "attention", a)
         check(library().jfh_paged_attention(self.ref, ref, ctypes.byref(a), a.head_dim ** -0.5 if scale is None else scale,
-                                            int(causal), ctypes.byref(b), at, space, size, _stream(self.device)))
+                                            int(causal), ctypes.byref(b), at, space, size, _stream(self._device)))
         return out, lse
 
     def weigh(self, batch: PagedBatch, q, lse, scale: float | None = None, causal: bool = True) -> None:
         """Adds the attention that the rows q (with attend's lse, scale and causal) give each position to
         the cache's weights."""
-        a = _rows(q, "q", self.device)
-        at = _array(lse, "lse", "float32", self.device, q.shape[:2])
+        a = _rows(q, "q", self._device)
+        at = _array(lse, "lse", "float32", self._device, q.shape[:2])
         ref = self._of(batch)
         space, size, _held = self._workspace(batch, "weigh", a)
         check(library().jfh_paged_weigh(self.ref, ref, ctypes.byref(a), at, a.head_dim ** -0.5 if scale is None else scale,
-                                        int(causal), space, size, _stream(self.device)))
+                                        int(causal), space, size, _stream(self._device)))
 
     def evict(self, batch: PagedBatch, budget: int, n_first: int = 4, n_recent: int = 1) -> None:
         """Cuts every longer sequence to budget slots per K/V head: the positions below n_first, the
         n_recent newest, then the heaviest stay; batch.lengths becomes what is left."""
         ref = self._of(batch)
         space, size, _held = self._workspace(batch, "evict", budget)
-        check(library().jfh_paged_evict(self.ref, ref, budget, n_first, n_recent, space, size, _stream(self.device)))
+        check(library().jfh_paged_evict(self.ref, ref, budget, n_first, n_recent, space, size, _stream(self._device)))

@@ -238,3 +238,15 @@ def test_a_closed_rotation_appends_nothing():
     with pytest.raises(jf.InvalidArgument, match="rotation is required"):
         rope.rotate(x, positions)
     assert torch.equal(cache.k.cpu(), seq.k) and torch.equal(cache.v.cpu(), seq.v)
+
+
+def test_handles_keep_their_tensors():
+    seq = Sequences([2], [20], 2, 64, 16, torch.float16, seed=1)
+    kp, vp, w, pos, table, lengths, starts = seq.to_gpu()
+    cache, batch = jf.PagedCache(kp, vp, w, pos), jf.PagedBatch(table, lengths, starts, 2, 20)
+    assert cache.k is kp and cache.v is vp and cache.weights is w and cache.positions is pos and cache.device == 0
+    assert batch.table is table and batch.lengths is lengths and batch.row_starts is starts and batch.device == 0
+    for handle, name in ((cache, "k"), (cache, "weights"), (batch, "lengths"), (batch, "table")):
+        with pytest.raises(AttributeError):
+            setattr(handle, name, getattr(handle, name).clone())
+    assert jf.PagedCache(kp, vp).weights is None

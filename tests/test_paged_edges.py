@@ -51,3 +51,12 @@ def test_a_closed_rotation_has_no_handle():
     x = rows()
     with pytest.raises(jf.InvalidArgument, match="a rotation is required"):
         check(jf.library().jfh_rope_rotate(rope._h, ctypes.byref(x), AT, ctypes.byref(x), 0, None))
+
+
+@pytest.mark.parametrize("handle,names", [(jf.PagedCache, ("k", "v", "weights", "positions", "device")),
+                                          (jf.PagedBatch, ("table", "lengths", "row_starts", "device"))])
+def test_tensors_of_a_handle_cannot_be_exchanged(handle, names):
+    """A handle has passed their addresses on: another tensor in their place would free them under the kernels."""
+    for name in names:
+        with pytest.raises(AttributeError):
+            setattr(object.__new__(handle), name, None)
