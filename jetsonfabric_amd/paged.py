@@ -2,7 +2,8 @@
 
 ``Rope`` rotates queries and keys; ``PagedCache`` is one layer's cache, whose
 pages, page tables and lengths belong to the caller; ``PagedBatch`` is what a
-step's sequences look like. Every call enqueues its kernels on torch's current
+step's sequences look like. They serve and give no gradients: tensors that
+require one are refused outside torch.no_grad(). Every call enqueues its kernels on torch's current
 stream of the cache's device and returns without waiting. It can be captured
 into a graph, and replayed with other contents of the same tensors.
 """
@@ -32,9 +33,17 @@ def _type(x, name: str) -> int:
     return t
 
 
+def _no_gradient(name: str) -> None:
+    """Of a tensor that requires one."""
+    if _torch().is_grad_enabled():
+        raise ValueError(f"{name} requires a gradient, and these operators give none: call them under torch.no_grad()")
+
+
 def _rows(x, name: str, device: int) -> _capi.Rows:
     """A tensor [rows, heads, head dim] of any strides whose heads are contiguous."""
     shape, stride = x.shape, x.stride()
+    if x.requires_grad:
+        _no_gradient(name)
     if len(shape) != 3:
         raise ValueError(f"{name} must be [rows, heads, head dim]")
     if x.get_device() != device or device < 0:
@@ -50,6 +59,8 @@ def _array(x, name: str, dtype: str, device: int, shape: tuple | None = None) ->
         raise ValueError(f"{name} must be a contiguous {dtype} tensor on GPU {device}")
     if shape is not None and x.shape != shape:
         raise ValueError(f"{name} must have shape {list(shape)}, not {list(x.shape)}")
+    if x.requires_grad:
+        _no_gradient(name)
     return x.data_ptr()
 
 
@@ -167,6 +178,9 @@ class PagedCache:
             raise ValueError("k and v must be on one GPU")
         if k.stride(3) != 1:
             raise ValueError("the values of a head must be contiguous")
+        for x, name in ((k, "k"), (v, "v")):
+            if x.requires_grad:
+                _no_gradient(name)
         pages, heads, page_size, dim = k.shape
         meta = (pages, heads, page_size)
         self._tensors = (k, v, weights, positions)

@@ -250,3 +250,23 @@ def test_handles_keep_their_tensors():
         with pytest.raises(AttributeError):
             setattr(handle, name, getattr(handle, name).clone())
     assert jf.PagedCache(kp, vp).weights is None
+
+
+def test_tensors_that_require_gradients_are_refused():
+    seq = Sequences([2], [20], 2, 64, 16, torch.float16, seed=1)
+    cache, batch, q = step(seq, 4, 2, 20)
+    kp, q, positions = cache.k.clone().requires_grad_(), q.cuda(), torch.zeros(2, dtype=torch.int32, device="cuda")
+    grad = q.clone().requires_grad_()
+    out, lse = cache.attend(batch, q)
+    calls = [("x", lambda: jf.Rope(64).rotate(grad, positions)), ("out", lambda: jf.Rope(64).rotate(q, positions, out=grad)),
+             ("k", lambda: cache.append(batch, grad[:, :2], q[:, 2:], positions)),
+             ("v", lambda: cache.append(batch, q[:, :2], grad[:, 2:], positions)),
+             ("q", lambda: cache.attend(batch, grad)), ("lse", lambda: cache.attend(batch, q, lse=lse.clone().requires_grad_())),
+             ("q", lambda: cache.weigh(batch, grad, lse)), ("k", lambda: jf.PagedCache(kp, cache.v)),
+             ("v", lambda: jf.PagedCache(cache.k, kp))]
+    for name, call in calls:
+        with pytest.raises(ValueError, match=f"{name} requires a gradient"):
+            call()
+    with torch.no_grad():
+        again, _ = cache.attend(batch, grad)
+    assert torch.equal(again, out)

@@ -60,3 +60,16 @@ def test_tensors_of_a_handle_cannot_be_exchanged(handle, names):
     for name in names:
         with pytest.raises(AttributeError):
             setattr(object.__new__(handle), name, None)
+
+
+def test_tensors_that_require_gradients_are_refused():
+    """No operator has a backward pass: a gradient would be lost without a word."""
+    import torch
+
+    x, positions = torch.zeros(2, 1, 64, requires_grad=True), torch.zeros(2, dtype=torch.int32)
+    with pytest.raises(ValueError, match="x requires a gradient"):
+        jf.Rope(64).rotate(x, positions)
+    with torch.no_grad(), pytest.raises(ValueError, match="on GPU"):  # as any tensor
+        jf.Rope(64).rotate(x, positions)
+    with pytest.raises(ValueError, match="out requires a gradient|on GPU"):
+        jf.Rope(64).rotate(x.detach(), positions, out=x)
