@@ -33,6 +33,13 @@ def _type(x, name: str) -> int:
     return t
 
 
+def _count(v: int, name: str) -> int:
+    """A number for a C uint32_t, which ctypes would cut to its low 32 bits."""
+    if not 0 <= v <= 0xFFFFFFFF:
+        raise _capi.InvalidArgument(1, f"{name} must be 0 to 2^32 - 1, not {v}")
+    return v
+
+
 def _no_gradient(name: str) -> None:
     """Of a tensor that requires one."""
     if _torch().is_grad_enabled():
@@ -99,8 +106,9 @@ class Rope:
             raise ValueError(f"layout must be one of {sorted(_LAYOUTS)}")
         if scaling not in _SCALINGS:
             raise ValueError(f"scaling must be one of {sorted(_SCALINGS)}")
-        params = _capi.RopeParams(n_rot, _LAYOUTS[layout], _SCALINGS[scaling], original_context, base, factor, beta_fast,
-                                  beta_slow, attention_factor)
+        params = _capi.RopeParams(_count(n_rot, "n_rot"), _LAYOUTS[layout], _SCALINGS[scaling],
+                                  _count(original_context, "original_context"), base, factor, beta_fast, beta_slow,
+                                  attention_factor)
         check(library().jfh_rope_create(ctypes.byref(params), ctypes.byref(self._h)))
 
     def close(self) -> None:
@@ -153,7 +161,7 @@ class PagedBatch:
         self.c = _capi.PagedBatch(_array(table, "table", "int32", device),
                                   _array(lengths, "lengths", "int32", device, (n,)),
                                   _array(row_starts, "row_starts", "int32", device, (n + 1,)), n, table.shape[1],
-                                  max_rows, max_length)
+                                  _count(max_rows, "max_rows"), _count(max_length, "max_length"))
         self.workspaces: dict = {}
         self.ref = ctypes.byref(self.c)
 
@@ -251,6 +259,8 @@ class PagedCache:
     def evict(self, batch: PagedBatch, budget: int, n_first: int = 4, n_recent: int = 1) -> None:
         """Cuts every longer sequence to budget slots per K/V head: the positions below n_first, the
         n_recent newest, then the heaviest stay; batch.lengths becomes what is left."""
+        budget = _count(budget, "budget")
         ref = self._of(batch)
         space, size, _held = self._workspace(batch, "evict", budget)
-        check(library().jfh_paged_evict(self.ref, ref, budget, n_first, n_recent, space, size, _stream(self._device)))
+        check(library().jfh_paged_evict(self.ref, ref, budget, _count(n_first, "n_first"), _count(n_recent, "n_recent"), space,
+                                        size, _stream(self._device)))

@@ -270,3 +270,18 @@ def test_tensors_that_require_gradients_are_refused():
     with torch.no_grad():
         again, _ = cache.attend(batch, grad)
     assert torch.equal(again, out)
+
+
+def test_numbers_beyond_32_bits_are_refused_not_cut():
+    seq = Sequences([0], [40], 2, 64, 16, torch.float16, seed=1)
+    cache, batch, _ = step(seq, 4, 1, 40)
+    far = 1 << 32
+    for args in ((far + 20,), (20 - far,), (20, far + 4), (20, 4, far + 1), (20, -1), (-5,)):
+        with pytest.raises(jf.InvalidArgument, match="must be 0 to"):
+            cache.evict(batch, *args)
+    assert batch.lengths.tolist() == [40]
+    for rows, length in ((far + 1, 40), (1, far + 40), (-1, 40), (1, -1)):
+        with pytest.raises(jf.InvalidArgument, match="must be 0 to"):
+            jf.PagedBatch(batch.table, batch.lengths, batch.row_starts, rows, length)
+    cache.evict(batch, 20)
+    assert batch.lengths.tolist() == [20]

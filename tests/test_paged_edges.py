@@ -73,3 +73,9 @@ def test_tensors_that_require_gradients_are_refused():
         jf.Rope(64).rotate(x, positions)
     with pytest.raises(ValueError, match="out requires a gradient|on GPU"):
         jf.Rope(64).rotate(x.detach(), positions, out=x)
+
+
+@pytest.mark.parametrize("kw", [{"n_rot": (1 << 32) + 64}, {"n_rot": -64}, {"original_context": (1 << 32) + 4096}, {"n_rot": 64 - (1 << 32)}])
+def test_numbers_beyond_32_bits_are_refused_not_cut(kw):
+    with pytest.raises(jf.InvalidArgument, match="must be 0 to 2\\^32 - 1"):
+        jf.Rope(**{"n_rot": 64, "scaling": "yarn", "factor": 2.0, **kw})
