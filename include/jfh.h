@@ -398,7 +398,8 @@ jfh_status jfh_engine_profile_batch(jfh_engine * engine, jfh_session * const * s
 typedef enum jfh_value_type { JFH_VALUE_F32 = 1, JFH_VALUE_F16 = 2, JFH_VALUE_BF16 = 3 } jfh_value_type;
 
 /* Rows of heads: value d of head h of row r at data[r * row_stride +
- * h * head_stride + d], strides in values. */
+ * h * head_stride + d], strides in values. Those of rows that a call reads may
+ * be anything, 0 included; rows that it writes must not overlap each other. */
 typedef struct jfh_rows {
     void * data;
     int64_t row_stride;

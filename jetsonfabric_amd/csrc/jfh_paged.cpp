@@ -62,6 +62,20 @@ paged::Rows rows_of(const jfh_rows* x, const char* name) {
     return paged::Rows{x->data, x->row_stride, x->head_stride, x->n_rows, x->n_head, x->head_dim, x->type};
 }
 
+// Rows that a call writes: each value has a place of its own, and the rows of the input are others or the same ones.
+void written(const paged::Rows& x, const paged::Rows& out, const char* name) {
+    const std::string n = name;
+    // the larger stride passes over all that the smaller one reaches
+    const bool by_rows = out.row_stride >= out.head_stride;
+    const int64_t small = by_rows ? out.head_stride : out.row_stride, large = by_rows ? out.row_stride : out.head_stride;
+    const int64_t inner = by_rows ? out.heads : out.rows, outer = by_rows ? out.rows : out.heads;
+    const int64_t reach = static_cast<int64_t>(std::min<uint64_t>(static_cast<uint64_t>(small), 1ULL << 31)) * (inner - 1);
+    require((inner <= 1 || small >= out.head_dim) && (outer <= 1 || large >= (inner <= 1 ? 0 : reach) + out.head_dim),
+            n + "'s strides let its rows overlap");
+    require(x.data != out.data || (x.type == out.type && x.row_stride == out.row_stride && x.head_stride == out.head_stride),
+            "rows written in place must keep their type and strides");
+}
+
 paged::Cache cache_of(const jfh_paged_cache* c) {
     require(c != nullptr, "a cache is required");
     require(c->k && c->v && aligned(c->k, 16) && aligned(c->v, 16), "the cache's k and v must be 16-byte aligned");
@@ -221,10 +235,8 @@ jfh_status jfh_rope_rotate(const jfh_rope* rope, const jfh_rows* x, const int32_
         require(in.rows == out.rows && in.heads == out.heads && in.head_dim == out.head_dim,
                 "x and y must have the same rows, heads and head dim");
         require(rope->rotation.n_rot <= in.head_dim, "the rotation turns more values than a head has");
-        require(in.data != out.data || (in.type == out.type && in.row_stride == out.row_stride &&
-                                        in.head_stride == out.head_stride),
-                "rows rotated in place must keep their type and strides");
         if (in.rows == 0) return;
+        written(in, out, "y");
         require(positions != nullptr && aligned(positions, 4), "positions are required");
         const OnDevice guard(device);
         check(paged::launch_rotate(rope->rotation, in, positions, out, static_cast<hipStream_t>(stream)), "rotate rows");
@@ -272,6 +284,7 @@ jfh_status jfh_paged_attention(const jfh_paged_cache* cache, const jfh_paged_bat
         a.batch = batch_of(batch, *cache, true, a.q.rows);
         a.out = attended(out, a.cache, "out");
         require(a.q.rows == a.out.rows && a.q.heads == a.out.heads, "q and out must have the same rows and heads");
+        if (a.q.rows > 0) written(a.q, a.out, "out");
         require(aligned(lse, 4), "lse must be aligned");
         a.lse = lse;
         a.scale_log2 = score_scale(scale);

@@ -79,3 +79,28 @@ def test_tensors_that_require_gradients_are_refused():
 def test_numbers_beyond_32_bits_are_refused_not_cut(kw):
     with pytest.raises(jf.InvalidArgument, match="must be 0 to 2\\^32 - 1"):
         jf.Rope(**{"n_rot": 64, "scaling": "yarn", "factor": 2.0, **kw})
+
+
+@pytest.mark.parametrize("change", [{"row_stride": 0}, {"head_stride": 0}, {"row_stride": 0, "head_stride": 0}, {"head_stride": 56},
+                                    {"row_stride": 64}, {"row_stride": 248}, {"row_stride": 64, "head_stride": 128}])
+def test_rows_that_overlap_are_not_written(change):
+    """Three rows of four heads of 64 values; an expanded tensor has stride 0."""
+    out = rows(data=AT + (1 << 16), **change)
+    refused(lambda: _attend(out=out), "out's strides let its rows overlap")
+    x = rows()
+    call = lambda: jf.library().jfh_rope_rotate(jf.Rope(64).handle, ctypes.byref(x), AT, ctypes.byref(out), 0, None)  # noqa: E731
+    refused(call, "y's strides let its rows overlap")
+
+
+@pytest.mark.parametrize("change", [{"row_stride": 512}, {"row_stride": 64, "head_stride": 192}])
+def test_attention_in_place_keeps_its_strides(change):
+    refused(lambda: _attend(out=rows(**change)), "in place must keep")
+
+
+@pytest.mark.parametrize("change", [{}, {"row_stride": 64, "head_stride": 192}, {"row_stride": 64, "head_stride": 256},
+                                    {"row_stride": 1 << 40}, {"head_stride": 64, "row_stride": 264},
+                                    {"n_rows": 1, "row_stride": 0}, {"n_head": 4, "n_rows": 1, "row_stride": 8}])
+def test_other_layouts_of_rows_are_written(change):
+    """Not refused for their layout: the next check, of the workspace's size, is."""
+    long = {"b": batch(n_seq=1, table_stride=4096, max_length=65536), "space": None}
+    refused(lambda: _attend(q=rows(n_rows=change.get("n_rows", 3)), out=rows(data=AT + (1 << 16), **change), **long), "bytes of workspace")
