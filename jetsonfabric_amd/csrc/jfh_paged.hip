@@ -1101,11 +1101,19 @@ __device__ __forceinline__ void weighed_rows(const Weigh& a, uint32_t s, uint32_
     }
 }
 
+// A query's lse in base 2 and 2^-(what its rounding left), which goes into the sums: without it every weight of the query
+// has the rounding's error, 2^-24 of an lse that may be large.
+__device__ __forceinline__ float2 lse_base2(float lse) {
+    constexpr float kLog2eRest = 1.92596303e-8F;  // log2(e) - kLog2e
+    const float ref = lse * kLog2e, rest = fmaf(lse, kLog2eRest, fmaf(lse, kLog2e, -ref));
+    return float2{ref, fabsf(lse) < INFINITY ? exp2f(-rest) : 1.0F};
+}
+
 // sum += the weights of 16 queries (lane i's: its lse in base 2, the slots it sees) for the wave's slots from `base`. All
 // seen: every query sees every one of the slots.
 template <typename T, bool ALL_SEEN, int U, int KC>
 __device__ __forceinline__ void weigh_queries(const Weigh& a, int base, const typename Values<T>::v8 (&k)[U][KC],
-                                              const typename Values<T>::v8 (&q)[KC], float ref, int limit, float4v (&sum)[U]) {
+                                              const typename Values<T>::v8 (&q)[KC], float2 ref, int limit, float4v (&sum)[U]) {
     const int g = threadIdx.x % 64 / 16;
     float4v sc[U];
 #pragma unroll
@@ -1119,8 +1127,8 @@ __device__ __forceinline__ void weigh_queries(const Weigh& a, int base, const ty
     for (int u = 0; u < U; ++u) {
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const float p = __builtin_amdgcn_exp2f(fmaf(sc[u][r], a.scale_log2, -ref));
-            sum[u][r] += ALL_SEEN || base + 16 * u + 4 * g + r < limit ? p : 0.0F;
+            const float p = __builtin_amdgcn_exp2f(fmaf(sc[u][r], a.scale_log2, -ref.x));
+            sum[u][r] = fmaf(ALL_SEEN || base + 16 * u + 4 * g + r < limit ? p : 0.0F, ref.y, sum[u][r]);
         }
     }
 }
@@ -1157,7 +1165,7 @@ __global__ __launch_bounds__(kWeighThreads) void k_weigh_few(Weigh a, int group,
         const float lse = a.lse[row * a.q.heads + query.head];
         // a row that saw nothing adds nothing
         const int limit = m0 + i >= queries || lse == -INFINITY ? 0 : a.causal ? slots_seen(span, query.row) : span.len;
-        weigh_queries<T, false>(a, base, k, q, lse * kLog2e, limit, sum);
+        weigh_queries<T, false>(a, base, k, q, lse_base2(lse), limit, sum);
     }
 #pragma unroll
     for (int u = 0; u < U; ++u) {
@@ -1183,7 +1191,7 @@ __global__ __launch_bounds__(kWeighThreads, 2) void k_weigh_many(Weigh a, int gr
     using v8 = typename Values<T>::v8;
     constexpr int KC = HDP / 32, U = kWeighTiles<HDP>, CH = HDP / 8, QS = CH + 1, QT = 64, KP = QT * CH / kWeighThreads;
     __shared__ uint4 q_lds[2][QT * QS];
-    __shared__ float refs[2][QT];
+    __shared__ float2 refs[2][QT];
     __shared__ int limits[2][QT];
     const int tid = threadIdx.x, lane = tid % 64, wave = tid / 64;
     const int i = lane % 16, g = lane / 16;
@@ -1236,7 +1244,7 @@ __global__ __launch_bounds__(kWeighThreads, 2) void k_weigh_many(Weigh a, int gr
             const float lse = a.lse[(span.row0 + query.row) * static_cast<int64_t>(a.q.heads) + query.head];
             // a row that saw nothing adds nothing
             limits[b][tid] = m >= queries || lse == -INFINITY ? 0 : a.causal ? slots_seen(span, query.row) : span.len;
-            refs[b][tid] = lse * kLog2e;
+            refs[b][tid] = lse_base2(lse);
         }
     };
 

@@ -285,3 +285,42 @@ def test_numbers_beyond_32_bits_are_refused_not_cut():
             jf.PagedBatch(batch.table, batch.lengths, batch.row_starts, rows, length)
     cache.evict(batch, 20)
     assert batch.lengths.tolist() == [20]
+
+
+# ---------------------------------------------------------------- attention weights
+
+@pytest.mark.parametrize("max_rows", [1, 100])
+@pytest.mark.parametrize("low", [-40.0, 12.0, 60.0])
+def test_weights_keep_the_bits_of_lse(max_rows, low):
+    """Scores of 0: each slot gets exp(-lse) of its sequence's one row, in either form."""
+    n = 100
+    seq = Sequences([1] * n, [1] * n, 1, 64, 1, torch.float16, seed=1)
+    seq.k.zero_()
+    seq.weights.zero_()
+    cache, batch, q = step(seq, 1, max_rows, 1)
+    lse = torch.rand(n, 1, generator=torch.Generator().manual_seed(3)) * 20 + low
+    cache.weigh(batch, q.cuda(), lse.cuda())
+    got = torch.stack([cache.weights[seq.slot(s, 0)[0], 0, 0] for s in range(n)]).cpu().double()
+    want = torch.exp(-lse[:, 0].double())
+    # the lse's two parts leave 2^-48 of it, exp2 is off by 2^-23, the factor of the second part and the sum by 2^-24 each
+    off = ((got - want) / want).abs().max().item()
+    assert off <= 2.0**-22, off
+
+
+def test_weights_of_rows_without_a_finite_lse():
+    """-inf: the row saw nothing and adds nothing; inf: its weights are 0; NaN: what it sees becomes NaN, nothing else."""
+    for rows, heads in ((5, 2), (70, 2)):
+        seq = Sequences([rows], [rows + 9], 1, 64, 16, torch.float16, seed=2)
+        cache, batch, q = step(seq, heads, rows, rows + 9)
+        lse = seq.attend(q, 0.125)[1].float()
+        lse[1, 0], lse[2, 1] = -math.inf, math.inf
+        some = lse.clone()
+        some[2, 1] = -math.inf  # adds as little
+        want, bound = seq.weigh(q, some, 0.125)
+        cache.weigh(batch, q.cuda(), lse.cuda(), 0.125)
+        assert ((cache.weights.cpu().double() - want).abs() <= bound).all()
+        lse[3, 1] = math.nan
+        cache.weigh(batch, q.cuda(), lse.cuda(), 0.125)
+        for t in range(rows + 9):
+            page, i = seq.slot(0, t)
+            assert torch.isnan(cache.weights[page, 0, i]).item() == (t <= 9 + 3)
