@@ -324,3 +324,69 @@ def test_weights_of_rows_without_a_finite_lse():
         for t in range(rows + 9):
             page, i = seq.slot(0, t)
             assert torch.isnan(cache.weights[page, 0, i]).item() == (t <= 9 + 3)
+
+
+# ---------------------------------------------------------------- every slot
+
+@pytest.mark.parametrize("rows,heads,length,dim,room", [
+    (1, 16, 40000, 64, 0), (1, 4, 2049, 128, 0), (4, 4, 5000, 72, 0), (2, 8, 4097, 200, 0), (1, 16, 3000, 256, 0),
+    (2, 16, 9000, 128, 1 << 15), (40, 2, 6001, 64, 0), (9, 5, 4096, 128, 0), (33, 4, 20000, 96, 0), (20, 2, 2500, 256, 0),
+    (300, 1, 3000, 128, 0), (130, 7, 257, 136, 0)])
+@pytest.mark.parametrize("kind", ["f16", "bf16"])
+def test_every_slot_is_seen_once(rows, heads, length, dim, room, kind):
+    """Keys of random signs, each row's query one of the keys that it sees: that slot takes all weight, so a slot that is
+    lost, or counted twice, at any seam of tiles, waves, parts or the causal end shows at once."""
+    seq = Sequences([rows], [length], 1, dim, 16, TYPES[kind], seed=dim)
+    g = torch.Generator().manual_seed(5)
+    seq.k = (torch.randint(0, 2, seq.k.shape, generator=g) * 2 - 1).to(seq.dtype)
+    kp, vp, _, _, table, lengths, starts = seq.to_gpu()
+    slots = torch.arange(length, device="cuda")
+    page, place = table[0, slots // 16].long(), slots % 16
+    k, v = kp[page, 0, place], vp[page, 0, place]
+    wide = torch.cat([table, torch.full((1, room), -1, dtype=torch.int32, device="cuda")], 1)
+    cache = jf.PagedCache(kp, vp)
+    batch = jf.PagedBatch(wide, lengths, starts, rows, wide.shape[1] * 16 if room else length)
+    scale = 192.0 / dim  # a score of 192
+    sees = length - rows + 1 + torch.arange(rows, device="cuda")[:, None]
+    query = torch.arange(rows * heads, device="cuda").reshape(rows, heads)
+    some = min(2000, length)
+    most = (k.float()[:some] @ k.float().T - 2 * dim * torch.eye(some, length, device="cuda")).max().item()
+    assert (dim - most) * scale > 40  # others' weights are below e^-40 each
+    for call in range(-(-length // (rows * heads))):
+        target = (query + call * rows * heads) % sees
+        out, lse = cache.attend(batch, k[target], scale)
+        assert torch.equal(out, v[target]), call
+        # a second count of the slot would add ln 2; the score and its logarithm keep 2^-22 of 192
+        assert (lse - 192.0).abs().max() < 1e-3
+    if rows > 1:  # the slot behind a row's own is not seen
+        target = torch.cat([sees[:-1], sees[:1] - 1]).expand(rows, heads)
+        out, lse = cache.attend(batch, k[target], scale)
+        assert (lse[:-1] < 192 - 40).all() and (lse[-1] - 192.0).abs().max() < 1e-3
+        assert torch.isfinite(out.float()).all()
+
+
+def test_threads_share_a_batch():
+    """Four threads, each on a stream of its own, with one cache and one batch."""
+    import threading
+
+    seq = Sequences([1, 3], [5000, 700], 2, 64, 16, torch.float16, seed=4)
+    cache, batch, q = step(seq, 8, 3, 5000)
+    queries = [normal(4, 8, 64, seed=50 + n).half().cuda() for n in range(4)]
+    want = [cache.attend(batch, x)[0] for x in queries]
+    torch.cuda.synchronize()
+    failed = []
+
+    def run(n):
+        stream = torch.cuda.Stream()
+        with torch.cuda.stream(stream):
+            got = [cache.attend(batch, queries[n])[0] for _ in range(50)]
+        stream.synchronize()
+        if not all(torch.equal(x, want[n]) for x in got):
+            failed.append(n)
+
+    threads = [threading.Thread(target=run, args=(n,)) for n in range(4)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    assert not failed
