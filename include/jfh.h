@@ -383,8 +383,9 @@ jfh_status jfh_engine_profile_batch(jfh_engine * engine, jfh_session * const * s
  * that keeps its K/V caches in pages (no counterpart in the reference, whose
  * sessions own one contiguous cache each): rotary positions, new rows written
  * into the pages, attention over them, and caches cut back to a budget by the
- * attention that their positions have had. They stand next to
- * jfh_engine_matmul_noalloc, which gives such code the weight products.
+ * attention that their positions have had. jfh_engine_matmul_noalloc can give
+ * such code the weight products, outside a captured step; sessions and
+ * generation do not use these operators.
  *
  * Every call checks its arguments, enqueues kernels on the caller's stream
  * (hipStream_t; NULL: the null stream) of `device` and returns without
@@ -546,7 +547,8 @@ jfh_status jfh_paged_weigh(const jfh_paged_cache * cache, const jfh_paged_batch 
  * order, with their weights and positions; nothing else moves, and lengths
  * become `budget`. Slots on absent pages are never moved to or from. The cache
  * needs weights and positions; no two sequences may share a page; the batch's
- * row_starts and max_rows are not used (row_starts may be NULL). Keys keep the
+ * row_starts and max_rows are not used (row_starts may be NULL). What a
+ * sequence has from max_length on is left out, and gone with a cut. Keys keep the
  * rotation of their positions, so that new rows go on at the positions of the
  * text. workspace as for jfh_paged_attention. */
 jfh_status jfh_paged_evict_workspace(const jfh_paged_cache * cache, const jfh_paged_batch * batch, uint32_t budget,

@@ -357,8 +357,9 @@ __device__ __forceinline__ Query query_of(int m, int group, uint32_t kv_head) {
 // rounding of the first left, so that the one rounding that counts is the output's: the bytes bound the call, and the
 // second product costs it 0 to 2 % (eight rows over up to 32701 positions, bf16: 104 us, error against 64 bits 1.66e-3,
 // with P rounded once 104 us and 1.77e-3; head dim 64, f16, 30000: 37.3 us and 2.03e-4, 36.6 and 2.18e-4).
-// Eight rows of 40 heads over 4087 to 32701 positions, bf16: 100 us and 5 for the join, 5.8 TB/s of K and V; one row over
-// 257: 11.7 us, the latency of its dependent loads.
+// Eight rows of 40 heads over 4087 to 32701 positions, bf16: 102 us and 5 for the join, 5.8 TB/s of K and V; one row over
+// 257: 10.9 us, latency. Head dims above 128 take 285 registers, one wave per SIMD: eight sequences of 30000 positions, 4
+// heads of one K/V head of 256, 58 us, 4.2 TB/s.
 constexpr int kFewKeys = 32;  // keys of a wave's tile
 template <int HDP> constexpr int kFewWaves = HDP <= 128 ? 8 : 4;
 
@@ -426,9 +427,11 @@ __global__ __launch_bounds__(64 * kFewWaves<HDP>) void k_attend_few(Attend a, in
             }
         }
     };
-    // V is read once, so where a load takes whole rows of 256 bytes it leaves nothing in the caches: eight sequences of
-    // 30000 positions 87 us, 95 through them; of 4000, which stay in the caches from call to call, 22.6 and 22.0. Loads of
-    // parts of rows (K's, and V's of other head dims) lose what the neighbouring loads find there (27.0 and 29.6 us).
+    // V is read once where sequences share no pages, so a load of a lane's 16 bytes of whole rows (head dims 65 to 128)
+    // leaves nothing in the caches. Eight sequences of 30000 positions, 40 heads: head dim 128 161 us, 176 through them;
+    // 96 137 and 140; 72 125 and 119; 128 with all pages shared 107 and 101. Of 8000, which stay in the caches from call to
+    // call, 23.6 and 23.1. Loads of parts of rows (K's, and V's of other head dims) lose what the neighbouring loads find
+    // there (27.0 and 29.6 us).
     typedef uint32_t Words __attribute__((ext_vector_type(kChunk)));
     const auto fetch_v = [&](const Keys& keys) {
 #pragma unroll
@@ -703,7 +706,8 @@ __global__ __launch_bounds__(64 * kFewWaves<HDP>) void k_attend_few(Attend a, in
 // form, and a second one for what the rounding leaves takes 2048 rows over 8192 positions of 7B heads from 280 to 368 us
 // (f16: error against 64 bits 2.5e-4, with the second product 2.1e-4, of which the output's own rounding is nearly all).
 // 2048 rows of 28 heads over 8192 positions of 4 K/V heads of 128 values, f16:
-// 270 us, 780 TFLOP/s; products and the softmax's instructions share the time, 36 % and 45 % of a SIMD's cycles.
+// 272 us, 780 TFLOP/s; products and the softmax's instructions share the time, 36 % and about half of a SIMD's cycles.
+// Head dims above 128: 325 registers, one wave per SIMD.
 constexpr int kTileThreads = 256;
 constexpr int kTileWaves = kTileThreads / 64;
 constexpr int kTileQueries = 32 * kTileWaves;
@@ -1183,7 +1187,7 @@ __global__ __launch_bounds__(kWeighThreads) void k_weigh_few(Weigh a, int group,
 // Many queries: products and exponentials bound the call, after the traffic of Q, which every work-group reads for its
 // slots. So a work-group has 256 slots (128 of wide heads) and stages 64 queries at a time in LDS for its four waves,
 // double-buffered; where that leaves the chip idle, the queries are divided into `splits` parts, whose sums go to the
-// workspace and are added in order. 1777 rows of 28 heads over 3999 positions: 76 us and 4 for the sum, 500 TFLOP/s.
+// workspace and are added in order. 1777 rows of 28 heads over 3999 positions: 77 us and 4 for the sum, 500 TFLOP/s.
 template <int HDP> constexpr int kWeighTiles = HDP <= 128 ? 4 : 2;  // 16-slot tiles of a wave
 
 template <typename T, int HDP>
