@@ -390,3 +390,36 @@ def test_threads_share_a_batch():
     for t in threads:
         t.join()
     assert not failed
+
+
+@pytest.mark.parametrize("heads,kv", [(100, 1), (71, 1), (130, 2)])
+@pytest.mark.parametrize("rows,lens", [([1, 1], [300, 40]), ([3, 70], [300, 90])])
+def test_more_heads_of_a_kv_head_than_a_tile_of_queries(heads, kv, rows, lens):
+    """A row's heads span tiles: 64 queries of the weights, 128 and 32 of attention."""
+    seq = Sequences(rows, lens, kv, 64, 16, torch.float16, seed=heads)
+    cache, batch, q = step(seq, heads, seq.max_rows, seq.max_length)
+    want, want_lse, bound, lse_bound = seq.attend(q, 0.125)
+    out, lse = cache.attend(batch, q.cuda(), 0.125)
+    assert ((out.cpu().double() - want).abs() <= bound).all()
+    assert ((lse.cpu().double() - want_lse).abs() <= lse_bound).all()
+    cache.weigh(batch, q.cuda(), lse, 0.125)
+    want, bound = seq.weigh(q, lse.cpu(), 0.125)
+    assert ((cache.weights.cpu().double() - want).abs() <= bound).all()
+
+
+def test_expanded_rows_are_read():
+    """One row for all, one head for all: stride 0 in what a call reads."""
+    seq = Sequences([4], [50], 2, 64, 16, torch.float16, seed=6)
+    cache, batch, x = step(seq, 4, 4, 50)
+    one = x[:1, :1].expand(4, 4, 64)
+    want, _, bound, _ = seq.attend(one, 0.125)
+    out, _ = cache.attend(batch, x.cuda()[:1, :1].expand(4, 4, 64), 0.125)
+    assert ((out.cpu().double() - want).abs() <= bound).all()
+    gpu, positions = x.cuda(), torch.arange(46, 50, dtype=torch.int32, device="cuda")
+    rope = jf.Rope(64)
+    wide = rope.rotate(gpu[:1, :1].expand(4, 2, 64), positions)
+    assert torch.equal(wide, rope.rotate(gpu[:1, :1].expand(4, 2, 64).contiguous(), positions))
+    cache.append(batch, gpu[:1, :1].expand(4, 2, 64), gpu[:, :1].expand(4, 2, 64), positions, rope)
+    for i in range(4):
+        page, place = seq.slot(0, 46 + i)
+        assert torch.equal(cache.k[page, :, place], wide[i]) and torch.equal(cache.v[page, :, place], gpu[i, :1].expand(2, 64))
